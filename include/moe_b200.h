@@ -563,6 +563,78 @@ int moe_ds_attention_block_forward_f32(void* handle, const float* hidden_in, con
                                        int64_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------
+ * Batched operators in front of the MoE layer (no reference counterpart: the
+ * reference's attention block takes one fp32 token and a contiguous cache).
+ * The steps of a DeepSeek-V3 attention block for a batch of tokens: 8-bit rows
+ * for the FP8 linears, those linears with e4m3 activations, a paged latent
+ * cache and the attention that reads it.  dtype codes: 0 fp32, 1 bf16, 2 fp16.
+ * Strides are in elements, the innermost dimension is contiguous, outputs do
+ * not overlap inputs.  Inference only.
+ * ------------------------------------------------------------------------- */
+
+/* h = x + residual rounded to x's type (h = x without a residual; written to
+ * residual_out [rows, cols] with one); y = h / sqrt(mean(h^2) + eps) * weight
+ * in fp32; for each group of 128 columns scales[row, g] = max(amax |y|,
+ * 2^-100) / 448 ([rows, ceil(cols / 128)]) and codes = e4m3(y / scale), to
+ * nearest even.  normed_out (may be NULL): y in x's type.  weight of x's type
+ * or fp32; cols <= 32768.  A NaN makes its row's scales and codes NaN. */
+int moe_rmsnorm_fp8(const void* x, int64_t x_stride, int x_dtype, const void* residual, int64_t residual_stride,
+                    const void* weight, int weight_dtype, int64_t rows, int64_t cols, float eps, uint8_t* codes,
+                    int64_t codes_stride, float* scales, void* residual_out, void* normed_out, void* stream);
+/* The same codes and scales of x's rows as they are. */
+int moe_fp8_quantize_rows(const void* x, int64_t x_stride, int x_dtype, int64_t rows, int64_t cols, uint8_t* codes,
+                          int64_t codes_stride, float* scales, void* stream);
+
+/* out[t, n] = sum_g x_scales[t, g] scale_inv[n / 128, g] sum_{k in group g}
+ * x[t, k] w[n, k]: e4m3 codes on both sides (x [rows, in_cols] with a scale
+ * per 128 columns, the weight [out_rows, in_cols] with 128 x 128 block
+ * scales), products and sums in fp32, one rounding to out_dtype.  Code rows
+ * start on 16-byte boundaries.  Unlike the fp32-activation linears above, the
+ * codes 0x7F / 0xFF are NaN here, as e4m3 defines them. */
+int moe_fp8_block_linear(const uint8_t* x_codes, int64_t x_stride, const float* x_scales, const uint8_t* fp8_weight,
+                         int64_t weight_stride, const float* scale_inv, int64_t rows, int64_t out_rows,
+                         int64_t in_cols, void* out, int out_dtype, void* stream);
+
+/* Token t's cache row [RMSNorm(kv[:kv_lora_rank]) * kv_norm_weight,
+ * rot(kv[kv_lora_rank:], positions[t])] to slot slots[t] = page * page_size +
+ * offset of cache [pages, page_size, kv_lora_rank + qk_rope_dim] (bf16 or
+ * fp16); rot turns the pairs (2p, 2p + 1) by rope_cos / rope_sin [table_rows,
+ * qk_rope_dim / 2] at the position.  A negative slot stores no row.  With
+ * q_pe [tokens, heads, qk_rope_dim] (the cache's type) its rotation goes to
+ * q_out (contiguous).  kv_rows and the norm weight are of the cache's type or
+ * fp32.  A slot past the cache, or a row to store whose position is outside
+ * the tables, is skipped and sets code 512 in moe_b200_device_error; queries
+ * of such a position are written as zeros.  The slots of one call are
+ * distinct (a slot given twice is left with an unspecified row). */
+int moe_paged_mla_append(const void* kv_rows, int64_t kv_stride, int kv_dtype, const void* kv_norm_weight,
+                         int norm_dtype, const int64_t* slots, const int64_t* positions, const float* rope_cos,
+                         const float* rope_sin, int64_t table_rows, void* cache, int cache_dtype, int64_t pages,
+                         int64_t page_size, int64_t page_stride, int64_t row_stride, const void* q_pe,
+                         int64_t q_stride, int64_t q_head_stride, int64_t heads, void* q_out, int64_t tokens,
+                         int64_t kv_lora_rank, int64_t qk_rope_dim, float rms_eps, void* stream);
+
+/* One query token per row b over the first lengths[b] positions of its pages
+ * (position l in page page_table[b, l / page_size]): score = softmax_scale *
+ * (q_latent . latent + q_pe . rope part), out [batch, heads, kv_lora_rank]
+ * (contiguous, the cache's type) = softmax(score) . latent, lse (may be NULL)
+ * fp32 [batch, heads] = log(sum exp(score)).  A row of length <= 0 gives
+ * zeros and -inf.  Several tokens of one sequence (a verify batch) are rows
+ * that share a table row with lengths one apart.  Table entries at and past a
+ * row's last page are not read.  A page outside [0, pages) or a length past
+ * the table is skipped and sets code 512 in moe_b200_device_error.
+ * kv_lora_rank <= 512 and qk_rope_dim <= 64, both multiples of 8; rows of
+ * queries and cache start on 16-byte boundaries; batch <= 65535.  workspace:
+ * moe_paged_mla_attention_workspace_bytes (-1 for dimensions it rejects). */
+int64_t moe_paged_mla_attention_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_lora_rank,
+                                                int64_t qk_rope_dim, int64_t table_cols, int64_t page_size);
+int moe_paged_mla_attention(const void* q_latent, int64_t ql_stride, int64_t ql_head_stride, const void* q_pe,
+                            int64_t qp_stride, int64_t qp_head_stride, const void* cache, int dtype, int64_t pages,
+                            int64_t page_size, int64_t page_stride, int64_t row_stride, const int32_t* page_table,
+                            int64_t table_stride, int64_t table_cols, const int32_t* lengths, int64_t batch,
+                            int64_t heads, int64_t kv_lora_rank, int64_t qk_rope_dim, float softmax_scale, void* out,
+                            float* lse, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------
  * Profiling (no reference counterpart): when enabled, moe_ds_moe_layer_fp8
  * records CUDA events on its stream at the boundaries of its stages:
  * start | route, dispatch, chunk list (+ f16 staging of x on the MMA path) |
@@ -649,7 +721,9 @@ int moe_read_spans(const char* path, int64_t n, const uint64_t* offsets, const u
  * tensor-core GEMM pipeline, 128: fused decode experts -- a down piece gave
  * up waiting for its expert's activations), or when an expert-parallel peer
  * kernel skipped a store whose rank, slot or row read from exchanged data was
- * out of range (64).  Synchronises
+ * out of range (64), or a paged cache operator skipped a slot, position, page
+ * or length out of range (512; 1024 and 2048: a wait of the FP8 linear or of
+ * the paged attention gave up).  Synchronises
  * `stream`, returns the word (-1 if it cannot be read) and clears it. */
 int moe_b200_device_error(void* stream);
 

@@ -20,6 +20,7 @@
 #include "route_host.cuh"
 #include "router.cuh"
 #include "router_device.cuh"
+#include "serving.cuh"
 #include "status.cuh"
 
 using namespace moe;
@@ -1992,7 +1993,9 @@ int moe_b200_device_error(void* stream) {
   const int b = read_and_clear_mma_device_error(as_stream(stream));
   const int c = read_and_clear_prefill_device_error(as_stream(stream));
   const int d = read_and_clear_ep_error(as_stream(stream));
-  return (a < 0 || b < 0 || c < 0 || d < 0) ? -1 : (a | b | c | d);
+  const int e = read_and_clear_linear_error(as_stream(stream));
+  const int f = read_and_clear_paged_error(as_stream(stream));
+  return (a < 0 || b < 0 || c < 0 || d < 0 || e < 0 || f < 0) ? -1 : (a | b | c | d | e | f);
 }
 
 int moe_b200_stage_times(float* ms, int max_n) {

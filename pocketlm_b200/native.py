@@ -154,6 +154,14 @@ _SIGNATURES: dict[str, tuple[list, object]] = {
     "moe_ep_experts_return_p2p": ([_P, _P, _P, _I64, _I64, _I64, _I64, _P, _I64, _P, _INT, _I64, _I64, _I64, _P,
                                    _P, _I64, _P], _INT),
     "moe_ep_experts_return_p2p_workspace_bytes": ([_I64] * 5 + [_INT], _I64),
+    "moe_rmsnorm_fp8": ([_P, _I64, _INT, _P, _I64, _P, _INT, _I64, _I64, _F32, _P, _I64, _P, _P, _P, _P], _INT),
+    "moe_fp8_quantize_rows": ([_P, _I64, _INT, _I64, _I64, _P, _I64, _P, _P], _INT),
+    "moe_fp8_block_linear": ([_P, _I64, _P, _P, _I64, _P, _I64, _I64, _I64, _P, _INT, _P], _INT),
+    "moe_paged_mla_append": ([_P, _I64, _INT, _P, _INT, _P, _P, _P, _P, _I64, _P, _INT, _I64, _I64, _I64, _I64, _P,
+                              _I64, _I64, _I64, _P, _I64, _I64, _I64, _F32, _P], _INT),
+    "moe_paged_mla_attention_workspace_bytes": ([_I64] * 6, _I64),
+    "moe_paged_mla_attention": ([_P, _I64, _I64, _P, _I64, _I64, _P, _INT, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P,
+                                 _I64, _I64, _I64, _I64, _F32, _P, _P, _P, _I64, _P], _INT),
     "moe_b200_fused_decode": ([_INT], _INT),
     "moe_b200_fused_decode_enabled": ([], _INT),
     "moe_b200_force_ksplit": ([_INT], _INT),

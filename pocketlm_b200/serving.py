@@ -1,0 +1,270 @@
+"""Batched operators in front of the MoE layer, for serving many sequences.
+
+The reference's attention block (native/__init__.py:878-1075) takes one fp32
+token and a contiguous cache; these are its steps for a batch of tokens in
+16 bits, 8-bit linears and a paged cache:
+
+  rmsnorm_fp8          the residual's addition, RMSNorm, e4m3 rows with a scale per 128 columns
+  quantize_fp8_rows    the same 8-bit form of rows as they are
+  fp8_block_linear     e4m3 rows times an e4m3 weight with 128 x 128 block scales
+  paged_mla_append     a batch's new latent rows into a paged cache, positions rotated on the way
+  paged_mla_attention  one query token per row over its pages
+
+Every tensor is on one CUDA device, which need not be the current one; the
+work is enqueued on that device's current stream (captured into a CUDA graph
+where one is being captured) and nothing synchronises.  Unlike the bridge
+calls of `native`, CPU tensors are refused.  Inference only: no gradients.
+Wrong shapes, types and devices raise ValueError, a failing call RuntimeError.
+Indexes that only the device knows (slots, pages, lengths, positions) are
+checked by the kernels, which skip what is out of range and set code 512 in
+the device error word (moe_b200_device_error).
+"""
+
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+
+from . import native
+
+_CODE = {torch.float32: native.DTYPE_F32, torch.bfloat16: native.DTYPE_BF16, torch.float16: native.DTYPE_F16}
+_FP8 = (torch.float8_e4m3fn, torch.uint8, torch.int8)
+
+
+class NormedRows(NamedTuple):
+    """rmsnorm_fp8's outputs."""
+
+    codes: torch.Tensor  # e4m3 [..., cols]
+    scales: torch.Tensor  # fp32 [..., ceil(cols / 128)]
+    residual: torch.Tensor  # the stream that was normalised: x + residual in x's type, or x itself
+    normed: torch.Tensor | None  # the normed rows in x's type, when asked for
+
+
+def _need(ok: bool, message: str) -> None:
+    if not ok:
+        raise ValueError(message)
+
+
+def _call(name: str, device: torch.device, *args) -> None:
+    lib = native.load_library()
+    if device.index == torch.cuda.current_device():
+        native._check(getattr(lib, name)(*args, torch.cuda.current_stream(device).cuda_stream), name)
+        return
+    with torch.cuda.device(device):
+        native._check(getattr(lib, name)(*args, torch.cuda.current_stream(device).cuda_stream), name)
+
+
+def _same_device(first: torch.Tensor, *others: torch.Tensor | None) -> torch.device:
+    device = first.device
+    _need(device.type == "cuda", "tensors must be on a CUDA device")
+    for t in others:
+        _need(t is None or t.device == device, "tensors must be on one device")
+    return device
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """t as [rows, cols] with contiguous columns: a view where its strides allow one."""
+    if t.ndim != 2:
+        t = t.reshape(-1, t.shape[-1])
+    return t if t.stride(1) == 1 else t.contiguous()
+
+
+def _new_codes(rows: int, cols: int, device: torch.device) -> torch.Tensor:
+    """Codes whose rows start on 16-byte boundaries, as fp8_block_linear reads them."""
+    wide = (cols + 15) // 16 * 16
+    codes = torch.empty((rows, wide), dtype=torch.float8_e4m3fn, device=device)
+    return codes if wide == cols else codes[:, :cols]
+
+
+def rmsnorm_fp8(x: torch.Tensor, weight: torch.Tensor, *, residual: torch.Tensor | None = None, eps: float = 1e-6,
+                return_normed: bool = False) -> NormedRows:
+    """h = x + residual (in x's type); y = h / sqrt(mean(h^2) + eps) * weight; y as e4m3 codes with one
+    fp32 scale per 128 columns, max(amax, 2^-100) / 448.
+
+    x [..., cols] bf16, fp16 or fp32 (rows of a wider tensor need no copy), cols <= 32768; weight [cols] of x's
+    type or fp32; residual like x.  The mean is of h as it is returned.  return_normed adds y in x's type, the
+    rows that a router reads."""
+    _need(x.dtype in _CODE, "x must be bf16, fp16 or fp32")
+    _need(x.ndim >= 1 and x.shape[-1] > 0, "x must be [..., cols]")
+    cols = x.shape[-1]
+    _need(weight.shape == (cols,), "weight must be [cols]")
+    _need(weight.dtype == x.dtype or weight.dtype == torch.float32, "weight must be of x's type or fp32")
+    _need(residual is None or (residual.shape == x.shape and residual.dtype == x.dtype), "residual must be like x")
+    _need(cols <= 32768, "x has more than 32768 columns")
+    device = _same_device(x, weight, residual)
+    lead, flat = x.shape[:-1], _rows(x)
+    rows = flat.shape[0]
+    weight = weight.contiguous()
+    codes = _new_codes(rows, cols, device)
+    scales = torch.empty((rows, (cols + 127) // 128), dtype=torch.float32, device=device)
+    normed = torch.empty((rows, cols), dtype=x.dtype, device=device) if return_normed else None
+    stream_rows, res, res_stride = None, None, 0
+    if residual is not None:
+        res = _rows(residual)
+        res_stride = res.stride(0)
+        stream_rows = torch.empty((rows, cols), dtype=x.dtype, device=device)
+    if rows:
+        _call("moe_rmsnorm_fp8", device, flat.data_ptr(), flat.stride(0), _CODE[x.dtype],
+              None if res is None else res.data_ptr(), res_stride, weight.data_ptr(), _CODE[weight.dtype], rows, cols,
+              float(eps), codes.data_ptr(), codes.stride(0), scales.data_ptr(),
+              None if stream_rows is None else stream_rows.data_ptr(), None if normed is None else normed.data_ptr())
+    if x.ndim != 2:
+        codes, scales = codes.view(x.shape), scales.view(*lead, scales.shape[1])
+        normed = None if normed is None else normed.reshape(x.shape)
+        stream_rows = None if stream_rows is None else stream_rows.reshape(x.shape)
+    return NormedRows(codes, scales, x if residual is None else stream_rows, normed)
+
+
+def quantize_fp8_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """x [..., cols] (bf16, fp16 or fp32) as e4m3 codes [..., cols] with one fp32 scale per 128 columns,
+    max(amax, 2^-100) / 448."""
+    _need(x.dtype in _CODE, "x must be bf16, fp16 or fp32")
+    _need(x.ndim >= 1 and x.shape[-1] > 0, "x must be [..., cols]")
+    device = _same_device(x)
+    cols, lead, flat = x.shape[-1], x.shape[:-1], _rows(x)
+    rows = flat.shape[0]
+    codes = _new_codes(rows, cols, device)
+    scales = torch.empty((rows, (cols + 127) // 128), dtype=torch.float32, device=device)
+    if rows:
+        _call("moe_fp8_quantize_rows", device, flat.data_ptr(), flat.stride(0), _CODE[x.dtype], rows, cols,
+              codes.data_ptr(), codes.stride(0), scales.data_ptr())
+    if x.ndim != 2:
+        codes, scales = codes.view(x.shape), scales.view(*lead, scales.shape[1])
+    return codes, scales
+
+
+def _code_rows(t: torch.Tensor) -> torch.Tensor:
+    """[rows, cols] codes whose rows start on 16-byte boundaries (a copy where they do not)."""
+    if t.stride(1) == 1 and t.stride(0) % 16 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0:
+        return t
+    wide = torch.empty((t.shape[0], (t.shape[1] + 15) // 16 * 16), dtype=t.dtype, device=t.device)[:, :t.shape[1]]
+    return wide.copy_(t)
+
+
+def fp8_block_linear(codes: torch.Tensor, scales: torch.Tensor, fp8_weight: torch.Tensor, scale_inv: torch.Tensor, *,
+                     out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """out[t, n] = sum_g scales[t, g] scale_inv[n // 128, g] sum_{k in group g} codes[t, k] fp8_weight[n, k].
+
+    codes [..., in] and scales [..., ceil(in / 128)] as rmsnorm_fp8 and quantize_fp8_rows give them; fp8_weight
+    [out, in] e4m3 (or its bytes) and scale_inv [ceil(out / 128), ceil(in / 128)] as the checkpoints hold them.
+    Sums in fp32, one rounding to out_dtype (bf16, fp16 or fp32).  NaN codes are NaN (the fp32-activation linears
+    of `native` read them as 0).  Rows that do not start on 16-byte boundaries are copied first."""
+    _need(codes.dtype in _FP8 and fp8_weight.dtype in _FP8, "codes and fp8_weight must be e4m3")
+    _need(scales.dtype == torch.float32 and scale_inv.dtype == torch.float32, "scales must be fp32")
+    _need(out_dtype in _CODE, "out_dtype must be bf16, fp16 or fp32")
+    _need(fp8_weight.ndim == 2, "fp8_weight must have shape [out_rows, in_cols]")
+    _need(scale_inv.ndim == 2, "scale_inv must have shape [scale_rows, scale_cols]")
+    outs, cols = fp8_weight.shape
+    blocks = (cols + 127) // 128
+    _need(outs > 0 and cols > 0, "fp8_weight must not be empty")
+    _need(codes.ndim >= 1 and codes.shape[-1] == cols, "hidden input size does not match FP8 weight columns")
+    _need(scale_inv.shape == ((outs + 127) // 128, blocks), "scale_inv shape does not match FP8 128x128 block layout")
+    lead = codes.shape[:-1]
+    _need(scales.shape == (*lead, blocks), "scales must be [..., ceil(in_cols / 128)]")
+    device = _same_device(codes, scales, fp8_weight, scale_inv)
+    x, w = codes if codes.ndim == 2 else codes.reshape(-1, cols), _code_rows(fp8_weight)
+    rows = x.shape[0]
+    x, scales, scale_inv = _code_rows(x), scales.contiguous(), scale_inv.contiguous()
+    out = torch.empty((rows, outs), dtype=out_dtype, device=device)
+    if rows:
+        _call("moe_fp8_block_linear", device, x.data_ptr(), x.stride(0), scales.data_ptr(), w.data_ptr(), w.stride(0),
+              scale_inv.data_ptr(), rows, outs, cols, out.data_ptr(), _CODE[out_dtype])
+    return out if len(lead) == 1 else out.reshape(*lead, outs)
+
+
+def paged_mla_append(kv_rows: torch.Tensor, kv_norm_weight: torch.Tensor, cache: torch.Tensor, slots: torch.Tensor,
+                     positions: torch.Tensor, rope_cos: torch.Tensor, rope_sin: torch.Tensor, *, eps: float = 1e-6,
+                     q_pe: torch.Tensor | None = None) -> torch.Tensor | None:
+    """Stores tokens' rows [RMSNorm(kv[:latent]) * kv_norm_weight, rot(kv[latent:], position)] in `cache`, in place,
+    and returns the queries' rope parts rotated by the same positions (None without q_pe).
+
+    kv_rows [tokens, latent + rope] (the kv_a projection's rows; a slice of wider ones needs no copy) and
+    kv_norm_weight [latent] of the cache's type or fp32; cache [pages, page_size, latent + rope] bf16 or fp16;
+    slots int64 [tokens] = page * page_size + offset, distinct, negative for rows to leave out; positions int64
+    [tokens] into rope_cos / rope_sin fp32 [max_positions, rope / 2], pairs (2p, 2p + 1); q_pe [tokens, heads,
+    rope] of the cache's type (a slice of the q_b projection's output needs no copy).  A position outside the
+    tables gives zero queries and stores no row."""
+    _need(cache.ndim == 3 and cache.stride(2) == 1 and cache.numel() > 0, "cache must be [pages, page_size, latent + rope]")
+    _need(cache.dtype in (torch.bfloat16, torch.float16), "cache must be bf16 or fp16")
+    pages, page_size, width = cache.shape
+    _need(kv_norm_weight.ndim == 1 and rope_cos.ndim == 2 and rope_cos.shape == rope_sin.shape,
+          "kv_norm_weight must be [latent], rope_cos and rope_sin [max_positions, rope / 2]")
+    latent, rope, tokens = kv_norm_weight.shape[0], 2 * rope_cos.shape[1], kv_rows.shape[0]
+    _need(kv_rows.ndim == 2 and kv_rows.shape[1] == latent + rope == width, "kv_rows, cache and norm weight sizes do not match")
+    _need(latent > 0 and rope > 0 and rope_cos.shape[0] > 0, "latent, rope and the tables must not be empty")
+    _need(slots.shape == (tokens,) and positions.shape == (tokens,), "slots and positions must be [tokens]")
+    _need(slots.dtype == torch.int64 and positions.dtype == torch.int64, "slots and positions must be int64")
+    _need(kv_rows.dtype in (cache.dtype, torch.float32), "kv_rows must be of the cache's type or fp32")
+    _need(kv_norm_weight.dtype in (cache.dtype, torch.float32), "kv_norm_weight must be of the cache's type or fp32")
+    _need(rope_cos.dtype == torch.float32 and rope_sin.dtype == torch.float32, "rope tables must be fp32")
+    _need(q_pe is None or (q_pe.ndim == 3 and q_pe.shape[0] == tokens and q_pe.shape[1] > 0 and q_pe.shape[2] == rope),
+          "q_pe must be [tokens, heads, rope]")
+    _need(q_pe is None or q_pe.dtype == cache.dtype, "q_pe must be of the cache's type")
+    device = _same_device(cache, kv_rows, kv_norm_weight, slots, positions, rope_cos, rope_sin, q_pe)
+    kv = _rows(kv_rows)
+    q_out, heads, q_strides = None, 0, (0, 0)
+    if q_pe is not None:
+        if q_pe.stride(2) != 1:
+            q_pe = q_pe.contiguous()
+        heads, q_strides = q_pe.shape[1], q_pe.stride()[:2]
+        q_out = torch.empty((tokens, heads, rope), dtype=cache.dtype, device=device)
+    if tokens:
+        norm_w, slots, positions = kv_norm_weight.contiguous(), slots.contiguous(), positions.contiguous()
+        cos, sin = rope_cos.contiguous(), rope_sin.contiguous()
+        _call("moe_paged_mla_append", device, kv.data_ptr(), kv.stride(0), _CODE[kv.dtype], norm_w.data_ptr(),
+              _CODE[norm_w.dtype], slots.data_ptr(), positions.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0],
+              cache.data_ptr(), _CODE[cache.dtype], pages, page_size, cache.stride(0), cache.stride(1),
+              None if q_pe is None else q_pe.data_ptr(), *q_strides, heads, None if q_out is None else q_out.data_ptr(),
+              tokens, latent, rope, float(eps))
+    return q_out
+
+
+def _query(t: torch.Tensor) -> torch.Tensor:
+    """Queries whose rows start on 16-byte boundaries (a copy where they do not)."""
+    if t.stride(2) == 1 and t.stride(0) % 8 == 0 and t.stride(1) % 8 == 0 and t.data_ptr() % 16 == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def paged_mla_attention(q_latent: torch.Tensor, q_pe: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor,
+                        lengths: torch.Tensor, *, softmax_scale: float, return_lse: bool = False):
+    """Attention of one new token per row over its pages of a latent cache, in the absorbed form:
+    score = softmax_scale * (q_latent . latent + q_pe . rope part), out = softmax(score) . latent.
+
+    q_latent [batch, heads, latent] (W_UK^T q_nope), q_pe [batch, heads, rope] (rotated) and cache [pages,
+    page_size, latent + rope], all bf16 or all fp16; page_table int32 [batch, max_pages], lengths int32 [batch]
+    (the new token included).  Returns [batch, heads, latent] in the queries' type, for W_UV, and with
+    return_lse also log(sum exp(score)) fp32 [batch, heads].  A row of length 0 gives zeros (and -inf); entries of
+    page_table past a row's last page are not read.  Several tokens of one sequence are rows with the same pages and
+    lengths one apart.  latent <= 512 and rope <= 64, multiples of 8; any page size."""
+    _need(cache.ndim == 3 and cache.stride(2) == 1 and cache.numel() > 0, "cache must be [pages, page_size, latent + rope]")
+    _need(cache.dtype in (torch.bfloat16, torch.float16), "cache must be bf16 or fp16")
+    _need(q_latent.ndim == 3 and q_pe.ndim == 3, "q_latent and q_pe must be [batch, heads, dim]")
+    batch, heads, latent = q_latent.shape
+    rope = q_pe.shape[2]
+    pages, page_size, width = cache.shape
+    _need(q_pe.shape[:2] == q_latent.shape[:2] and heads > 0, "batch or head count mismatch")
+    _need(latent > 0 and rope > 0 and latent + rope == width, "query and cache sizes do not match")
+    _need(q_latent.dtype == cache.dtype and q_pe.dtype == cache.dtype, "queries must be of the cache's type")
+    _need(page_table.ndim == 2 and page_table.shape[0] == batch and page_table.shape[1] > 0,
+          "page_table must be [batch, max_pages]")
+    _need(lengths.shape == (batch,), "lengths must be [batch]")
+    _need(page_table.dtype == torch.int32 and lengths.dtype == torch.int32, "page_table and lengths must be int32")
+    _need(cache.stride(0) % 8 == 0 and cache.stride(1) % 8 == 0 and cache.data_ptr() % 16 == 0,
+          "cache rows must start on 16-byte boundaries")
+    device = _same_device(cache, q_latent, q_pe, page_table, lengths)
+    q_latent, q_pe = _query(q_latent), _query(q_pe)
+    out = torch.empty((batch, heads, latent), dtype=cache.dtype, device=device)
+    lse = torch.empty((batch, heads), dtype=torch.float32, device=device) if return_lse else None
+    if batch:
+        table = page_table if page_table.stride(1) == 1 else page_table.contiguous()
+        lengths = lengths.contiguous()
+        need = native.load_library().moe_paged_mla_attention_workspace_bytes(batch, heads, latent, rope, table.shape[1], page_size)
+        work = torch.empty((max(int(need), 256),), dtype=torch.uint8, device=device)
+        _call("moe_paged_mla_attention", device, q_latent.data_ptr(), q_latent.stride(0), q_latent.stride(1),
+              q_pe.data_ptr(), q_pe.stride(0), q_pe.stride(1), cache.data_ptr(), _CODE[cache.dtype], pages, page_size,
+              cache.stride(0), cache.stride(1), table.data_ptr(), table.stride(0), table.shape[1], lengths.data_ptr(),
+              batch, heads, latent, rope, float(softmax_scale), out.data_ptr(), None if lse is None else lse.data_ptr(),
+              work.data_ptr(), work.numel())
+    return (out, lse) if return_lse else out
