@@ -22,6 +22,7 @@
 #include "plan.cuh"
 #include "router.cuh"
 #include "serving.cuh"
+#include "tcgen05.cuh"
 
 namespace moe {
 namespace {
@@ -175,58 +176,603 @@ cudaError_t launch_append_types(const AppendArgs& a, int x_dtype, int norm_dtype
   return wide ? launch_append<C, float, C>(a, stream) : launch_append<C, C, C>(a, stream);
 }
 
-// One CTA per (row, head): its warps take positions in turn, each with a
-// running maximum, sum and latent sums, joined at the end.
-constexpr int kSimpleWarps = 8;
+// ------------------------------------------------------------- attention
+//
+// A CTA takes 128 heads of one row and half of the latent columns of the
+// result; the two CTAs of a pair compute the same scores.  Tensor memory holds
+// the 128 x 256 fp32 result, two 128 x 64 score tiles (the softmax of one while
+// the other is computed; its 16-bit probabilities replace the scores) and 256
+// columns of the queries: all 512 columns.  Shared memory holds the queries'
+// other columns (80 KiB) and the cache rows in chunks of 64 positions x 64
+// columns (8 KiB, 128B-swizzled): the chunks of this CTA's own columns stay
+// until the second product has read them (3 tiles of them), the others pass
+// through 6 slots as the scores are computed.
+//   scores  S = Q K^T:  M = 128 heads, N = 64 positions, k over the columns
+//   result  O += P V:   M = 128 heads, N = own columns, k over the positions;
+// V is the same shared memory as K, read as an MN-major operand.
+// Halving the columns costs the scores twice (832 instead of 544 multiply-adds
+// per head and position and CTA) but leaves room in tensor memory for the
+// overlap; the cache is read from memory once, the pair's second read hits L2.
+//
+// The softmax's reference maximum moves only when a tile's maximum exceeds it
+// by 2^8 (log2 domain): probabilities stay below 2^8 of the reference's 1, well
+// inside 16-bit range, and the 256 columns of the result are rescaled rarely.
+// Probabilities are rounded to the cache's type for the second product, half a
+// step each; their sum is of the unrounded fp32 values.
+//
+// Work: all rows' tiles of 64 positions in one sequence, cut into equal
+// ranges, one per CTA pair, so that lengths need not be alike.  A row inside
+// one range is finished there; a row that is cut leaves fp32 parts in the
+// workspace, which the second kernel joins.  A range has at most two parts.
+//
+// Warps 0-3: softmax, result (a thread per head).  4-7: cache rows by 16-byte
+// asynchronous copies (any page size; rows past the length arrive as zeros).
+// 8: tensor memory and the products.
+constexpr int kTile = 64;
+constexpr int kHeads = 128;
+constexpr int kChunkBytes = kTile * 128;
+constexpr int kQChunkBytes = kHeads * 128;
+constexpr int kQTmemChunks = 4, kQSmemChunks = 5;
+constexpr int kKeptStages = 3, kKeptChunks = 4;
+constexpr int kPassing = 6;
+constexpr int kSoftmaxThreads = 128, kCopyThreads = 128;
+constexpr int kAttnThreads = kSoftmaxThreads + kCopyThreads + kWarp;
+constexpr int kAttnWarps = kAttnThreads / kWarp;
+constexpr uint32_t kColO = 0, kColS = 256, kColQ = 384;
+constexpr int kMinTiles = 2;  // fewest tiles worth a range of their own
+constexpr float kMovesBy = 8.0f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+struct AttnBarriers {
+  uint64_t kept_full[kKeptStages], kept_empty[kKeptStages];
+  uint64_t pass_full[kPassing], pass_empty[kPassing];
+  uint64_t s_full[2];    // scores complete
+  uint64_t p_ready[2];   // probabilities written (one arrival per softmax warp)
+  uint64_t q_ready;      // queries of the next part in place
+  uint64_t o_done;       // a tile's second product complete
+  uint64_t o_read;       // the part's result has been read
+  uint64_t drain;
+  uint32_t tmem_base;
+  int abort;
+  int first_item, first_tile;
+  long long sums[kAttnWarps];
+};
+constexpr size_t kAttnSmem = 1024 + static_cast<size_t>(kQSmemChunks) * kQChunkBytes +
+                             static_cast<size_t>(kKeptStages * kKeptChunks + kPassing) * kChunkBytes + sizeof(AttnBarriers);
+static_assert(kAttnSmem <= 232448, "shared memory per block");
+
+struct AttnPlan {
+  float* part_o;       // [2 workers][128 heads][latent]: unnormalised
+  float2* part_ml;     // [2 workers][128 heads]: reference maximum (log2 domain), sum
+  int64_t* before;     // [batch + 1]: tiles before each row
+  int workers;         // pairs of CTAs
+  int groups;          // groups of 128 heads: an item is a row's group
+};
+
+MOE_HD int64_t range_start(int64_t w, int64_t total, int64_t workers) { return w * total / workers; }
+MOE_D int64_t used_workers(int64_t total, int64_t workers) {
+  return max(int64_t(1), min(workers, total / kMinTiles));
+}
+
+MOE_D int row_length(const PagedAttnArgs& a, int64_t b) {
+  const int64_t room = a.table_cols * a.page_size;
+  const int n = a.lengths[b];
+  return n < 0 ? 0 : n > room ? static_cast<int>(room) : n;
+}
+MOE_D int tiles_of(int len) { return (len + kTile - 1) / kTile; }
+
+// The parts of a range in order; every role walks them by itself.
+struct Part {
+  int64_t b;
+  int group, tile0, tiles, len;
+  bool whole;
+  int slot;
+};
+struct Walk {
+  int64_t item;
+  int tile0;
+  int64_t left;
+  MOE_D bool next(const PagedAttnArgs& a, int groups, int worker, Part& p) {
+    if (left <= 0) return false;
+    int n;
+    while (true) {
+      p.b = item / groups;
+      p.len = row_length(a, p.b);
+      n = tiles_of(p.len) - tile0;
+      if (n > 0) break;
+      ++item;
+      tile0 = 0;
+    }
+    p.group = static_cast<int>(item - p.b * groups);
+    p.tile0 = tile0;
+    p.tiles = static_cast<int>(min(static_cast<int64_t>(n), left));
+    p.whole = tile0 == 0 && p.tiles == n;
+    p.slot = 2 * worker + (tile0 > 0 ? 0 : 1);
+    left -= p.tiles;
+    ++item;
+    tile0 = 0;
+    return true;
+  }
+};
+
+MOE_D float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
 template <typename T>
-__global__ void __launch_bounds__(kSimpleWarps * kWarp) paged_attention_simple_kernel(PagedAttnArgs a) {
-  constexpr int kCols = 16;  // latent columns per lane: latent <= 512
-  __shared__ float m_s[kSimpleWarps], l_s[kSimpleWarps], acc_s[kSimpleWarps][kCols * kWarp];
-  const int lane = threadIdx.x % kWarp, warp = threadIdx.x / kWarp;
-  const int64_t b = blockIdx.y, h = blockIdx.x;
-  const T* ql = static_cast<const T*>(a.q_latent) + b * a.ql_stride + h * a.ql_head_stride;
-  const T* qp = static_cast<const T*>(a.q_pe) + b * a.qp_stride + h * a.qp_head_stride;
-  const int64_t len = std::max(0, a.lengths[b]);
-  float acc[kCols];
-  for (int i = 0; i < kCols; ++i) acc[i] = 0.0f;
-  float m = -INFINITY, l = 0.0f;
-  for (int64_t p = warp; p < len; p += kSimpleWarps) {
-    const int64_t col = p / a.page_size;
-    const int64_t page = col < a.table_cols ? a.table[b * a.table_stride + col] : -1;
-    if (page < 0 || page >= a.pages) {
-      if (lane == 0) atomicOr(&g_device_error, kPagedRangeError);
-      continue;
-    }
-    const T* row = static_cast<const T*>(a.cache) + page * a.page_stride + (p - col * a.page_size) * a.row_stride;
-    float s = 0.0f, c[kCols];
-    for (int i = 0; i < kCols; ++i) {
-      const int k = lane + i * kWarp;
-      c[i] = k < a.latent ? widen<T>(row[k]) : 0.0f;
-      if (k < a.latent) s = fmaf(widen<T>(ql[k]), c[i], s);
-    }
-    for (int k = lane; k < a.rope; k += kWarp) s = fmaf(widen<T>(qp[k]), widen<T>(row[a.latent + k]), s);
-    s = warp_sum(s) * a.scale;
-    const float top = fmaxf(m, s), old = m == -INFINITY ? 0.0f : expf(m - top), e = expf(s - top);
-    l = l * old + e;
-    for (int i = 0; i < kCols; ++i) acc[i] = acc[i] * old + e * c[i];
-    m = top;
+MOE_D uint32_t pack2(float lo, float hi);
+template <>
+MOE_D uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+template <>
+MOE_D uint32_t pack2<__half>(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+MOE_D void copy16(uint32_t dst, const void* src, bool present) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(present ? 16 : 0) : "memory");
+}
+MOE_D void copies_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+
+// A wait of a whole warp: every lane sees the same answer.
+MOE_D bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int code) {
+  return __all_sync(0xFFFFFFFFu, wait_or_abort(bar, parity, abort, code));
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(PagedAttnArgs a, AttnPlan plan) {
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  unsigned char* q_smem = smem;
+  unsigned char* kept_smem = q_smem + kQSmemChunks * kQChunkBytes;
+  unsigned char* pass_smem = kept_smem + kKeptStages * kKeptChunks * kChunkBytes;
+  AttnBarriers* bars = reinterpret_cast<AttnBarriers*>(pass_smem + kPassing * kChunkBytes);
+  const int tid = threadIdx.x, warp = tid / kWarp, lane = tid % kWarp;
+  volatile int* abort = &bars->abort;
+  const int latent = static_cast<int>(a.latent), rope = static_cast<int>(a.rope);
+  const int lat_chunks = (latent + 63) / 64, chunks = lat_chunks + 1;  // the last one holds the rope part
+  const int halves = lat_chunks > 1 ? 2 : 1, per_half = (lat_chunks + halves - 1) / halves;
+  const int worker = blockIdx.x / halves, half = blockIdx.x % halves;
+  const int kept0 = half * per_half, kept_n = min(per_half, lat_chunks - kept0);
+  const int q_tmem = min(kQTmemChunks, lat_chunks);
+
+  // tiles before each thread's rows; the range's first item
+  long long mine = 0;
+  const int64_t per = ceil_div(a.batch, kAttnThreads), b0 = min(a.batch, tid * per), b1 = min(a.batch, b0 + per);
+  for (int64_t b = b0; b < b1; ++b) mine += static_cast<long long>(tiles_of(row_length(a, b))) * plan.groups;
+  long long upto = mine;
+#pragma unroll
+  for (int o = 1; o < kWarp; o <<= 1) {
+    const long long v = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+    if (lane >= o) upto += v;
   }
-  for (int i = 0; i < kCols; ++i) acc_s[warp][lane + i * kWarp] = acc[i];
-  if (lane == 0) {
-    m_s[warp] = m;
-    l_s[warp] = l;
-  }
+  if (lane == kWarp - 1) bars->sums[warp] = upto;
   __syncthreads();
-  float top = -INFINITY, total = 0.0f;
-  for (int w = 0; w < kSimpleWarps; ++w) top = fmaxf(top, m_s[w]);
-  for (int w = 0; w < kSimpleWarps; ++w) total += l_s[w] == 0.0f ? 0.0f : l_s[w] * expf(m_s[w] - top);
-  for (int k = threadIdx.x; k < a.latent; k += kSimpleWarps * kWarp) {
-    float v = 0.0f;
-    for (int w = 0; w < kSimpleWarps; ++w)
-      if (l_s[w] != 0.0f) v += acc_s[w][k] * expf(m_s[w] - top);
-    static_cast<T*>(a.out)[(b * a.heads + h) * a.latent + k] = from_float<T>(total == 0.0f ? 0.0f : v / total);
+  long long before = upto - mine, total = 0;
+  for (int w = 0; w < kAttnWarps; ++w) {
+    if (w < warp) before += bars->sums[w];
+    total += bars->sums[w];
   }
-  if (a.lse && threadIdx.x == 0) a.lse[b * a.heads + h] = total == 0.0f ? -INFINITY : top + logf(total);
+  if (blockIdx.x == 0) {
+    long long at = before;
+    for (int64_t b = b0; b < b1; ++b) {
+      plan.before[b] = at;
+      at += static_cast<long long>(tiles_of(row_length(a, b))) * plan.groups;
+      if (a.lengths[b] > a.table_cols * a.page_size) atomicOr(&g_device_error, kPagedRangeError);
+    }
+    if (tid == 0) plan.before[a.batch] = total;
+  }
+  const int64_t workers = used_workers(total, plan.workers);
+  if (worker >= workers || total == 0) return;
+  const int64_t start = range_start(worker, total, workers), stop = range_start(worker + 1, total, workers);
+  if (start >= before && start < before + mine) {
+    long long at = before;
+    int64_t item = b0 * plan.groups;
+    while (true) {
+      const int n = tiles_of(row_length(a, item / plan.groups));
+      if (start < at + n) break;
+      at += n;
+      ++item;
+    }
+    bars->first_item = static_cast<int>(item);
+    bars->first_tile = static_cast<int>(start - at);
+  }
+  if (tid == 0) {
+    for (int s = 0; s < kKeptStages; ++s) {
+      mbar_init(&bars->kept_full[s], kCopyThreads);
+      mbar_init(&bars->kept_empty[s], 1);
+    }
+    for (int s = 0; s < kPassing; ++s) {
+      mbar_init(&bars->pass_full[s], kCopyThreads);
+      mbar_init(&bars->pass_empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&bars->s_full[s], 1);
+      mbar_init(&bars->p_ready[s], kSoftmaxThreads / kWarp);
+    }
+    mbar_init(&bars->q_ready, kSoftmaxThreads / kWarp);
+    mbar_init(&bars->o_done, 1);
+    mbar_init(&bars->o_read, kSoftmaxThreads / kWarp);
+    mbar_init(&bars->drain, 1);
+    bars->abort = 0;
+    fence_barrier_init();
+  }
+  if (warp == kAttnWarps - 1) {
+    tmem_alloc(&bars->tmem_base, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars->tmem_base;
+  Walk walk{bars->first_item, bars->first_tile, stop - start};
+  Part p;
+
+  if (warp >= kSoftmaxThreads / kWarp && warp < kAttnWarps - 1) {
+    // ------------------------------------------------------------ copies
+    const int ct = tid - kSoftmaxThreads, unit = ct % 8, row0 = ct / 8;
+    const uint32_t kept_at = smem_addr(kept_smem), pass_at = smem_addr(pass_smem);
+    uint32_t g = 0, pc = 0;
+    bool ok = true;
+    while (ok && walk.next(a, plan.groups, worker, p)) {
+      const int32_t* table = a.table + p.b * a.table_stride;
+      for (int i = 0; i < p.tiles && ok; ++i, ++g) {
+        const T* src[4];
+        bool live[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int pos = (p.tile0 + i) * kTile + row0 + 16 * j;
+          src[j] = static_cast<const T*>(a.cache);
+          live[j] = pos < p.len;
+          if (live[j]) {
+            const int col = pos / static_cast<int>(a.page_size);
+            const int page = __ldg(table + col);
+            live[j] = page >= 0 && page < a.pages;
+            if (live[j]) src[j] += page * a.page_stride + (pos - col * static_cast<int>(a.page_size)) * a.row_stride;
+          }
+        }
+        // chunk c: columns 64 c .. of the latent part, or the rope part
+        auto fetch = [&](int c, uint32_t dst) {
+          const int col = (c < lat_chunks ? c * 64 : latent) + unit * 8;
+          const bool in = c < lat_chunks ? col < latent : unit * 8 < rope;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int r = row0 + 16 * j;
+            copy16(dst + r * 128 + ((unit ^ (r % 8)) * 16), src[j] + (in ? col : 0), live[j] && in);
+          }
+        };
+        const int s = g % kKeptStages;
+        if (g >= kKeptStages && !wait_or_abort(&bars->kept_empty[s], ((g / kKeptStages) - 1) & 1, abort, kPagedWaitError)) {
+          ok = false;
+          break;
+        }
+        for (int k = 0; k < kept_n; ++k) fetch(kept0 + k, kept_at + (s * kKeptChunks + k) * kChunkBytes);
+        copies_arrive(&bars->kept_full[s]);
+        for (int c = 0; c < chunks; ++c) {
+          if (c >= kept0 && c < kept0 + kept_n) continue;
+          const int slot = pc % kPassing;
+          if (pc >= kPassing && !wait_or_abort(&bars->pass_empty[slot], ((pc / kPassing) - 1) & 1, abort, kPagedWaitError)) {
+            ok = false;
+            break;
+          }
+          fetch(c, pass_at + slot * kChunkBytes);
+          copies_arrive(&bars->pass_full[slot]);
+          ++pc;
+        }
+      }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  } else if (warp == kAttnWarps - 1) {
+    // ---------------------------------------------------------- products
+    if (lane == 0) {
+      const int format = sizeof(T) == 2 && __is_same(T, __nv_bfloat16) ? 1 : 0;
+      const uint32_t idesc_s = umma_idesc(kHeads, kTile, format, false);
+      const uint32_t idesc_o = umma_idesc(kHeads, 64 * kept_n, format, true);
+      const uint32_t q_at = smem_addr(q_smem), kept_at = smem_addr(kept_smem), pass_at = smem_addr(pass_smem);
+      uint32_t g = 0, pc = 0, parts = 0;
+      bool ok = true;
+      auto chunk_scores = [&](int c, uint32_t k_at, uint32_t d, bool first) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint64_t b = sw128_desc_k(k_at + k * 32);
+          const uint32_t acc = !(first && k == 0);
+          if (c < q_tmem) umma_f16_ts(d, tmem + kColQ + c * 32 + k * 8, b, idesc_s, acc);
+          else umma_f16_ss(d, sw128_desc_k(q_at + (c - q_tmem) * kQChunkBytes + k * 32), b, idesc_s, acc);
+        }
+      };
+      // the scores of the tile whose number is t
+      auto scores = [&](uint32_t t) {
+        const int s = t % kKeptStages;
+        const uint32_t d = tmem + kColS + (t % 2) * kTile;
+        if (!wait_or_abort(&bars->kept_full[s], (t / kKeptStages) & 1, abort, kPagedWaitError)) return false;
+        fence_proxy_async_shared();
+        tc_fence_after();
+        for (int k = 0; k < kept_n; ++k) chunk_scores(kept0 + k, kept_at + (s * kKeptChunks + k) * kChunkBytes, d, k == 0);
+        for (int c = 0; c < chunks; ++c) {
+          if (c >= kept0 && c < kept0 + kept_n) continue;
+          const int slot = pc % kPassing;
+          if (!wait_or_abort(&bars->pass_full[slot], (pc / kPassing) & 1, abort, kPagedWaitError)) return false;
+          fence_proxy_async_shared();
+          chunk_scores(c, pass_at + slot * kChunkBytes, d, false);
+          umma_commit(&bars->pass_empty[slot]);
+          ++pc;
+        }
+        umma_commit(&bars->s_full[t % 2]);
+        return true;
+      };
+      while (ok && walk.next(a, plan.groups, worker, p)) {
+        if (!wait_or_abort(&bars->q_ready, parts & 1, abort, kPagedWaitError)) break;
+        tc_fence_after();
+        ok = scores(g);
+        for (int i = 0; i < p.tiles && ok; ++i, ++g) {
+          if (i + 1 < p.tiles && !(ok = scores(g + 1))) break;
+          if (!(ok = wait_or_abort(&bars->p_ready[g % 2], (g / 2) & 1, abort, kPagedWaitError))) break;
+          if (i == 0 && parts > 0 && !(ok = wait_or_abort(&bars->o_read, (parts - 1) & 1, abort, kPagedWaitError))) break;
+          tc_fence_after();
+          const int s = g % kKeptStages;
+          const uint32_t v_at = kept_at + s * kKeptChunks * kChunkBytes;
+#pragma unroll
+          for (int k = 0; k < kTile / 16; ++k)
+            umma_f16_ts(tmem + kColO, tmem + kColS + (g % 2) * kTile + k * 8, sw128_desc(v_at + k * 2048, kChunkBytes),
+                        idesc_o, i > 0 || k > 0);
+          umma_commit(&bars->kept_empty[s]);
+          umma_commit(&bars->o_done);
+        }
+        ++parts;
+      }
+      umma_commit(&bars->drain);  // every product issued is complete before tensor memory is freed
+      mbar_wait(&bars->drain, 0, kPagedWaitError);
+    }
+  } else {
+    // ------------------------------------------------- softmax and result
+    const float c2 = fmaxf(a.scale * kLog2e, 1e-37f);  // above 0: a masked score's -inf stays one
+    const uint32_t my_lanes = static_cast<uint32_t>(warp * kWarp) << 16;
+    const int page_size = static_cast<int>(a.page_size);
+    auto load_queries = [&](const Part& p) {
+      const int h0 = p.group * kHeads, nh = static_cast<int>(min(a.heads - h0, static_cast<int64_t>(kHeads)));
+      const T* ql = static_cast<const T*>(a.q_latent) + p.b * a.ql_stride + h0 * a.ql_head_stride;
+      const T* qp = static_cast<const T*>(a.q_pe) + p.b * a.qp_stride + h0 * a.qp_head_stride;
+      const uint4 zero = make_uint4(0, 0, 0, 0);
+      for (int c = q_tmem; c < chunks; ++c) {  // eight threads a row, 16 rows at a time
+        const int unit = tid % 8;
+        const bool is_lat = c < lat_chunks;
+        const int col = (is_lat ? c * 64 : 0) + unit * 8;
+        const bool in = col < (is_lat ? latent : rope);
+        uint4 v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int r = tid / 8 + 16 * j;
+          const T* src = (is_lat ? ql + r * a.ql_head_stride : qp + r * a.qp_head_stride) + col;
+          v[j] = in && r < nh ? __ldg(reinterpret_cast<const uint4*>(src)) : zero;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int r = tid / 8 + 16 * j;
+          *reinterpret_cast<uint4*>(q_smem + (c - q_tmem) * kQChunkBytes + r * 128 + ((unit ^ (r % 8)) * 16)) = v[j];
+        }
+      }
+      for (int c = 0; c < q_tmem; ++c) {  // a thread its own row
+        __align__(16) uint32_t v[32];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const int col = c * 64 + u * 8;
+          *reinterpret_cast<uint4*>(v + 4 * u) =
+              tid < nh && col < latent ? __ldg(reinterpret_cast<const uint4*>(ql + tid * a.ql_head_stride + col)) : zero;
+        }
+        tmem_st32(tmem + my_lanes + kColQ + c * 32, v);
+      }
+      tmem_st_wait();
+      fence_proxy_async_shared();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->q_ready);
+    };
+    uint32_t g = 0;
+    bool ok = true, more = walk.next(a, plan.groups, worker, p);
+    if (more) load_queries(p);
+    while (ok && more) {
+      float m = -INFINITY, l = 0.0f;
+      const int32_t* table = a.table + p.b * a.table_stride;
+      for (int i = 0; i < p.tiles; ++i, ++g) {
+        // positions that take part: inside the length, on a page of the cache
+        uint32_t live[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int pos = (p.tile0 + i) * kTile + k * kWarp + lane;
+          bool in = pos < p.len;
+          if (in) {
+            const int page = __ldg(table + pos / page_size);
+            in = page >= 0 && page < a.pages;
+            if (!in) atomicOr(&g_device_error, kPagedRangeError);
+          }
+          live[k] = __ballot_sync(0xFFFFFFFFu, in);
+        }
+        if (!warp_wait(&bars->s_full[g % 2], (g / 2) & 1, abort, kPagedWaitError)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t s_at = tmem + my_lanes + kColS + (g % 2) * kTile;
+        uint32_t r[kTile];
+        tmem_ld32(s_at, r);
+        tmem_ld32(s_at + 32, r + 32);
+        tmem_ld_wait();
+        if ((live[0] & live[1]) != 0xFFFFFFFFu) {
+#pragma unroll
+          for (int j = 0; j < kTile; ++j)
+            if (!(live[j / 32] >> (j % 32) & 1u)) r[j] = 0xFF800000u;  // -inf
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < kTile; ++j) top = fmaxf(top, __uint_as_float(r[j]));
+        top *= c2;
+        const bool moves = top > m + kMovesBy || (m == -INFINITY && top > m);
+        if (__any_sync(0xFFFFFFFFu, moves)) {
+          const float f = !moves ? 1.0f : m == -INFINITY ? 0.0f : exp2_fast(m - top);
+          if (moves) {
+            l *= f;
+            m = top;
+          }
+          if (i > 0) {
+            if (!warp_wait(&bars->o_done, (g - 1) & 1, abort, kPagedWaitError)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            for (int c = 0; c < 64 * kept_n; c += 32) {
+              uint32_t o[32];
+              tmem_ld32(tmem + my_lanes + kColO + c, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+              tmem_st32(tmem + my_lanes + kColO + c, o);
+            }
+            tmem_st_wait();
+          }
+        }
+        const float ref = m == -INFINITY ? 0.0f : m;
+        float sum0 = 0.0f, sum1 = 0.0f;
+#pragma unroll
+        for (int j = 0; j < kTile; j += 2) {
+          const float p0 = exp2_fast(fmaf(__uint_as_float(r[j]), c2, -ref));
+          const float p1 = exp2_fast(fmaf(__uint_as_float(r[j + 1]), c2, -ref));
+          sum0 += p0;
+          sum1 += p1;
+          r[j / 2] = pack2<T>(p0, p1);
+        }
+        l += sum0 + sum1;
+        tmem_st32(s_at, r);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->p_ready[g % 2]);
+      }
+      if (!ok) break;
+      const Part done = p;
+      more = walk.next(a, plan.groups, worker, p);
+      if (more) load_queries(p);  // the last scores are complete: the queries' places are free
+      if (!warp_wait(&bars->o_done, (g - 1) & 1, abort, kPagedWaitError)) break;
+      tc_fence_after();
+      const int64_t h = done.group * kHeads + tid;
+      const bool has = h < a.heads;
+      const int col0 = kept0 * 64, cols = min(64 * kept_n, latent - col0);
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      T* out = static_cast<T*>(a.out) + (done.b * a.heads + h) * latent + col0;
+      float* part = plan.part_o + (static_cast<int64_t>(done.slot) * kHeads + tid) * latent + col0;
+      for (int c = 0; c < cols; c += 32) {
+        uint32_t o[32];
+        tmem_ld32(tmem + my_lanes + kColO + c, o);
+        tmem_ld_wait();
+        if (!has) continue;
+#pragma unroll
+        for (int j = 0; j < 32; j += 8) {
+          if (c + j >= cols) break;
+          if (done.whole) {
+            uint4 v;
+            v.x = pack2<T>(__uint_as_float(o[j]) * inv, __uint_as_float(o[j + 1]) * inv);
+            v.y = pack2<T>(__uint_as_float(o[j + 2]) * inv, __uint_as_float(o[j + 3]) * inv);
+            v.z = pack2<T>(__uint_as_float(o[j + 4]) * inv, __uint_as_float(o[j + 5]) * inv);
+            v.w = pack2<T>(__uint_as_float(o[j + 6]) * inv, __uint_as_float(o[j + 7]) * inv);
+            *reinterpret_cast<uint4*>(out + c + j) = v;
+          } else {
+            *reinterpret_cast<uint4*>(part + c + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+            *reinterpret_cast<uint4*>(part + c + j + 4) = make_uint4(o[j + 4], o[j + 5], o[j + 6], o[j + 7]);
+          }
+        }
+      }
+      if (half == 0 && has) {
+        if (!done.whole) plan.part_ml[static_cast<int64_t>(done.slot) * kHeads + tid] = make_float2(m, l);
+        else if (a.lse) a.lse[done.b * a.heads + h] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->o_read);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == kAttnWarps - 1) tmem_dealloc(tmem, 512);
+}
+
+// Joins the parts of the rows that were cut, and writes the rows without
+// positions.  A CTA takes two heads of a row; a thread four columns.
+constexpr int kJoinThreads = 256;
+template <typename T>
+__global__ void __launch_bounds__(kJoinThreads) paged_attention_join_kernel(PagedAttnArgs a, AttnPlan plan) {
+  const int64_t pairs = ceil_div(a.heads, 2);
+  const int64_t b = blockIdx.x / pairs, h = (blockIdx.x - b * pairs) * 2 + threadIdx.x / (kJoinThreads / 2);
+  if (h >= a.heads) return;
+  const int64_t c = 4 * (threadIdx.x % (kJoinThreads / 2));
+  const bool in = c < a.latent;
+  const int64_t total = plan.before[a.batch], tiles = (plan.before[b + 1] - plan.before[b]) / plan.groups;
+  T* out = static_cast<T*>(a.out) + (b * a.heads + h) * a.latent + c;
+  if (tiles == 0) {
+    if (in) *reinterpret_cast<uint2*>(out) = make_uint2(0, 0);
+    if (a.lse && c == 0) a.lse[b * a.heads + h] = -INFINITY;
+    return;
+  }
+  const int64_t workers = used_workers(total, plan.workers), group = h / kHeads;
+  const int64_t t0 = plan.before[b] + group * tiles, t1 = t0 + tiles - 1;  // the item's first and last tile
+  const int64_t w0 = ((t0 + 1) * workers - 1) / total, w1 = ((t1 + 1) * workers - 1) / total;
+  if (w0 == w1) return;  // finished where it was computed
+  // the first part is its range's last (unless the range starts with the row), the others open theirs
+  auto at = [&](int64_t w) { return (2 * w + (w == w0 ? 1 : 0)) * kHeads + (h - group * kHeads); };
+  float top = -INFINITY;
+  for (int64_t w = w0; w <= w1; ++w) top = fmaxf(top, plan.part_ml[at(w)].x);
+  if (top == -INFINITY) top = 0.0f;
+  float sum = 0.0f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (int64_t w = w0; w <= w1; ++w) {
+    const float2 ml = plan.part_ml[at(w)];
+    const float f = exp2_fast(ml.x - top);
+    sum = fmaf(ml.y, f, sum);
+    if (in) {
+      const float4 o = *reinterpret_cast<const float4*>(plan.part_o + at(w) * a.latent + c);
+      acc.x = fmaf(o.x, f, acc.x);
+      acc.y = fmaf(o.y, f, acc.y);
+      acc.z = fmaf(o.z, f, acc.z);
+      acc.w = fmaf(o.w, f, acc.w);
+    }
+  }
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  if (in) *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+  if (a.lse && c == 0) a.lse[b * a.heads + h] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
+}
+
+AttnPlan attn_plan(Plan& p, int64_t batch, int64_t heads, int64_t latent, int64_t table_cols, int64_t page_size) {
+  AttnPlan l{};
+  const int64_t halves = latent > 64 ? 2 : 1;
+  l.groups = static_cast<int>(ceil_div(heads, kHeads));
+  // at most one pair of CTAs per pair of SMs, and no more than there can be ranges
+  const int64_t most = batch * l.groups * ceil_div(table_cols * page_size, kTile);
+  l.workers = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(gemv_grid_ctas() / halves, ceil_div(most, kMinTiles))));
+  l.part_o = p.take<float>(2 * l.workers * kHeads * latent);
+  l.part_ml = p.take<float2>(2 * l.workers * kHeads);
+  l.before = p.take<int64_t>(batch + 1);
+  return l;
+}
+
+template <typename T>
+cudaError_t launch_attention(const PagedAttnArgs& a, const AttnPlan& plan, cudaStream_t stream) {
+  cudaError_t err = cudaFuncSetAttribute(paged_attention_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         static_cast<int>(kAttnSmem));
+  if (err != cudaSuccess) return err;
+  const unsigned ctas = static_cast<unsigned>(plan.workers * (a.latent > 64 ? 2 : 1));
+  paged_attention_kernel<T><<<ctas, kAttnThreads, kAttnSmem, stream>>>(a, plan);
+  err = cudaGetLastError();
+  if (err != cudaSuccess) return err;
+  paged_attention_join_kernel<T><<<static_cast<unsigned>(a.batch * ceil_div(a.heads, 2)), kJoinThreads, 0, stream>>>(a, plan);
+  return cudaGetLastError();
 }
 
 }  // namespace
@@ -236,13 +782,16 @@ cudaError_t launch_paged_append(const AppendArgs& a, int x_dtype, int norm_dtype
   return launch_append_types<__half>(a, x_dtype, norm_dtype, stream);
 }
 
-int64_t paged_attn_workspace_bytes(int64_t, int64_t, int64_t, int64_t, int64_t) { return 0; }
+int64_t paged_attn_workspace_bytes(int64_t batch, int64_t heads, int64_t latent, int64_t table_cols, int64_t page_size) {
+  Plan p;
+  attn_plan(p, batch, heads, latent, table_cols, page_size);
+  return static_cast<int64_t>(p.used());
+}
 
-cudaError_t launch_paged_attention(const PagedAttnArgs& a, int dtype, char*, cudaStream_t stream) {
-  const dim3 grid(static_cast<unsigned>(a.heads), static_cast<unsigned>(a.batch));
-  if (dtype == kDtypeBF16) paged_attention_simple_kernel<__nv_bfloat16><<<grid, kSimpleWarps * kWarp, 0, stream>>>(a);
-  else paged_attention_simple_kernel<__half><<<grid, kSimpleWarps * kWarp, 0, stream>>>(a);
-  return cudaGetLastError();
+cudaError_t launch_paged_attention(const PagedAttnArgs& a, int dtype, char* workspace, cudaStream_t stream) {
+  Plan p(workspace);
+  const AttnPlan plan = attn_plan(p, a.batch, a.heads, a.latent, a.table_cols, a.page_size);
+  return dtype == kDtypeBF16 ? launch_attention<__nv_bfloat16>(a, plan, stream) : launch_attention<__half>(a, plan, stream);
 }
 
 int read_and_clear_paged_error(cudaStream_t stream) { return read_and_clear_local_error(stream); }

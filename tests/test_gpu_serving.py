@@ -344,8 +344,9 @@ def test_attention_infinite_and_nan_values_stay_in_their_rows():
     ql = ql.clone()
     ql[2, 5, 7] = math.inf
     out, lse = serving.paged_mla_attention(ql, qp, cache, table, lengths, softmax_scale=scale, return_lse=True)
-    clean = serving.paged_mla_attention(ql[:1], qp[:1], cache, table[:1], lengths[:1], softmax_scale=scale)
-    assert torch.equal(out[0], clean[0]) and not out[0].isnan().any()
+    # not bit by bit what row 0 gives alone: where its positions are cut, and so which maximum its rounded
+    # probabilities are relative to, goes by the whole batch; what the roundings may cost holds either way
+    _check_attn(out[:1], lse[:1], (ql[:1], qp[:1], cache, table[:1], lengths[:1], scale))
     assert bool(out[1, :, 100].isnan().all())
     rest = torch.arange(128, device="cuda") != 5
     assert not out[2, rest].isnan().any() and bool(out[2, 5].isnan().any())
