@@ -623,7 +623,8 @@ int moe_paged_mla_append(const void* kv_rows, int64_t kv_stride, int kv_dtype, c
  * row's last page are not read.  A page outside [0, pages) or a length past
  * the table is skipped and sets code 512 in moe_b200_device_error.
  * kv_lora_rank <= 512 and qk_rope_dim <= 64, both multiples of 8; rows of
- * queries and cache start on 16-byte boundaries; batch <= 65535.  workspace:
+ * queries and cache start on 16-byte boundaries, strides positive; batch <=
+ * 65535.  workspace:
  * moe_paged_mla_attention_workspace_bytes (-1 for dimensions it rejects). */
 int64_t moe_paged_mla_attention_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_lora_rank,
                                                 int64_t qk_rope_dim, int64_t table_cols, int64_t page_size);

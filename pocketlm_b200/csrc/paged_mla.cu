@@ -205,9 +205,16 @@ cudaError_t launch_append_types(const AppendArgs& a, int x_dtype, int norm_dtype
 // one range is finished there; a row that is cut leaves fp32 parts in the
 // workspace, which the second kernel joins.  A range has at most two parts.
 //
-// Warps 0-3: softmax, result (a thread per head).  4-7: cache rows by 16-byte
-// asynchronous copies (any page size; rows past the length arrive as zeros).
-// 8: tensor memory and the products.
+// Warps 0-3: softmax, result (a thread per head).  4-7: the cache's rows.
+// 8: tensor memory and the products (the whole warp walks the work, so that
+// operand descriptors stay in uniform registers; one lane issues).
+//
+// Rows arrive by TMA, one box per chunk and run of positions that no page
+// border cuts (gcd(page size, 64) of them), or, where such runs are shorter than
+// 8, by 16-byte asynchronous copies of four warps.  Positions that do not take
+// part (past the length, or on a page outside the cache) are masked in the scores;
+// their rows may hold anything, NaN among it, so the softmax warps clear them
+// in shared memory before the second product reads them with probability 0.
 constexpr int kTile = 64;
 constexpr int kHeads = 128;
 constexpr int kChunkBytes = kTile * 128;
@@ -246,6 +253,7 @@ struct AttnPlan {
   float2* part_ml;     // [2 workers][128 heads]: reference maximum (log2 domain), sum
   int64_t* before;     // [batch + 1]: tiles before each row
   int workers;         // pairs of CTAs
+  int run;             // positions per TMA box
   int groups;          // groups of 128 heads: an item is a row's group
 };
 
@@ -327,15 +335,18 @@ MOE_D bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int co
   return __all_sync(0xFFFFFFFFu, wait_or_abort(bar, parity, abort, code));
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(PagedAttnArgs a, AttnPlan plan) {
+template <typename T, bool TMA>
+__global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const __grid_constant__ CUtensorMap map_cache,
+                                                                          const __grid_constant__ CUtensorMap map_ql,
+                                                                          const __grid_constant__ CUtensorMap map_qp,
+                                                                          PagedAttnArgs a, AttnPlan plan) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   unsigned char* q_smem = smem;
   unsigned char* kept_smem = q_smem + kQSmemChunks * kQChunkBytes;
   unsigned char* pass_smem = kept_smem + kKeptStages * kKeptChunks * kChunkBytes;
   AttnBarriers* bars = reinterpret_cast<AttnBarriers*>(pass_smem + kPassing * kChunkBytes);
-  const int tid = threadIdx.x, warp = tid / kWarp, lane = tid % kWarp;
+  const int tid = threadIdx.x, lane = tid % kWarp, warp = __shfl_sync(0xFFFFFFFFu, tid / kWarp, 0);
   volatile int* abort = &bars->abort;
   const int latent = static_cast<int>(a.latent), rope = static_cast<int>(a.rope);
   const int lat_chunks = (latent + 63) / 64, chunks = lat_chunks + 1;  // the last one holds the rope part
@@ -387,18 +398,18 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(PagedA
   }
   if (tid == 0) {
     for (int s = 0; s < kKeptStages; ++s) {
-      mbar_init(&bars->kept_full[s], kCopyThreads);
+      mbar_init(&bars->kept_full[s], TMA ? 1 : kCopyThreads);
       mbar_init(&bars->kept_empty[s], 1);
     }
     for (int s = 0; s < kPassing; ++s) {
-      mbar_init(&bars->pass_full[s], kCopyThreads);
+      mbar_init(&bars->pass_full[s], TMA ? 1 : kCopyThreads);
       mbar_init(&bars->pass_empty[s], 1);
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&bars->s_full[s], 1);
       mbar_init(&bars->p_ready[s], kSoftmaxThreads / kWarp);
     }
-    mbar_init(&bars->q_ready, kSoftmaxThreads / kWarp);
+    mbar_init(&bars->q_ready, kSoftmaxThreads / kWarp + 1);
     mbar_init(&bars->o_done, 1);
     mbar_init(&bars->o_read, kSoftmaxThreads / kWarp);
     mbar_init(&bars->drain, 1);
@@ -416,7 +427,71 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(PagedA
   Walk walk{bars->first_item, bars->first_tile, stop - start};
   Part p;
 
-  if (warp >= kSoftmaxThreads / kWarp && warp < kAttnWarps - 1) {
+  if (TMA && warp >= kSoftmaxThreads / kWarp && warp < kAttnWarps - 1) {
+    // --------------------------------------------------------------- TMA
+    if (warp == kSoftmaxThreads / kWarp) {
+      const uint32_t kept_at = smem_addr(kept_smem), pass_at = smem_addr(pass_smem);
+      const int run = plan.run, runs = kTile / run, page_size = static_cast<int>(a.page_size);
+      const bool leader = elect_one();
+      uint32_t g = 0, pc = 0, kept = 0;
+      bool ok = true;
+      // lane r: the page of the tile's run r (-1: none) and its first row there
+      auto lookup = [&](int tile, int& page, int& row) {
+        const int pos = tile * kTile + lane * run;
+        page = -1;
+        row = 0;
+        if (lane < runs && pos < p.len) {
+          const int col = pos / page_size;
+          page = __ldg(a.table + p.b * a.table_stride + col);
+          row = pos - col * page_size;
+          if (page >= a.pages) page = -1;
+        }
+      };
+      while (ok && walk.next(a, plan.groups, worker, p)) {
+        int page, row, next_page = -1, next_row = 0;
+        lookup(p.tile0, page, row);
+        for (int i = 0; i < p.tiles && ok; ++i, ++g) {
+          if (i + 1 < p.tiles) lookup(p.tile0 + i + 1, next_page, next_row);
+          const int present = __popc(__ballot_sync(0xFFFFFFFFu, page >= 0));
+          auto fetch = [&](int c, uint32_t dst, uint64_t* bar) {
+            const int x = c < lat_chunks ? c * 64 : latent;
+            for (int r = 0; r < runs; ++r) {
+              const int pg = __shfl_sync(0xFFFFFFFFu, page, r), at = __shfl_sync(0xFFFFFFFFu, row, r);
+              if (pg >= 0 && leader) tma_load_3d(dst + r * run * 128, &map_cache, x, at, pg, bar);
+            }
+          };
+          const int s = g % kKeptStages;
+          if (g >= kKeptStages && !warp_wait(&bars->kept_empty[s], ((g / kKeptStages) - 1) & 1, abort, kPagedWaitError)) {
+            ok = false;
+            break;
+          }
+          if (leader) mbar_arrive_expect_tx(&bars->kept_full[s], present * run * 128 * kept_n);
+          __syncwarp();
+          ++kept;
+          for (int k = 0; k < kept_n; ++k) fetch(kept0 + k, kept_at + (s * kKeptChunks + k) * kChunkBytes, &bars->kept_full[s]);
+          for (int c = 0; c < chunks; ++c) {
+            if (c >= kept0 && c < kept0 + kept_n) continue;
+            const int slot = pc % kPassing;
+            if (pc >= kPassing && !warp_wait(&bars->pass_empty[slot], ((pc / kPassing) - 1) & 1, abort, kPagedWaitError)) {
+              ok = false;
+              break;
+            }
+            if (leader) mbar_arrive_expect_tx(&bars->pass_full[slot], present * run * 128);
+            __syncwarp();
+            fetch(c, pass_at + slot * kChunkBytes, &bars->pass_full[slot]);
+            ++pc;
+          }
+          page = next_page;
+          row = next_row;
+        }
+      }
+      // every copy issued lands before the CTA may exit
+      for (uint32_t j = kept > kKeptStages ? kept - kKeptStages : 0; j < kept; ++j)
+        mbar_wait(&bars->kept_full[j % kKeptStages], (j / kKeptStages) & 1, kPagedWaitError);
+      for (uint32_t j = pc > kPassing ? pc - kPassing : 0; j < pc; ++j)
+        mbar_wait(&bars->pass_full[j % kPassing], (j / kPassing) & 1, kPagedWaitError);
+    }
+  } else if (!TMA && warp >= kSoftmaxThreads / kWarp && warp < kAttnWarps - 1) {
     // ------------------------------------------------------------ copies
     const int ct = tid - kSoftmaxThreads, unit = ct % 8, row0 = ct / 8;
     const uint32_t kept_at = smem_addr(kept_smem), pass_at = smem_addr(pass_smem);
@@ -472,105 +547,106 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(PagedA
     asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (warp == kAttnWarps - 1) {
     // ---------------------------------------------------------- products
-    if (lane == 0) {
-      const int format = sizeof(T) == 2 && __is_same(T, __nv_bfloat16) ? 1 : 0;
-      const uint32_t idesc_s = umma_idesc(kHeads, kTile, format, false);
-      const uint32_t idesc_o = umma_idesc(kHeads, 64 * kept_n, format, true);
-      const uint32_t q_at = smem_addr(q_smem), kept_at = smem_addr(kept_smem), pass_at = smem_addr(pass_smem);
-      uint32_t g = 0, pc = 0, parts = 0;
-      bool ok = true;
-      auto chunk_scores = [&](int c, uint32_t k_at, uint32_t d, bool first) {
+    const bool leader = elect_one();
+    const int format = __is_same(T, __nv_bfloat16) ? 1 : 0;
+    const uint32_t idesc_s = umma_idesc(kHeads, kTile, format, false);
+    const uint32_t idesc_o = umma_idesc(kHeads, 64 * kept_n, format, true);
+    const uint64_t q_desc = sw128_desc_k(smem_addr(q_smem)), k_desc = sw128_desc_k(smem_addr(kept_smem));
+    const uint64_t pass_desc = sw128_desc_k(smem_addr(pass_smem)), v_desc = sw128_desc(smem_addr(kept_smem), kChunkBytes);
+    uint32_t g = 0, pc = 0, parts = 0;
+    bool ok = true;
+    // descriptors advance in units of 16 bytes: 2 per 16 columns of a swizzled row
+    auto chunk_scores = [&](int c, uint64_t b, uint32_t d, bool first) {
+      if (c < q_tmem) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint64_t b = sw128_desc_k(k_at + k * 32);
-          const uint32_t acc = !(first && k == 0);
-          if (c < q_tmem) umma_f16_ts(d, tmem + kColQ + c * 32 + k * 8, b, idesc_s, acc);
-          else umma_f16_ss(d, sw128_desc_k(q_at + (c - q_tmem) * kQChunkBytes + k * 32), b, idesc_s, acc);
-        }
-      };
-      // the scores of the tile whose number is t
-      auto scores = [&](uint32_t t) {
-        const int s = t % kKeptStages;
-        const uint32_t d = tmem + kColS + (t % 2) * kTile;
-        if (!wait_or_abort(&bars->kept_full[s], (t / kKeptStages) & 1, abort, kPagedWaitError)) return false;
-        fence_proxy_async_shared();
+        for (int k = 0; k < 4; ++k) umma_f16_ts(d, tmem + kColQ + c * 32 + k * 8, b + 2 * k, idesc_s, !(first && k == 0));
+      } else {
+        const uint64_t q = q_desc + (c - q_tmem) * (kQChunkBytes / 16);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) umma_f16_ss(d, q + 2 * k, b + 2 * k, idesc_s, !(first && k == 0));
+      }
+    };
+    // the scores of the tile whose number is t
+    auto scores = [&](uint32_t t) {
+      const uint32_t s = t % kKeptStages, d = tmem + kColS + (t % 2) * kTile;
+      if (!warp_wait(&bars->kept_full[s], (t / kKeptStages) & 1, abort, kPagedWaitError)) return false;
+      if (!TMA) fence_proxy_async_shared();
+      tc_fence_after();
+      for (int k = 0; k < kept_n; ++k)
+        if (leader) chunk_scores(kept0 + k, k_desc + (s * kKeptChunks + k) * (kChunkBytes / 16), d, k == 0);
+      for (int c = 0; c < chunks; ++c) {
+        if (c >= kept0 && c < kept0 + kept_n) continue;
+        const uint32_t slot = pc % kPassing;
+        if (!warp_wait(&bars->pass_full[slot], (pc / kPassing) & 1, abort, kPagedWaitError)) return false;
+        if (!TMA) fence_proxy_async_shared();
         tc_fence_after();
-        for (int k = 0; k < kept_n; ++k) chunk_scores(kept0 + k, kept_at + (s * kKeptChunks + k) * kChunkBytes, d, k == 0);
-        for (int c = 0; c < chunks; ++c) {
-          if (c >= kept0 && c < kept0 + kept_n) continue;
-          const int slot = pc % kPassing;
-          if (!wait_or_abort(&bars->pass_full[slot], (pc / kPassing) & 1, abort, kPagedWaitError)) return false;
-          fence_proxy_async_shared();
-          chunk_scores(c, pass_at + slot * kChunkBytes, d, false);
+        if (leader) {
+          chunk_scores(c, pass_desc + slot * (kChunkBytes / 16), d, false);
           umma_commit(&bars->pass_empty[slot]);
-          ++pc;
         }
-        umma_commit(&bars->s_full[t % 2]);
-        return true;
-      };
-      while (ok && walk.next(a, plan.groups, worker, p)) {
-        if (!wait_or_abort(&bars->q_ready, parts & 1, abort, kPagedWaitError)) break;
+        __syncwarp();
+        ++pc;
+      }
+      if (leader) umma_commit(&bars->s_full[t % 2]);
+      __syncwarp();
+      return true;
+    };
+    while (ok && walk.next(a, plan.groups, worker, p)) {
+      const int tiles = __shfl_sync(0xFFFFFFFFu, p.tiles, 0);
+      if (!warp_wait(&bars->q_ready, parts & 1, abort, kPagedWaitError)) break;
+      tc_fence_after();
+      ok = scores(g);
+      for (int i = 0; i < tiles && ok; ++i, ++g) {
+        if (i + 1 < tiles && !(ok = scores(g + 1))) break;
+        if (!(ok = warp_wait(&bars->p_ready[g % 2], (g / 2) & 1, abort, kPagedWaitError))) break;
+        if (i == 0 && parts > 0 && !(ok = warp_wait(&bars->o_read, (parts - 1) & 1, abort, kPagedWaitError))) break;
         tc_fence_after();
-        ok = scores(g);
-        for (int i = 0; i < p.tiles && ok; ++i, ++g) {
-          if (i + 1 < p.tiles && !(ok = scores(g + 1))) break;
-          if (!(ok = wait_or_abort(&bars->p_ready[g % 2], (g / 2) & 1, abort, kPagedWaitError))) break;
-          if (i == 0 && parts > 0 && !(ok = wait_or_abort(&bars->o_read, (parts - 1) & 1, abort, kPagedWaitError))) break;
-          tc_fence_after();
-          const int s = g % kKeptStages;
-          const uint32_t v_at = kept_at + s * kKeptChunks * kChunkBytes;
+        const uint32_t s = g % kKeptStages;
+        if (leader) {
+          const uint64_t v = v_desc + s * (kKeptChunks * kChunkBytes / 16);
 #pragma unroll
           for (int k = 0; k < kTile / 16; ++k)
-            umma_f16_ts(tmem + kColO, tmem + kColS + (g % 2) * kTile + k * 8, sw128_desc(v_at + k * 2048, kChunkBytes),
-                        idesc_o, i > 0 || k > 0);
+            umma_f16_ts(tmem + kColO, tmem + kColS + (g % 2) * kTile + k * 8, v + k * (2048 / 16), idesc_o, i > 0 || k > 0);
           umma_commit(&bars->kept_empty[s]);
           umma_commit(&bars->o_done);
         }
-        ++parts;
+        __syncwarp();
       }
-      umma_commit(&bars->drain);  // every product issued is complete before tensor memory is freed
-      mbar_wait(&bars->drain, 0, kPagedWaitError);
+      ++parts;
     }
+    if (leader) umma_commit(&bars->drain);  // every product issued is complete before tensor memory is freed
+    __syncwarp();
+    mbar_wait(&bars->drain, 0, kPagedWaitError);
   } else {
     // ------------------------------------------------- softmax and result
     const float c2 = fmaxf(a.scale * kLog2e, 1e-37f);  // above 0: a masked score's -inf stays one
     const uint32_t my_lanes = static_cast<uint32_t>(warp * kWarp) << 16;
     const int page_size = static_cast<int>(a.page_size);
+    // the part's queries: columns from 64 q_tmem on by TMA (absent heads and columns arrive as zeros), the others a
+    // thread its own row, all loads in flight together
     auto load_queries = [&](const Part& p) {
       const int h0 = p.group * kHeads, nh = static_cast<int>(min(a.heads - h0, static_cast<int64_t>(kHeads)));
-      const T* ql = static_cast<const T*>(a.q_latent) + p.b * a.ql_stride + h0 * a.ql_head_stride;
-      const T* qp = static_cast<const T*>(a.q_pe) + p.b * a.qp_stride + h0 * a.qp_head_stride;
-      const uint4 zero = make_uint4(0, 0, 0, 0);
-      for (int c = q_tmem; c < chunks; ++c) {  // eight threads a row, 16 rows at a time
-        const int unit = tid % 8;
-        const bool is_lat = c < lat_chunks;
-        const int col = (is_lat ? c * 64 : 0) + unit * 8;
-        const bool in = col < (is_lat ? latent : rope);
-        uint4 v[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int r = tid / 8 + 16 * j;
-          const T* src = (is_lat ? ql + r * a.ql_head_stride : qp + r * a.qp_head_stride) + col;
-          v[j] = in && r < nh ? __ldg(reinterpret_cast<const uint4*>(src)) : zero;
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int r = tid / 8 + 16 * j;
-          *reinterpret_cast<uint4*>(q_smem + (c - q_tmem) * kQChunkBytes + r * 128 + ((unit ^ (r % 8)) * 16)) = v[j];
-        }
+      if (tid == 0) {
+        mbar_arrive_expect_tx(&bars->q_ready, (chunks - q_tmem) * kQChunkBytes);
+        for (int c = q_tmem; c < chunks; ++c)
+          tma_load_3d(smem_addr(q_smem) + (c - q_tmem) * kQChunkBytes, c < lat_chunks ? &map_ql : &map_qp,
+                      c < lat_chunks ? c * 64 : 0, h0, static_cast<int>(p.b), &bars->q_ready);
       }
-      for (int c = 0; c < q_tmem; ++c) {  // a thread its own row
-        __align__(16) uint32_t v[32];
+      __syncwarp();
+      const T* ql = static_cast<const T*>(a.q_latent) + p.b * a.ql_stride + (h0 + tid) * a.ql_head_stride;
+      __align__(16) uint32_t v[kQTmemChunks][32];
+#pragma unroll
+      for (int c = 0; c < kQTmemChunks; ++c)
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
           const int col = c * 64 + u * 8;
-          *reinterpret_cast<uint4*>(v + 4 * u) =
-              tid < nh && col < latent ? __ldg(reinterpret_cast<const uint4*>(ql + tid * a.ql_head_stride + col)) : zero;
+          *reinterpret_cast<uint4*>(v[c] + 4 * u) = tid < nh && c < q_tmem && col < latent
+                                                        ? __ldg(reinterpret_cast<const uint4*>(ql + col))
+                                                        : make_uint4(0, 0, 0, 0);
         }
-        tmem_st32(tmem + my_lanes + kColQ + c * 32, v);
-      }
+#pragma unroll
+      for (int c = 0; c < kQTmemChunks; ++c) tmem_st32(tmem + my_lanes + kColQ + c * 32, v[c]);
       tmem_st_wait();
-      fence_proxy_async_shared();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->q_ready);
@@ -609,6 +685,14 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(PagedA
 #pragma unroll
           for (int j = 0; j < kTile; ++j)
             if (!(live[j / 32] >> (j % 32) & 1u)) r[j] = 0xFF800000u;  // -inf
+          if (TMA) {  // the scores are complete: nothing reads these rows now but the second product
+            unsigned char* v_at = kept_smem + (g % kKeptStages) * kKeptChunks * kChunkBytes;
+            for (int row = tid / 8; row < kTile; row += kSoftmaxThreads / 8)
+              if (!(live[row / 32] >> (row % 32) & 1u))
+                for (int k = 0; k < kept_n; ++k)
+                  *reinterpret_cast<uint4*>(v_at + k * kChunkBytes + row * 128 + (tid % 8) * 16) = make_uint4(0, 0, 0, 0);
+            fence_proxy_async_shared();
+          }
         }
         float top = -INFINITY;
 #pragma unroll
@@ -756,19 +840,45 @@ AttnPlan attn_plan(Plan& p, int64_t batch, int64_t heads, int64_t latent, int64_
   // at most one pair of CTAs per pair of SMs, and no more than there can be ranges
   const int64_t most = batch * l.groups * ceil_div(table_cols * page_size, kTile);
   l.workers = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(gemv_grid_ctas() / halves, ceil_div(most, kMinTiles))));
+  l.run = 1;
+  while (l.run < kTile && page_size % (2 * l.run) == 0) l.run *= 2;
   l.part_o = p.take<float>(2 * l.workers * kHeads * latent);
   l.part_ml = p.take<float2>(2 * l.workers * kHeads);
   l.before = p.take<int64_t>(batch + 1);
   return l;
 }
 
+// A tensor [z][y][x] of 16-bit values with a box of 64 columns and `rows` rows, 128B-swizzled.
+template <typename T>
+bool encode_rows(CUtensorMap* map, const void* base, int64_t x, int64_t y, int64_t z, int64_t y_stride, int64_t z_stride,
+                 int rows) {
+  const auto encode = tensor_map_encoder();
+  if (!encode) return false;
+  // a dimension of one has no stride of its own, but the map wants one
+  if (y == 1) y_stride = 64;
+  if (z == 1) z_stride = 64;
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(x), static_cast<cuuint64_t>(y), static_cast<cuuint64_t>(z)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(y_stride) * 2, static_cast<cuuint64_t>(z_stride) * 2};
+  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(rows), 1}, steps[3] = {1, 1, 1};
+  return encode(map, __is_same(T, __nv_bfloat16) ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                const_cast<void*>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T>
 cudaError_t launch_attention(const PagedAttnArgs& a, const AttnPlan& plan, cudaStream_t stream) {
-  cudaError_t err = cudaFuncSetAttribute(paged_attention_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         static_cast<int>(kAttnSmem));
+  const bool tma = plan.run >= 8;
+  CUtensorMap cache{}, ql, qp;
+  if (!encode_rows<T>(&ql, a.q_latent, a.latent, a.heads, a.batch, a.ql_head_stride, a.ql_stride, kHeads) ||
+      !encode_rows<T>(&qp, a.q_pe, a.rope, a.heads, a.batch, a.qp_head_stride, a.qp_stride, kHeads) ||
+      (tma && !encode_rows<T>(&cache, a.cache, a.latent + a.rope, a.page_size, a.pages, a.row_stride, a.page_stride, plan.run)))
+    return cudaErrorInvalidValue;
+  auto kernel = tma ? paged_attention_kernel<T, true> : paged_attention_kernel<T, false>;
+  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kAttnSmem));
   if (err != cudaSuccess) return err;
   const unsigned ctas = static_cast<unsigned>(plan.workers * (a.latent > 64 ? 2 : 1));
-  paged_attention_kernel<T><<<ctas, kAttnThreads, kAttnSmem, stream>>>(a, plan);
+  kernel<<<ctas, kAttnThreads, kAttnSmem, stream>>>(cache, ql, qp, a, plan);
   err = cudaGetLastError();
   if (err != cudaSuccess) return err;
   paged_attention_join_kernel<T><<<static_cast<unsigned>(a.batch * ceil_div(a.heads, 2)), kJoinThreads, 0, stream>>>(a, plan);

@@ -127,6 +127,10 @@ int moe_paged_mla_attention(const void* q_latent, int64_t ql_stride, int64_t ql_
         reinterpret_cast<uintptr_t>(out)) & 15u) ||
       (ql_stride | ql_head_stride | qp_stride | qp_head_stride | page_stride | row_stride) % 8)
     return fail(kUnsupported, "rows of queries and cache must start on 16-byte boundaries");
+  // (a dimension of one has no stride)
+  if ((batch > 1 && (ql_stride <= 0 || qp_stride <= 0)) || (heads > 1 && (ql_head_stride <= 0 || qp_head_stride <= 0)) ||
+      (pages > 1 && page_stride <= 0) || (page_size > 1 && row_stride <= 0))
+    return fail(kUnsupported, "strides must be positive");
   if (batch == 0) return kOk;
   PagedAttnArgs a{};
   a.q_latent = q_latent; a.q_pe = q_pe; a.cache = cache; a.table = page_table; a.lengths = lengths; a.out = out;

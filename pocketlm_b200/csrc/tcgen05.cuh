@@ -2,6 +2,9 @@
 // that the serving kernels share: tensor memory, tcgen05.mma, its commits,
 // operand descriptors and the bounded waits of a CTA whose warps have roles.
 #pragma once
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
 #include "async_copy.cuh"
 #include "common.cuh"
 
@@ -77,6 +80,27 @@ MOE_D void tmem_st32(uint32_t taddr, const uint32_t* r) {
       : "memory");
 }
 
+// One lane of a converged warp, the same one every time.
+MOE_D bool elect_one() {
+  uint32_t is;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xFFFFFFFF;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(is));
+  return is != 0;
+}
+
+MOE_D void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          dst),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar))
+      : "memory");
+}
+MOE_D void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(smem_addr(bar))
+      : "memory");
+}
+
 // Shared-memory operand descriptors, 128B swizzle (rows of 128 bytes whose
 // 16-byte units are XORed with the row's index mod 8, atoms of 8 rows).
 // K-major: a row holds consecutive k; atoms of 8 rows of M or N are 1024
@@ -112,6 +136,19 @@ MOE_D bool wait_or_abort(uint64_t* bar, uint32_t parity, volatile int* abort, in
     }
   }
   return true;
+}
+
+// The driver's cuTensorMapEncodeTiled (no link against libcuda), or null.
+inline PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
+  static const auto fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &r) != cudaSuccess ||
+        r != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+  }();
+  return fn;
 }
 
 }  // namespace moe

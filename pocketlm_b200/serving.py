@@ -221,8 +221,9 @@ def paged_mla_append(kv_rows: torch.Tensor, kv_norm_weight: torch.Tensor, cache:
 
 
 def _query(t: torch.Tensor) -> torch.Tensor:
-    """Queries whose rows start on 16-byte boundaries (a copy where they do not)."""
-    if t.stride(2) == 1 and t.stride(0) % 8 == 0 and t.stride(1) % 8 == 0 and t.data_ptr() % 16 == 0:
+    """Queries whose rows start on 16-byte boundaries and are stored one by one (a copy where they are not)."""
+    s0, s1, s2 = t.stride()
+    if s2 == 1 and s0 > 0 and s1 > 0 and s0 % 8 == 0 and s1 % 8 == 0 and t.data_ptr() % 16 == 0:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
