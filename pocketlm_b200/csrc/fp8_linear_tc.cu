@@ -1,54 +1,485 @@
 // The block-scaled FP8 linear for batches whose rows are e4m3 too:
 //   out[t, n] = sum_g sx[t, g] sw[n / 128, g] sum_{k in group g} x[t, k] w[n, k],
-// groups of 128 columns, 128 x 128 weight blocks; products and sums in fp32,
-// one rounding to the output's type.
+// groups of 128 columns, 128 x 128 weight blocks.  A group's products are summed
+// by tcgen05.mma kind::f8f6f4 (four steps of K = 32, exact products, fp32
+// sums in tensor memory); its sum leaves tensor memory once and is added, times
+// the group's scales, to an fp32 sum in registers.  One rounding to the
+// output's type.  A 128-column group of e4m3 is one row of the 128B swizzle,
+// so a pipeline stage is one group of both operands, loaded by TMA as stored;
+// absent rows and columns arrive as zeros.
+//
+// Few rows (linear_rows_kernel): the weights' bytes bound it.  The weight's rows
+// are M (128 of them per CTA), the tokens N (16 to 128), so no tensor work is
+// spent on absent tokens; the groups are cut over the CTAs of a cluster, whose
+// sums are added through distributed shared memory in rank order (the same
+// result on every run).
+//
+// Many rows (linear_tiles_kernel): the tensor cores bound it.  128 tokens x 256
+// outputs per CTA and tile, two 256-column accumulators so that the sums of one
+// group are read while the next is computed; persistent CTAs.
 #include <algorithm>
 
-#include "async_copy.cuh"
 #include "fp8_gemv.cuh"
 #include "router.cuh"
 #include "serving.cuh"
+#include "tcgen05.cuh"
 
 namespace moe {
 namespace {
 
-// A 64 x 64 tile of the output per CTA, 16 columns of k a step.
-constexpr int kT = 64, kK = 16;
+constexpr int kGroup = 128;  // columns per scale group: a stage of the pipeline
+
 template <typename O>
-__global__ void __launch_bounds__(256) fp8_linear_simple_kernel(LinearArgs a) {
-  __shared__ float xs[kK][kT + 4], ws[kK][kT + 4];
-  const int64_t t0 = static_cast<int64_t>(blockIdx.y) * kT, n0 = static_cast<int64_t>(blockIdx.x) * kT;
-  const int64_t kb = ceil_div(a.cols, 128);
-  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-  float acc[4][4] = {};
-  for (int64_t k0 = 0; k0 < a.cols; k0 += kK) {
-    for (int i = threadIdx.x; i < kT * kK; i += 256) {
-      const int r = i / kK, c = i % kK;
-      const int64_t k = k0 + c, t = t0 + r, n = n0 + r;
-      xs[c][r] = t < a.rows && k < a.cols ? e4m3x2_to_float2(a.x[t * a.x_stride + k]).x * a.x_scales[t * kb + k / 128] : 0.0f;
-      ws[c][r] = n < a.outs && k < a.cols ? e4m3x2_to_float2(a.w[n * a.w_stride + k]).x * a.w_scales[n / 128 * kb + k / 128] : 0.0f;
+MOE_D O out_value(float v);
+template <>
+MOE_D float out_value<float>(float v) { return v; }
+template <>
+MOE_D __nv_bfloat16 out_value<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <>
+MOE_D __half out_value<__half>(float v) { return __float2half_rn(v); }
+
+MOE_D bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  return __all_sync(0xFFFFFFFFu, wait_or_abort(bar, parity, abort, kLinearWaitError));
+}
+
+// ------------------------------------------------------------------ few rows
+
+constexpr int kRowsThreads = 192;  // warps 0-3: sums (a thread per weight row); 4: TMA; 5: products
+constexpr int kWTileBytes = 128 * kGroup;
+template <int NT>
+struct RowsShape {
+  static constexpr int kStages = NT <= 32 ? 5 : NT <= 64 ? 4 : 3;
+  static constexpr int kBufs = NT <= 64 ? 4 : 2;  // accumulators in tensor memory
+  static constexpr int kCols = NT * kBufs < 32 ? 32 : NT * kBufs;
+  static constexpr int kStageBytes = kWTileBytes + NT * kGroup;
+  static constexpr int kPipeBytes = kStages * kStageBytes;
+};
+template <int NT>
+struct RowsBarriers {
+  uint64_t full[RowsShape<NT>::kStages], empty[RowsShape<NT>::kStages];
+  uint64_t sum_full[RowsShape<NT>::kBufs], sum_empty[RowsShape<NT>::kBufs];
+  uint64_t drain;
+  uint32_t tmem_base;
+  int abort;
+};
+
+
+template <int NT>
+size_t rows_smem(int groups) {
+  return 1024 + RowsShape<NT>::kPipeBytes + sizeof(float) * NT * groups + sizeof(RowsBarriers<NT>);
+}
+
+MOE_D uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+MOE_D void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+MOE_D float4 ld_cluster(uint32_t addr, uint32_t rank) {
+  uint32_t at;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(addr), "r"(rank));
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(at)
+               : "memory");
+  return v;
+}
+
+// grid: (tile of 128 weight rows x cluster, tile of NT tokens); rank r of a
+// cluster of S takes groups [r G / S, (r + 1) G / S).
+template <typename O, int NT>
+__global__ void __launch_bounds__(kRowsThreads) linear_rows_kernel(const __grid_constant__ CUtensorMap map_x,
+                                                                   const __grid_constant__ CUtensorMap map_w, LinearArgs a,
+                                                                   int splits, int max_groups) {
+  using Shape = RowsShape<NT>;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* factor = reinterpret_cast<float*>(smem + Shape::kPipeBytes);  // [group][token]: the two scales' product
+  auto* bars = reinterpret_cast<RowsBarriers<NT>*>(factor + NT * max_groups);
+  const int tid = threadIdx.x, lane = tid % kWarp, warp = __shfl_sync(0xFFFFFFFFu, tid / kWarp, 0);
+  volatile int* abort = &bars->abort;
+  const int rank = splits > 1 ? static_cast<int>(cluster_rank()) : 0;
+  const int tile = blockIdx.x / splits, n0 = tile * 128, t0 = blockIdx.y * NT;
+  const int groups_all = static_cast<int>((a.cols + kGroup - 1) / kGroup);
+  const int g0 = static_cast<int>(static_cast<int64_t>(rank) * groups_all / splits);
+  const int groups = static_cast<int>(static_cast<int64_t>(rank + 1) * groups_all / splits) - g0;
+
+  if (tid == 0) {
+    for (int s = 0; s < Shape::kStages; ++s) {
+      mbar_init(&bars->full[s], 1);
+      mbar_init(&bars->empty[s], 1);
     }
-    __syncthreads();
-    for (int c = 0; c < kK; ++c)
-      for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(xs[c][ty * 4 + i], ws[c][tx * 4 + j], acc[i][j]);
-    __syncthreads();
+    for (int b = 0; b < Shape::kBufs; ++b) {
+      mbar_init(&bars->sum_full[b], 1);
+      mbar_init(&bars->sum_empty[b], 4);
+    }
+    mbar_init(&bars->drain, 1);
+    bars->abort = 0;
+    fence_barrier_init();
   }
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int64_t t = t0 + ty * 4 + i, n = n0 + tx * 4 + j;
-      if (t < a.rows && n < a.outs) static_cast<O*>(a.out)[t * a.outs + n] = static_cast<O>(acc[i][j]);
+  if (warp == 5) {
+    tmem_alloc(&bars->tmem_base, Shape::kCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars->tmem_base;
+  float acc[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) acc[j] = 0.0f;
+
+  if (warp == 4) {
+    const bool leader = elect_one();
+    const uint32_t at = smem_addr(smem);
+    int i = 0;
+    for (; i < groups; ++i) {
+      const int s = i % Shape::kStages;
+      if (i >= Shape::kStages && !warp_wait(&bars->empty[s], ((i / Shape::kStages) - 1) & 1, abort)) break;
+      if (leader) {
+        mbar_arrive_expect_tx(&bars->full[s], Shape::kStageBytes);
+        tma_load_2d(at + s * Shape::kStageBytes, &map_w, (g0 + i) * kGroup, n0, &bars->full[s]);
+        tma_load_2d(at + s * Shape::kStageBytes + kWTileBytes, &map_x, (g0 + i) * kGroup, t0, &bars->full[s]);
+      }
+      __syncwarp();
     }
+    for (int j = std::max(0, i - Shape::kStages); j < i; ++j)  // every copy issued lands before the memory is reused
+      mbar_wait(&bars->full[j % Shape::kStages], (j / Shape::kStages) & 1, kLinearWaitError);
+  } else if (warp == 5) {
+    const bool leader = elect_one();
+    const uint32_t idesc = umma_idesc(128, NT, 0, false);
+    const uint64_t w_desc = sw128_desc_k(smem_addr(smem)), x_desc = sw128_desc_k(smem_addr(smem) + kWTileBytes);
+    for (int i = 0; i < groups; ++i) {
+      const int s = i % Shape::kStages, b = i % Shape::kBufs;
+      if (!warp_wait(&bars->full[s], (i / Shape::kStages) & 1, abort) ||
+          (i >= Shape::kBufs && !warp_wait(&bars->sum_empty[b], ((i / Shape::kBufs) - 1) & 1, abort)))
+        break;
+      tc_fence_after();
+      if (leader) {
+        const uint64_t step = static_cast<uint64_t>(s * (Shape::kStageBytes / 16));
+#pragma unroll
+        for (int k = 0; k < kGroup / 32; ++k) umma_f8_ss(tmem + b * NT, w_desc + step + 2 * k, x_desc + step + 2 * k, idesc, k > 0);
+        umma_commit(&bars->empty[s]);
+        umma_commit(&bars->sum_full[b]);
+      }
+      __syncwarp();
+    }
+    if (leader) umma_commit(&bars->drain);
+    __syncwarp();
+    mbar_wait(&bars->drain, 0, kLinearWaitError);
+  } else {
+    // the groups' factors: a token's scales are consecutive
+    for (int i = tid; i < NT * groups; i += 128) {
+      const int t = i / groups, g = i - t * groups;
+      const float sw = __ldg(a.w_scales + static_cast<int64_t>(tile) * groups_all + g0 + g);
+      factor[g * NT + t] = t0 + t < a.rows ? __ldg(a.x_scales + static_cast<int64_t>(t0 + t) * groups_all + g0 + g) * sw : 0.0f;
+    }
+    named_barrier_sync(1, 128);
+    const uint32_t my_lanes = static_cast<uint32_t>(warp * kWarp) << 16;
+    for (int i = 0; i < groups; ++i) {
+      const int b = i % Shape::kBufs;
+      if (!warp_wait(&bars->sum_full[b], (i / Shape::kBufs) & 1, abort)) break;
+      tc_fence_after();
+      const float4* f4 = reinterpret_cast<const float4*>(factor + i * NT);
+#pragma unroll
+      for (int c = 0; c < NT; c += 16) {
+        uint32_t d[16];
+        tmem_ld16(tmem + my_lanes + b * NT + c, d);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+          const float4 f = f4[(c + j) / 4];
+          acc[c + j] = fmaf(__uint_as_float(d[j]), f.x, acc[c + j]);
+          acc[c + j + 1] = fmaf(__uint_as_float(d[j + 1]), f.y, acc[c + j + 1]);
+          acc[c + j + 2] = fmaf(__uint_as_float(d[j + 2]), f.z, acc[c + j + 2]);
+          acc[c + j + 3] = fmaf(__uint_as_float(d[j + 3]), f.w, acc[c + j + 3]);
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->sum_empty[b]);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 5) tmem_dealloc(tmem, Shape::kCols);
+
+  O* out = static_cast<O*>(a.out);
+  if (splits == 1) {
+    const int64_t n = n0 + tid;
+    if (tid < 128 && n < a.outs) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+        if (t0 + j < a.rows) out[(t0 + j) * a.outs + n] = out_value<O>(acc[j]);
+    }
+    return;
+  }
+  // the cluster's sums: each CTA's [NT][128] in its own shared memory (the
+  // pipeline's, now idle), a share of the tokens added up by each
+  float* part = reinterpret_cast<float*>(smem);
+  if (tid < 128) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j) part[j * 128 + tid] = acc[j];
+  }
+  cluster_sync();
+  for (int i = tid; i < NT * 32 / splits; i += kRowsThreads) {
+    const int e = i + rank * (NT * 32 / splits), t = e / 32, c = (e % 32) * 4;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int r = 0; r < splits; ++r) {
+      const float4 v = ld_cluster(smem_addr(part + t * 128 + c), r);
+      sum.x += v.x;
+      sum.y += v.y;
+      sum.z += v.z;
+      sum.w += v.w;
+    }
+    if (t0 + t >= a.rows) continue;
+    const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (n0 + c + j < a.outs) out[(t0 + t) * a.outs + n0 + c + j] = out_value<O>(v[j]);
+  }
+  cluster_sync();  // nobody leaves while its sums are being read
+}
+
+// ----------------------------------------------------------------- many rows
+
+constexpr int kTileM = 128, kTileN = 256, kTileStages = 4;
+constexpr int kTileABytes = kTileM * kGroup, kTileBBytes = kTileN * kGroup, kTileStageBytes = kTileABytes + kTileBBytes;
+constexpr int kSumWarps = 8;  // warp w: rows 32 (w % 4) .. + 31, columns 128 (w / 4) .. + 127
+constexpr int kTilesThreads = (kSumWarps + 2) * kWarp;
+struct TilesBarriers {
+  uint64_t full[kTileStages], empty[kTileStages];
+  uint64_t sum_full[2], sum_empty[2];
+  uint64_t drain;
+  uint32_t tmem_base;
+  int abort;
+};
+constexpr size_t kTilesSmem = 1024 + kTileStages * kTileStageBytes + sizeof(TilesBarriers);
+static_assert(kTilesSmem <= 232448, "shared memory per block");
+
+template <typename O>
+__global__ void __launch_bounds__(kTilesThreads, 1) linear_tiles_kernel(const __grid_constant__ CUtensorMap map_x,
+                                                                        const __grid_constant__ CUtensorMap map_w,
+                                                                        LinearArgs a, int m_tiles, int n_tiles) {
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  TilesBarriers* bars = reinterpret_cast<TilesBarriers*>(smem + kTileStages * kTileStageBytes);
+  const int tid = threadIdx.x, lane = tid % kWarp, warp = __shfl_sync(0xFFFFFFFFu, tid / kWarp, 0);
+  volatile int* abort = &bars->abort;
+  const int groups = static_cast<int>((a.cols + kGroup - 1) / kGroup);
+  const int tiles = m_tiles * n_tiles;
+
+  if (tid == 0) {
+    for (int s = 0; s < kTileStages; ++s) {
+      mbar_init(&bars->full[s], 1);
+      mbar_init(&bars->empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&bars->sum_full[b], 1);
+      mbar_init(&bars->sum_empty[b], kSumWarps);
+    }
+    mbar_init(&bars->drain, 1);
+    bars->abort = 0;
+    fence_barrier_init();
+  }
+  if (warp == kSumWarps + 1) {
+    tmem_alloc(&bars->tmem_base, 2 * kTileN);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars->tmem_base;
+
+  if (warp == kSumWarps) {
+    const bool leader = elect_one();
+    const uint32_t at = smem_addr(smem);
+    uint32_t i = 0;
+    for (int t = blockIdx.x; t < tiles && !*abort; t += gridDim.x) {
+      const int m0 = t % m_tiles * kTileM, n0 = t / m_tiles * kTileN;
+      for (int g = 0; g < groups; ++g, ++i) {
+        const uint32_t s = i % kTileStages;
+        if (i >= kTileStages && !warp_wait(&bars->empty[s], ((i / kTileStages) - 1) & 1, abort)) break;
+        if (leader) {
+          mbar_arrive_expect_tx(&bars->full[s], kTileStageBytes);
+          tma_load_2d(at + s * kTileStageBytes, &map_x, g * kGroup, m0, &bars->full[s]);
+          tma_load_2d(at + s * kTileStageBytes + kTileABytes, &map_w, g * kGroup, n0, &bars->full[s]);
+        }
+        __syncwarp();
+      }
+    }
+    for (uint32_t j = i > kTileStages ? i - kTileStages : 0; j < i; ++j)
+      mbar_wait(&bars->full[j % kTileStages], (j / kTileStages) & 1, kLinearWaitError);
+  } else if (warp == kSumWarps + 1) {
+    const bool leader = elect_one();
+    const uint32_t idesc = umma_idesc(kTileM, kTileN, 0, false);
+    const uint64_t x_desc = sw128_desc_k(smem_addr(smem)), w_desc = sw128_desc_k(smem_addr(smem) + kTileABytes);
+    uint32_t i = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      for (int g = 0; g < groups; ++g, ++i) {
+        const uint32_t s = i % kTileStages, b = i % 2;
+        if (!warp_wait(&bars->full[s], (i / kTileStages) & 1, abort) ||
+            (i >= 2 && !warp_wait(&bars->sum_empty[b], ((i / 2) - 1) & 1, abort))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        if (leader) {
+          const uint64_t step = static_cast<uint64_t>(s * (kTileStageBytes / 16));
+#pragma unroll
+          for (int k = 0; k < kGroup / 32; ++k)
+            umma_f8_ss(tmem + b * kTileN, x_desc + step + 2 * k, w_desc + step + 2 * k, idesc, k > 0);
+          umma_commit(&bars->empty[s]);
+          umma_commit(&bars->sum_full[b]);
+        }
+        __syncwarp();
+      }
+    }
+    if (leader) umma_commit(&bars->drain);
+    __syncwarp();
+    mbar_wait(&bars->drain, 0, kLinearWaitError);
+  } else {
+    const int quad = warp % 4, half = warp / 4;
+    const uint32_t from = tmem + (static_cast<uint32_t>(quad * kWarp) << 16) + half * 128;
+    uint32_t i = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      const int64_t row = t % m_tiles * kTileM + quad * kWarp + lane, n0 = t / m_tiles * kTileN + half * 128;
+      const float* sx = a.x_scales + std::min<int64_t>(row, a.rows - 1) * groups;
+      const float* sw = a.w_scales + std::min<int64_t>(n0, a.outs - 1) / 128 * groups;
+      float acc[128];
+#pragma unroll
+      for (int j = 0; j < 128; ++j) acc[j] = 0.0f;
+      float next = __ldg(sx) * __ldg(sw);
+      for (int g = 0; g < groups; ++g, ++i) {
+        const uint32_t b = i % 2;
+        const float f = next;
+        if (g + 1 < groups) next = __ldg(sx + g + 1) * __ldg(sw + g + 1);
+        if (!warp_wait(&bars->sum_full[b], (i / 2) & 1, abort)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < 128; c += 32) {
+          uint32_t d[32];
+          tmem_ld32(from + b * kTileN + c, d);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) acc[c + j] = fmaf(__uint_as_float(d[j]), f, acc[c + j]);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->sum_empty[b]);
+      }
+      if (!ok) break;
+      if (row < a.rows) {
+        O* out = static_cast<O*>(a.out) + row * a.outs + n0;
+        constexpr int kV = 16 / sizeof(O);
+        if (n0 + 128 <= a.outs && a.outs % kV == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15u) == 0) {
+#pragma unroll
+          for (int j = 0; j < 128; j += kV) {
+            __align__(16) O v[kV];
+#pragma unroll
+            for (int k = 0; k < kV; ++k) v[k] = out_value<O>(acc[j + k]);
+            *reinterpret_cast<uint4*>(out + j) = *reinterpret_cast<const uint4*>(v);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 128; ++j)
+            if (n0 + j < a.outs) out[j] = out_value<O>(acc[j]);
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == kSumWarps + 1) tmem_dealloc(tmem, 2 * kTileN);
+}
+
+// [rows][cols] bytes with a box of one group's columns and `box` rows, 128B-swizzled.
+bool encode_codes(CUtensorMap* map, const uint8_t* base, int64_t rows, int64_t cols, int64_t stride, int box) {
+  const auto encode = tensor_map_encoder();
+  if (!encode) return false;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride)};
+  const cuuint32_t boxes[2] = {kGroup, static_cast<cuuint32_t>(box)}, steps[2] = {1, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(base), dims, strides, boxes, steps,
+                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename O>
+cudaError_t launch_tiles(const LinearArgs& a, cudaStream_t stream);
+
+template <typename O, int NT>
+cudaError_t launch_rows(const LinearArgs& a, cudaStream_t stream) {
+  CUtensorMap mx, mw;
+  if (!encode_codes(&mx, a.x, a.rows, a.cols, a.x_stride, NT) || !encode_codes(&mw, a.w, a.outs, a.cols, a.w_stride, 128))
+    return cudaErrorInvalidValue;
+  const int64_t tiles = ceil_div(a.outs, 128), groups = ceil_div(a.cols, kGroup), token_tiles = ceil_div(a.rows, NT);
+  // the largest cluster that keeps at least two groups per CTA and two CTAs per SM
+  int splits = 1;
+  while (splits < 8 && tiles * token_tiles * splits * 2 <= 2 * gemv_grid_ctas() && groups >= splits * 4) splits *= 2;
+  const int max_groups = static_cast<int>(ceil_div(groups, splits));
+  auto kernel = linear_rows_kernel<O, NT>;
+  const size_t smem = rows_smem<NT>(max_groups);
+  if (smem > 232448) return launch_tiles<O>(a, stream);  // the factors of so many groups do not fit
+  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  if (err != cudaSuccess) return err;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(static_cast<unsigned>(tiles * splits), static_cast<unsigned>(token_tiles));
+  config.blockDim = dim3(kRowsThreads);
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = static_cast<unsigned>(splits);
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, kernel, mx, mw, a, splits, max_groups);
+}
+
+template <typename O>
+cudaError_t launch_tiles(const LinearArgs& a, cudaStream_t stream) {
+  CUtensorMap mx, mw;
+  if (!encode_codes(&mx, a.x, a.rows, a.cols, a.x_stride, kTileM) || !encode_codes(&mw, a.w, a.outs, a.cols, a.w_stride, kTileN))
+    return cudaErrorInvalidValue;
+  auto kernel = linear_tiles_kernel<O>;
+  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kTilesSmem));
+  if (err != cudaSuccess) return err;
+  const int64_t m_tiles = ceil_div(a.rows, kTileM), n_tiles = ceil_div(a.outs, kTileN);
+  if (m_tiles * n_tiles > INT32_MAX) return cudaErrorInvalidValue;
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(m_tiles * n_tiles, gemv_grid_ctas()));
+  kernel<<<grid, kTilesThreads, kTilesSmem, stream>>>(mx, mw, a, static_cast<int>(m_tiles), static_cast<int>(n_tiles));
+  return cudaGetLastError();
+}
+
+template <typename O>
+cudaError_t launch_linear(const LinearArgs& a, cudaStream_t stream) {
+  if (a.rows <= 16) return launch_rows<O, 16>(a, stream);
+  if (a.rows <= 32) return launch_rows<O, 32>(a, stream);
+  if (a.rows <= 64) return launch_rows<O, 64>(a, stream);
+  // 128 x 256 tiles once they fill the SMs, smaller and cut ones until then
+  if (ceil_div(a.rows, kTileM) * ceil_div(a.outs, kTileN) * 2 < gemv_grid_ctas()) return launch_rows<O, 128>(a, stream);
+  return launch_tiles<O>(a, stream);
 }
 
 }  // namespace
 
 cudaError_t launch_fp8_linear(const LinearArgs& a, int out_dtype, cudaStream_t stream) {
-  const dim3 grid(static_cast<unsigned>(ceil_div(a.outs, kT)), static_cast<unsigned>(ceil_div(a.rows, kT)));
-  if (out_dtype == kDtypeF32) fp8_linear_simple_kernel<float><<<grid, 256, 0, stream>>>(a);
-  else if (out_dtype == kDtypeBF16) fp8_linear_simple_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(a);
-  else fp8_linear_simple_kernel<__half><<<grid, 256, 0, stream>>>(a);
-  return cudaGetLastError();
+  switch (out_dtype) {
+    case kDtypeF32: return launch_linear<float>(a, stream);
+    case kDtypeBF16: return launch_linear<__nv_bfloat16>(a, stream);
+    default: return launch_linear<__half>(a, stream);
+  }
 }
 
 int read_and_clear_linear_error(cudaStream_t stream) { return read_and_clear_local_error(stream); }
