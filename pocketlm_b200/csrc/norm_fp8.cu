@@ -14,6 +14,8 @@
 // mean and the codes).  Eight consecutive columns belong to a thread, so
 // sixteen neighbouring lanes hold a scale group and find its amax with four
 // shuffles.
+#include <algorithm>
+
 #include "fp8_gemv.cuh"
 #include "router.cuh"
 #include "serving.cuh"
@@ -47,34 +49,42 @@ MOE_D __half from_float<__half>(float v) { return __float2half_rn(v); }
 template <typename T>
 MOE_D float widen(T v) { return static_cast<float>(v); }
 
-// Eight columns of a row: 16-byte accesses when VEC (whole and aligned), else
-// one element at a time, `n` of them present.
+// Eight columns of a row as they are stored: 16-byte accesses when VEC (whole
+// and aligned), else one element at a time, `n` of them present.
+template <typename T>
+struct alignas(16) Eight {
+  T v[8];
+};
 template <typename T, bool VEC>
-MOE_D void load8(const T* p, int n, float (&f)[8]) {
+MOE_D void load8(const T* p, int n, Eight<T>& e) {
   if (VEC) {
-    constexpr int kV = 16 / sizeof(T);
 #pragma unroll
-    for (int i = 0; i < 8 / kV; ++i) unpack16<T>(__ldg(reinterpret_cast<const uint4*>(p) + i), f + i * kV);
+    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
+      reinterpret_cast<uint4*>(e.v)[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = i < n ? widen<T>(p[i]) : 0.0f;
+    for (int i = 0; i < 8; ++i) e.v[i] = i < n ? p[i] : from_float<T>(0.0f);
   }
 }
 template <typename T, bool VEC>
-MOE_D void store8(T* p, int n, const float (&f)[8]) {
+MOE_D void store8(T* p, int n, const Eight<T>& e) {
   if (VEC) {
-    __align__(16) T v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = from_float<T>(f[i]);
-#pragma unroll
-    for (int i = 0; i < 8 * static_cast<int>(sizeof(T)) / 16; ++i)
-      reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(v)[i];
+    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
+      reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(e.v)[i];
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (i < n) p[i] = from_float<T>(f[i]);
+      if (i < n) p[i] = e.v[i];
   }
 }
+template <typename T>
+MOE_D void clear8(Eight<T>& e) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) e.v[i] = from_float<T>(0.0f);
+}
+
+MOE_D int columns_from(int64_t c, int64_t cols) { return static_cast<int>(cols - c < 8 ? cols - c : 8); }
 
 // The group's scale and this lane's eight codes; the sixteen lanes of a group
 // are neighbours and all take part.
@@ -86,10 +96,18 @@ MOE_D void codes8(const float (&y)[8], int n, uint8_t* codes, float* scale, bool
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
   const float s = max_nan(amax, kTinyAmax) / kE4m3Max;
-  const float inv = 1.0f / s;  // a code off by its neighbour only within 2 ulp of a rounding border
+  const float inv = 1.0f / s;
   if (n <= 0) return;
-  const uint32_t lo = e4m3x2(y[0] * inv, y[1] * inv) | e4m3x2(y[2] * inv, y[3] * inv) << 16;
-  const uint32_t hi = e4m3x2(y[4] * inv, y[5] * inv) | e4m3x2(y[6] * inv, y[7] * inv) << 16;
+  // y / s: the product with the reciprocal and one Newton step on its remainder (an infinite scale's
+  // remainder is none: 0 * inf), so that a value on the border between two codes goes to the even one
+  float q[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float p = y[i] * inv;
+    q[i] = inv == 0.0f ? p : fmaf(fmaf(-p, s, y[i]), inv, p);
+  }
+  const uint32_t lo = e4m3x2(q[0], q[1]) | e4m3x2(q[2], q[3]) << 16;
+  const uint32_t hi = e4m3x2(q[4], q[5]) | e4m3x2(q[6], q[7]) << 16;
   if (VEC) {
     *reinterpret_cast<uint2*>(codes) = make_uint2(lo, hi);
   } else {
@@ -100,75 +118,100 @@ MOE_D void codes8(const float (&y)[8], int n, uint8_t* codes, float* scale, bool
   if (first) *scale = s;
 }
 
-MOE_D int columns_from(int64_t c, int64_t cols) { return static_cast<int>(cols - c < 8 ? cols - c : 8); }
-
 // A row per CTA and step; thread t holds columns 8 (t + i blockDim) .. + 7,
-// i < V, as fp32 values of the stored type.
+// i < V, in the stored type.  All loads of a row are in flight before the first
+// is used; many narrow CTAs per SM overlap one row's sum with others' bytes.
 template <typename T, typename W, bool VEC, int V>
-__global__ void __launch_bounds__(1024) rmsnorm_fp8_kernel(NormArgs a) {
-  __shared__ float part[32];
+__global__ void __launch_bounds__(V == 1 ? 1024 : 512) rmsnorm_fp8_kernel(NormArgs a) {
+  __shared__ float part[2][32];
   const int t = threadIdx.x, nt = blockDim.x, lane = t % kWarp, warp = t / kWarp;
   const int64_t groups = ceil_div(a.cols, 128);
-  for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+  int turn = 0;
+  for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x, turn ^= 1) {
     const T* x = static_cast<const T*>(a.x) + r * a.x_stride;
-    const T* res = a.residual ? static_cast<const T*>(a.residual) + r * a.residual_stride : nullptr;
-    float h[V][8];
-    float ss = 0.0f;
+    Eight<T> h[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const int64_t c = 8 * (t + static_cast<int64_t>(i) * nt);
-      const int n = columns_from(c, a.cols);
+      const int c = 8 * (t + i * nt), n = columns_from(c, a.cols);
+      clear8(h[i]);
+      if (n > 0) load8<T, VEC>(x + c, n, h[i]);
+    }
+    if (a.residual) {
+      const T* res = static_cast<const T*>(a.residual) + r * a.residual_stride;
+      Eight<T> e[V];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) h[i][j] = 0.0f;
-      if (n > 0) {
-        load8<T, VEC>(x + c, n, h[i]);
-        if (res) {
-          float e[8];
-          load8<T, VEC>(res + c, n, e);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) h[i][j] = widen<T>(from_float<T>(h[i][j] + e[j]));
-          store8<T, VEC>(static_cast<T*>(a.residual_out) + r * a.cols + c, n, h[i]);
-        }
+      for (int i = 0; i < V; ++i) {
+        const int c = 8 * (t + i * nt), n = columns_from(c, a.cols);
+        clear8(e[i]);
+        if (n > 0) load8<T, VEC>(res + c, n, e[i]);
       }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) ss = fmaf(h[i][j], h[i][j], ss);
+      for (int i = 0; i < V; ++i) {
+        const int c = 8 * (t + i * nt), n = columns_from(c, a.cols);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) h[i].v[j] = from_float<T>(widen<T>(h[i].v[j]) + widen<T>(e[i].v[j]));
+        if (n > 0) store8<T, VEC>(static_cast<T*>(a.residual_out) + r * a.cols + c, n, h[i]);
+      }
     }
+    float ss = 0.0f;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) ss = fmaf(widen<T>(h[i].v[j]), widen<T>(h[i].v[j]), ss);
     ss = warp_sum(ss);
-    __syncthreads();  // the previous row's sums have been read
-    if (lane == 0) part[warp] = ss;
-    __syncthreads();
+    if (lane == 0) part[turn][warp] = ss;
+    __syncthreads();  // one per row: the other half of `part` is written meanwhile
     float total = 0.0f;
-    for (int i = 0; i < nt / kWarp; ++i) total += part[i];
+    for (int i = 0; i < nt / kWarp; ++i) total += part[turn][i];
     const float inv = 1.0f / sqrtf(total / static_cast<float>(a.cols) + a.eps);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const int64_t c = 8 * (t + static_cast<int64_t>(i) * nt);
-      const int n = columns_from(c, a.cols);
+      const int c = 8 * (t + i * nt), n = columns_from(c, a.cols);
+      if (V > 1 && c - 8 * lane >= a.cols) break;  // the whole warp is past the row
+      Eight<W> w;
+      clear8(w);
+      if (n > 0) load8<W, VEC>(static_cast<const W*>(a.weight) + c, n, w);
       float y[8];
-      if (n > 0) load8<W, VEC>(static_cast<const W*>(a.weight) + c, n, y);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = n > 0 ? h[i][j] * inv * y[j] : 0.0f;
-      if (a.normed_out && n > 0) store8<T, VEC>(static_cast<T*>(a.normed_out) + r * a.cols + c, n, y);
+      for (int j = 0; j < 8; ++j) y[j] = n > 0 ? widen<T>(h[i].v[j]) * inv * widen<W>(w.v[j]) : 0.0f;
+      if (a.normed_out && n > 0) {
+        Eight<T> o;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o.v[j] = from_float<T>(y[j]);
+        store8<T, VEC>(static_cast<T*>(a.normed_out) + r * a.cols + c, n, o);
+      }
       codes8<VEC>(y, n, a.codes + r * a.codes_stride + c, a.scales + r * groups + c / 128, c % 128 == 0);
     }
   }
 }
 
-// Sixteen lanes per (row, group); whole warps stay together for the shuffles.
+// Sixteen lanes per (row, group), kUnits of them per thread with their loads in
+// flight together; whole warps stay together for the shuffles.
+constexpr int kUnits = 4, kQuantThreads = 256, kCtaUnits = kQuantThreads / 16 * kUnits;
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) quantize_rows_kernel(NormArgs a) {
+__global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(NormArgs a) {
   const int64_t groups = ceil_div(a.cols, 128), units = a.rows * groups;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * kCtaUnits, row0 = first / groups;
+  const uint32_t rest = static_cast<uint32_t>(first - row0 * groups), per_row = static_cast<uint32_t>(groups);
   const int sub = threadIdx.x % 16;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * (256 / 16);
-  for (int64_t u0 = static_cast<int64_t>(blockIdx.x) * (256 / 16); u0 < units; u0 += step) {
-    const int64_t u = u0 + threadIdx.x / 16;
-    const int64_t r = u / groups, g = u - r * groups, c = g * 128 + sub * 8;
-    const int n = u < units ? columns_from(c, a.cols) : 0;
+  Eight<T> e[kUnits];
+  int64_t row[kUnits];
+  int col[kUnits], n[kUnits];
+#pragma unroll
+  for (int i = 0; i < kUnits; ++i) {
+    const uint32_t local = rest + threadIdx.x / 16 + i * (kQuantThreads / 16), r = local / per_row;
+    row[i] = row0 + r;
+    col[i] = static_cast<int>(local - r * per_row) * 128 + sub * 8;
+    n[i] = first + threadIdx.x / 16 + i * (kQuantThreads / 16) < units ? columns_from(col[i], a.cols) : 0;
+    clear8(e[i]);
+    if (n[i] > 0) load8<T, VEC>(static_cast<const T*>(a.x) + row[i] * a.x_stride + col[i], n[i], e[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < kUnits; ++i) {
     float y[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = 0.0f;
-    if (n > 0) load8<T, VEC>(static_cast<const T*>(a.x) + r * a.x_stride + c, n, y);
-    codes8<VEC>(y, n, a.codes + r * a.codes_stride + c, a.scales + u, sub == 0);
+    for (int j = 0; j < 8; ++j) y[j] = widen<T>(e[i].v[j]);
+    codes8<VEC>(y, n[i], a.codes + row[i] * a.codes_stride + col[i], a.scales + row[i] * groups + col[i] / 128, sub == 0);
   }
 }
 
@@ -176,13 +219,15 @@ bool aligned(const void* p, int64_t bytes) { return reinterpret_cast<uintptr_t>(
 
 template <typename T, typename W, bool VEC>
 cudaError_t launch_norm(const NormArgs& a, cudaStream_t stream) {
+  // Few rows: as many threads per row as there are vectors, the shortest way
+  // through one row.  More rows than the SMs hold that way: four vectors per thread.
   const int64_t vectors = ceil_div(a.cols, 8);
-  const int v = vectors <= 1024 ? 1 : vectors <= 2048 ? 2 : 4;
+  const int v = vectors <= 1024 && a.rows <= 2 * gemv_grid_ctas() ? 1 : vectors <= 2048 ? 4 : 8;
   const int threads = static_cast<int>(ceil_div(ceil_div(vectors, v), 32) * 32);
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(a.rows, int64_t(gemv_grid_ctas()) * 8));
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(a.rows, INT32_MAX));
   if (v == 1) rmsnorm_fp8_kernel<T, W, VEC, 1><<<grid, threads, 0, stream>>>(a);
-  else if (v == 2) rmsnorm_fp8_kernel<T, W, VEC, 2><<<grid, threads, 0, stream>>>(a);
-  else rmsnorm_fp8_kernel<T, W, VEC, 4><<<grid, threads, 0, stream>>>(a);
+  else if (v == 4) rmsnorm_fp8_kernel<T, W, VEC, 4><<<grid, threads, 0, stream>>>(a);
+  else rmsnorm_fp8_kernel<T, W, VEC, 8><<<grid, threads, 0, stream>>>(a);
   return cudaGetLastError();
 }
 
@@ -206,10 +251,11 @@ template <typename T>
 cudaError_t launch_quant(const NormArgs& a, cudaStream_t stream) {
   const bool vec = a.cols % 8 == 0 && aligned(a.x, 16) && a.x_stride * static_cast<int64_t>(sizeof(T)) % 16 == 0 &&
                    aligned(a.codes, 8) && a.codes_stride % 8 == 0;
-  const int64_t units = a.rows * ceil_div(a.cols, 128);
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(ceil_div(units, 16), int64_t(gemv_grid_ctas()) * 64));
-  if (vec) quantize_rows_kernel<T, true><<<grid, 256, 0, stream>>>(a);
-  else quantize_rows_kernel<T, false><<<grid, 256, 0, stream>>>(a);
+  const int64_t ctas = ceil_div(a.rows * ceil_div(a.cols, 128), kCtaUnits);
+  if (ctas > INT32_MAX || a.cols > INT32_MAX / 2) return cudaErrorInvalidValue;
+  const unsigned grid = static_cast<unsigned>(ctas);
+  if (vec) quantize_rows_kernel<T, true><<<grid, kQuantThreads, 0, stream>>>(a);
+  else quantize_rows_kernel<T, false><<<grid, kQuantThreads, 0, stream>>>(a);
   return cudaGetLastError();
 }
 

@@ -79,19 +79,22 @@ MOE_D void rotate8(float (&f)[8], int n, const float* cos, const float* sin, int
   }
 }
 
-// Unit u of a token: 0 its cache row, 1 .. its queries' rope values 256 (u - 1) .. + 255.
+// A CTA per token (and step): its last warp the cache row, the others the
+// queries, eight values of one head's group per thread and up to kAppendLoads
+// of them in flight.  The thread's column within a head stays the same where
+// the threads are a multiple of a head's vectors, and its angles with it.
+constexpr int kAppendLoads = 4;
 template <typename T, typename W, typename C, bool VEC>
-__global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(AppendArgs a, int units) {
-  const int lane = threadIdx.x % kWarp;
-  const int64_t total = a.tokens * units, warps = static_cast<int64_t>(gridDim.x) * (kAppendThreads / kWarp);
-  for (int64_t i = (static_cast<int64_t>(blockIdx.x) * kAppendThreads + threadIdx.x) / kWarp; i < total; i += warps) {
-    const int64_t t = i / units;
-    const int unit = static_cast<int>(i - t * units);
-    const int64_t slot = a.slots[t], pos = a.positions[t];
+__global__ void __launch_bounds__(kAppendThreads + kWarp) paged_append_kernel(AppendArgs a) {
+  const int tid = threadIdx.x, q_threads = blockDim.x - kWarp, lane = tid % kWarp;
+  const int latent = static_cast<int>(a.latent), rope = static_cast<int>(a.rope);
+  for (int64_t t = blockIdx.x; t < a.tokens; t += gridDim.x) {
+    const int64_t pos = a.positions[t];
     const bool placed = pos >= 0 && pos < a.table_rows;
-    const float* cos = a.cos + (placed ? pos : 0) * (a.rope / 2);
-    const float* sin = a.sin + (placed ? pos : 0) * (a.rope / 2);
-    if (unit == 0) {
+    const float* cos = a.cos + (placed ? pos : 0) * (rope / 2);
+    const float* sin = a.sin + (placed ? pos : 0) * (rope / 2);
+    if (tid >= q_threads) {
+      const int64_t slot = a.slots[t];
       if (slot < 0) continue;
       if (!placed || slot >= a.pages * a.page_size) {
         if (lane == 0) atomicOr(&g_device_error, kPagedRangeError);
@@ -104,19 +107,17 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(AppendArgs
       float ss = 0.0f;
 #pragma unroll
       for (int v = 0; v < kAppendVectors; ++v) {
-        const int64_t c = 8 * (lane + static_cast<int64_t>(v) * kWarp);
-        const int n = static_cast<int>(a.latent - c < 8 ? a.latent - c : 8);
+        const int c = 8 * (lane + v * kWarp), n = min(latent - c, 8);
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[v][j] = 0.0f;
         if (n > 0) load8<T, VEC>(src + c, n, f[v]);
 #pragma unroll
         for (int j = 0; j < 8; ++j) ss = fmaf(f[v][j], f[v][j], ss);
       }
-      const float inv = 1.0f / sqrtf(warp_sum(ss) / static_cast<float>(a.latent) + a.eps);
+      const float inv = 1.0f / sqrtf(warp_sum(ss) / static_cast<float>(latent) + a.eps);
 #pragma unroll
       for (int v = 0; v < kAppendVectors; ++v) {
-        const int64_t c = 8 * (lane + static_cast<int64_t>(v) * kWarp);
-        const int n = static_cast<int>(a.latent - c < 8 ? a.latent - c : 8);
+        const int c = 8 * (lane + v * kWarp), n = min(latent - c, 8);
         if (n <= 0) continue;
         float w[8];
         load8<W, VEC>(static_cast<const W*>(a.norm_w) + c, n, w);
@@ -124,28 +125,36 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(AppendArgs
         for (int j = 0; j < 8; ++j) f[v][j] *= inv * w[j];
         store8<C, VEC>(dst + c, n, f[v]);
       }
-      for (int64_t c = 8 * lane; c < a.rope; c += 8 * kWarp) {
-        const int n = static_cast<int>(a.rope - c < 8 ? a.rope - c : 8);
-        load8<T, VEC>(src + a.latent + c, n, f[0]);
+      for (int c = 8 * lane; c < rope; c += 8 * kWarp) {
+        const int n = min(rope - c, 8);
+        load8<T, VEC>(src + latent + c, n, f[0]);
         rotate8(f[0], n, cos, sin, c);
-        store8<C, VEC>(dst + a.latent + c, n, f[0]);
+        store8<C, VEC>(dst + latent + c, n, f[0]);
       }
-    } else {
-      // eight values of one head's group per lane (groups of eight never cross heads)
-      const int64_t per_head = ceil_div(a.rope, 8);
-      const int64_t v = (unit - 1) * static_cast<int64_t>(kWarp) + lane, h = v / per_head;
-      if (h >= a.heads) continue;
-      const int64_t c = 8 * (v - h * per_head);
-      const int n = static_cast<int>(a.rope - c < 8 ? a.rope - c : 8);
-      float f[8];
-      load8<C, VEC>(static_cast<const C*>(a.q) + t * a.q_stride + h * a.q_head_stride + c, n, f);
-      if (placed) {
-        rotate8(f, n, cos, sin, c);
-      } else {  // a row that has no place in the sequence: zeros
+      continue;
+    }
+    const int per_head = (rope + 7) / 8, vectors = static_cast<int>(a.heads) * per_head;
+    const C* q = static_cast<const C*>(a.q) + t * a.q_stride;
+    C* out = static_cast<C*>(a.q_out) + t * a.heads * rope;
+    for (int v0 = tid; v0 < vectors; v0 += q_threads * kAppendLoads) {
+      float f[kAppendLoads][8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = 0.0f;
+      for (int i = 0; i < kAppendLoads; ++i) {
+        const int v = v0 + i * q_threads, h = v / per_head, c = 8 * (v - h * per_head);
+        if (v < vectors) load8<C, VEC>(q + h * a.q_head_stride + c, min(rope - c, 8), f[i]);
       }
-      store8<C, VEC>(static_cast<C*>(a.q_out) + (t * a.heads + h) * a.rope + c, n, f);
+#pragma unroll
+      for (int i = 0; i < kAppendLoads; ++i) {
+        const int v = v0 + i * q_threads, h = v / per_head, c = 8 * (v - h * per_head), n = min(rope - c, 8);
+        if (v >= vectors) break;
+        if (placed) {
+          rotate8(f[i], n, cos, sin, c);
+        } else {  // a row that has no place in the sequence: zeros
+#pragma unroll
+          for (int j = 0; j < 8; ++j) f[i][j] = 0.0f;
+        }
+        store8<C, VEC>(out + h * rope + c, n, f[i]);
+      }
     }
   }
 }
@@ -154,17 +163,17 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 
 template <typename T, typename W, typename C>
 cudaError_t launch_append(const AppendArgs& a, cudaStream_t stream) {
-  const int64_t units = 1 + (a.q ? ceil_div(a.heads * ceil_div(a.rope, 8), kWarp) : 0);
   auto whole = [](int64_t n, int64_t size) { return n * size % 16 == 0; };
   const bool vec = a.latent % 8 == 0 && a.rope % 8 == 0 && aligned16(a.kv) && whole(a.kv_stride, sizeof(T)) &&
                    aligned16(a.norm_w) && aligned16(a.cache) && whole(a.page_stride, sizeof(C)) &&
                    whole(a.row_stride, sizeof(C)) &&
                    (!a.q || (aligned16(a.q) && aligned16(a.q_out) && whole(a.q_stride, sizeof(C)) &&
                              whole(a.q_head_stride, sizeof(C))));
-  const int64_t ctas = ceil_div(a.tokens * units, kAppendThreads / kWarp);
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(ctas, int64_t(gemv_grid_ctas()) * 32));
-  if (vec) paged_append_kernel<T, W, C, true><<<grid, kAppendThreads, 0, stream>>>(a, static_cast<int>(units));
-  else paged_append_kernel<T, W, C, false><<<grid, kAppendThreads, 0, stream>>>(a, static_cast<int>(units));
+  const int64_t vectors = a.q ? a.heads * ceil_div(a.rope, 8) : 0;
+  const int threads = static_cast<int>(std::min<int64_t>(ceil_div(vectors, kWarp) * kWarp, kAppendThreads)) + kWarp;
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(a.tokens, INT32_MAX));
+  if (vec) paged_append_kernel<T, W, C, true><<<grid, threads, 0, stream>>>(a);
+  else paged_append_kernel<T, W, C, false><<<grid, threads, 0, stream>>>(a);
   return cudaGetLastError();
 }
 

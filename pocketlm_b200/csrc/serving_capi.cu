@@ -40,6 +40,7 @@ int moe_fp8_quantize_rows(const void* x, int64_t x_stride, int x_dtype, int64_t 
   if (!x || !codes || !scales) return fail(kNullPointer, "null pointer");
   if (rows < 0 || cols <= 0 || codes_stride < cols) return fail(kBadDims, "bad dimensions");
   if (!is_type(x_dtype)) return fail(kUnsupported, "x is fp32, bf16 or fp16");
+  if (cols > INT32_MAX / 2) return fail(kUnsupported, "dimension too large");
   if (rows == 0) return kOk;
   NormArgs a{};
   a.x = x; a.codes = codes; a.scales = scales; a.rows = rows; a.cols = cols; a.x_stride = x_stride;

@@ -22,6 +22,7 @@ the device error word (moe_b200_device_error).
 
 from __future__ import annotations
 
+import functools
 from typing import NamedTuple
 
 import torch
@@ -30,6 +31,8 @@ from . import native
 
 _CODE = {torch.float32: native.DTYPE_F32, torch.bfloat16: native.DTYPE_BF16, torch.float16: native.DTYPE_F16}
 _FP8 = (torch.float8_e4m3fn, torch.uint8, torch.int8)
+# The current stream's handle without a Stream object around it (2 us of a 10 us call).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 
 
 class NormedRows(NamedTuple):
@@ -47,19 +50,23 @@ def _need(ok: bool, message: str) -> None:
 
 
 def _call(name: str, device: torch.device, *args) -> None:
-    lib = native.load_library()
-    if device.index == torch.cuda.current_device():
-        native._check(getattr(lib, name)(*args, torch.cuda.current_stream(device).cuda_stream), name)
-        return
-    with torch.cuda.device(device):
-        native._check(getattr(lib, name)(*args, torch.cuda.current_stream(device).cuda_stream), name)
+    fn, index = getattr(native.load_library(), name), device.index
+    if index == torch.cuda.current_device():
+        code = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            code = fn(*args, _raw_stream(index))
+    if code:
+        native._check(code, name)
 
 
-def _same_device(first: torch.Tensor, *others: torch.Tensor | None) -> torch.device:
-    device = first.device
-    _need(device.type == "cuda", "tensors must be on a CUDA device")
-    for t in others:
-        _need(t is None or t.device == device, "tensors must be on one device")
+def _one_device(*tensors: torch.Tensor | None) -> torch.device:
+    device = tensors[0].device
+    if device.type != "cuda":
+        raise ValueError("tensors must be on a CUDA device")
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError("tensors must be on one device")
     return device
 
 
@@ -70,11 +77,11 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(1) == 1 else t.contiguous()
 
 
-def _new_codes(rows: int, cols: int, device: torch.device) -> torch.Tensor:
-    """Codes whose rows start on 16-byte boundaries, as fp8_block_linear reads them."""
-    wide = (cols + 15) // 16 * 16
-    codes = torch.empty((rows, wide), dtype=torch.float8_e4m3fn, device=device)
-    return codes if wide == cols else codes[:, :cols]
+def _new_codes(flat: torch.Tensor, rows: int, cols: int) -> torch.Tensor:
+    """Codes [rows, cols] whose rows start on 16-byte boundaries, as fp8_block_linear reads them."""
+    if cols % 16 == 0:
+        return flat.new_empty((rows, cols), dtype=torch.float8_e4m3fn)
+    return flat.new_empty((rows, (cols + 15) // 16 * 16), dtype=torch.float8_e4m3fn)[:, :cols]
 
 
 def rmsnorm_fp8(x: torch.Tensor, weight: torch.Tensor, *, residual: torch.Tensor | None = None, eps: float = 1e-6,
@@ -85,52 +92,54 @@ def rmsnorm_fp8(x: torch.Tensor, weight: torch.Tensor, *, residual: torch.Tensor
     x [..., cols] bf16, fp16 or fp32 (rows of a wider tensor need no copy), cols <= 32768; weight [cols] of x's
     type or fp32; residual like x.  The mean is of h as it is returned.  return_normed adds y in x's type, the
     rows that a router reads."""
-    _need(x.dtype in _CODE, "x must be bf16, fp16 or fp32")
-    _need(x.ndim >= 1 and x.shape[-1] > 0, "x must be [..., cols]")
-    cols = x.shape[-1]
+    shape, dtype = x.shape, x.dtype
+    cols = shape[-1] if shape else 0
+    code = _CODE.get(dtype)
+    _need(code is not None, "x must be bf16, fp16 or fp32")
+    _need(cols > 0, "x must be [..., cols]")
     _need(weight.shape == (cols,), "weight must be [cols]")
-    _need(weight.dtype == x.dtype or weight.dtype == torch.float32, "weight must be of x's type or fp32")
-    _need(residual is None or (residual.shape == x.shape and residual.dtype == x.dtype), "residual must be like x")
+    _need(weight.dtype == dtype or weight.dtype == torch.float32, "weight must be of x's type or fp32")
+    _need(residual is None or (residual.shape == shape and residual.dtype == dtype), "residual must be like x")
     _need(cols <= 32768, "x has more than 32768 columns")
-    device = _same_device(x, weight, residual)
-    lead, flat = x.shape[:-1], _rows(x)
+    device = _one_device(x, weight, residual)
+    flat, weight = _rows(x), weight.contiguous()
     rows = flat.shape[0]
-    weight = weight.contiguous()
-    codes = _new_codes(rows, cols, device)
-    scales = torch.empty((rows, (cols + 127) // 128), dtype=torch.float32, device=device)
-    normed = torch.empty((rows, cols), dtype=x.dtype, device=device) if return_normed else None
-    stream_rows, res, res_stride = None, None, 0
+    codes = _new_codes(flat, rows, cols)
+    scales = flat.new_empty((rows, (cols + 127) // 128), dtype=torch.float32)
+    normed = flat.new_empty((rows, cols)) if return_normed else None
+    stream = res = None
     if residual is not None:
-        res = _rows(residual)
-        res_stride = res.stride(0)
-        stream_rows = torch.empty((rows, cols), dtype=x.dtype, device=device)
+        res, stream = _rows(residual), flat.new_empty((rows, cols))
     if rows:
-        _call("moe_rmsnorm_fp8", device, flat.data_ptr(), flat.stride(0), _CODE[x.dtype],
-              None if res is None else res.data_ptr(), res_stride, weight.data_ptr(), _CODE[weight.dtype], rows, cols,
-              float(eps), codes.data_ptr(), codes.stride(0), scales.data_ptr(),
-              None if stream_rows is None else stream_rows.data_ptr(), None if normed is None else normed.data_ptr())
-    if x.ndim != 2:
-        codes, scales = codes.view(x.shape), scales.view(*lead, scales.shape[1])
-        normed = None if normed is None else normed.reshape(x.shape)
-        stream_rows = None if stream_rows is None else stream_rows.reshape(x.shape)
-    return NormedRows(codes, scales, x if residual is None else stream_rows, normed)
+        _call("moe_rmsnorm_fp8", device, flat.data_ptr(), flat.stride(0), code, None if res is None else res.data_ptr(),
+              0 if res is None else res.stride(0), weight.data_ptr(), code if weight.dtype == dtype else native.DTYPE_F32,
+              rows, cols, eps, codes.data_ptr(), codes.stride(0), scales.data_ptr(),
+              None if stream is None else stream.data_ptr(), None if normed is None else normed.data_ptr())
+    if len(shape) != 2:
+        codes, scales = codes.view(shape), scales.view(*shape[:-1], scales.shape[1])
+        normed = None if normed is None else normed.view(shape)
+        stream = None if stream is None else stream.view(shape)
+    return NormedRows(codes, scales, x if stream is None else stream, normed)
 
 
 def quantize_fp8_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """x [..., cols] (bf16, fp16 or fp32) as e4m3 codes [..., cols] with one fp32 scale per 128 columns,
     max(amax, 2^-100) / 448."""
-    _need(x.dtype in _CODE, "x must be bf16, fp16 or fp32")
-    _need(x.ndim >= 1 and x.shape[-1] > 0, "x must be [..., cols]")
-    device = _same_device(x)
-    cols, lead, flat = x.shape[-1], x.shape[:-1], _rows(x)
+    shape = x.shape
+    cols = shape[-1] if shape else 0
+    code = _CODE.get(x.dtype)
+    _need(code is not None, "x must be bf16, fp16 or fp32")
+    _need(cols > 0, "x must be [..., cols]")
+    device = _one_device(x)
+    flat = _rows(x)
     rows = flat.shape[0]
-    codes = _new_codes(rows, cols, device)
-    scales = torch.empty((rows, (cols + 127) // 128), dtype=torch.float32, device=device)
+    codes = _new_codes(flat, rows, cols)
+    scales = flat.new_empty((rows, (cols + 127) // 128), dtype=torch.float32)
     if rows:
-        _call("moe_fp8_quantize_rows", device, flat.data_ptr(), flat.stride(0), _CODE[x.dtype], rows, cols,
-              codes.data_ptr(), codes.stride(0), scales.data_ptr())
-    if x.ndim != 2:
-        codes, scales = codes.view(x.shape), scales.view(*lead, scales.shape[1])
+        _call("moe_fp8_quantize_rows", device, flat.data_ptr(), flat.stride(0), code, rows, cols, codes.data_ptr(),
+              codes.stride(0), scales.data_ptr())
+    if len(shape) != 2:
+        codes, scales = codes.view(shape), scales.view(*shape[:-1], scales.shape[1])
     return codes, scales
 
 
@@ -162,11 +171,11 @@ def fp8_block_linear(codes: torch.Tensor, scales: torch.Tensor, fp8_weight: torc
     _need(scale_inv.shape == ((outs + 127) // 128, blocks), "scale_inv shape does not match FP8 128x128 block layout")
     lead = codes.shape[:-1]
     _need(scales.shape == (*lead, blocks), "scales must be [..., ceil(in_cols / 128)]")
-    device = _same_device(codes, scales, fp8_weight, scale_inv)
+    device = _one_device(codes, scales, fp8_weight, scale_inv)
     x, w = codes if codes.ndim == 2 else codes.reshape(-1, cols), _code_rows(fp8_weight)
     rows = x.shape[0]
     x, scales, scale_inv = _code_rows(x), scales.contiguous(), scale_inv.contiguous()
-    out = torch.empty((rows, outs), dtype=out_dtype, device=device)
+    out = scales.new_empty((rows, outs), dtype=out_dtype)
     if rows:
         _call("moe_fp8_block_linear", device, x.data_ptr(), x.stride(0), scales.data_ptr(), w.data_ptr(), w.stride(0),
               scale_inv.data_ptr(), rows, outs, cols, out.data_ptr(), _CODE[out_dtype])
@@ -201,14 +210,14 @@ def paged_mla_append(kv_rows: torch.Tensor, kv_norm_weight: torch.Tensor, cache:
     _need(q_pe is None or (q_pe.ndim == 3 and q_pe.shape[0] == tokens and q_pe.shape[1] > 0 and q_pe.shape[2] == rope),
           "q_pe must be [tokens, heads, rope]")
     _need(q_pe is None or q_pe.dtype == cache.dtype, "q_pe must be of the cache's type")
-    device = _same_device(cache, kv_rows, kv_norm_weight, slots, positions, rope_cos, rope_sin, q_pe)
+    device = _one_device(cache, kv_rows, kv_norm_weight, slots, positions, rope_cos, rope_sin, q_pe)
     kv = _rows(kv_rows)
     q_out, heads, q_strides = None, 0, (0, 0)
     if q_pe is not None:
         if q_pe.stride(2) != 1:
             q_pe = q_pe.contiguous()
         heads, q_strides = q_pe.shape[1], q_pe.stride()[:2]
-        q_out = torch.empty((tokens, heads, rope), dtype=cache.dtype, device=device)
+        q_out = cache.new_empty((tokens, heads, rope))
     if tokens:
         norm_w, slots, positions = kv_norm_weight.contiguous(), slots.contiguous(), positions.contiguous()
         cos, sin = rope_cos.contiguous(), rope_sin.contiguous()
@@ -218,6 +227,11 @@ def paged_mla_append(kv_rows: torch.Tensor, kv_norm_weight: torch.Tensor, cache:
               None if q_pe is None else q_pe.data_ptr(), *q_strides, heads, None if q_out is None else q_out.data_ptr(),
               tokens, latent, rope, float(eps))
     return q_out
+
+
+@functools.lru_cache(maxsize=256)
+def _attention_workspace(*dims: int) -> int:
+    return max(int(native.load_library().moe_paged_mla_attention_workspace_bytes(*dims)), 256)
 
 
 def _query(t: torch.Tensor) -> torch.Tensor:
@@ -254,15 +268,14 @@ def paged_mla_attention(q_latent: torch.Tensor, q_pe: torch.Tensor, cache: torch
     _need(page_table.dtype == torch.int32 and lengths.dtype == torch.int32, "page_table and lengths must be int32")
     _need(cache.stride(0) % 8 == 0 and cache.stride(1) % 8 == 0 and cache.data_ptr() % 16 == 0,
           "cache rows must start on 16-byte boundaries")
-    device = _same_device(cache, q_latent, q_pe, page_table, lengths)
+    device = _one_device(cache, q_latent, q_pe, page_table, lengths)
     q_latent, q_pe = _query(q_latent), _query(q_pe)
-    out = torch.empty((batch, heads, latent), dtype=cache.dtype, device=device)
-    lse = torch.empty((batch, heads), dtype=torch.float32, device=device) if return_lse else None
+    out = cache.new_empty((batch, heads, latent))
+    lse = cache.new_empty((batch, heads), dtype=torch.float32) if return_lse else None
     if batch:
         table = page_table if page_table.stride(1) == 1 else page_table.contiguous()
         lengths = lengths.contiguous()
-        need = native.load_library().moe_paged_mla_attention_workspace_bytes(batch, heads, latent, rope, table.shape[1], page_size)
-        work = torch.empty((max(int(need), 256),), dtype=torch.uint8, device=device)
+        work = cache.new_empty((_attention_workspace(batch, heads, latent, rope, table.shape[1], page_size),), dtype=torch.uint8)
         _call("moe_paged_mla_attention", device, q_latent.data_ptr(), q_latent.stride(0), q_latent.stride(1),
               q_pe.data_ptr(), q_pe.stride(0), q_pe.stride(1), cache.data_ptr(), _CODE[cache.dtype], pages, page_size,
               cache.stride(0), cache.stride(1), table.data_ptr(), table.stride(0), table.shape[1], lengths.data_ptr(),
