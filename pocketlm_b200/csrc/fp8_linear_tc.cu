@@ -14,13 +14,14 @@
 // sums are added through distributed shared memory in rank order (the same
 // result on every run).
 //
-// Many rows (linear_tiles_kernel): the tensor cores bound it.  128 tokens x 256
-// outputs per CTA and tile, two 256-column accumulators so that the sums of one
+// Many rows (linear_tiles_kernel): the tensor cores bound it.  128 tokens x up
+// to 256 outputs per CTA and tile, two accumulators so that the sums of one
 // group are read while the next is computed; persistent CTAs.
 #include <algorithm>
 
 #include "fp8_gemv.cuh"
 #include "router.cuh"
+#include "rows.cuh"
 #include "serving.cuh"
 #include "tcgen05.cuh"
 
@@ -28,15 +29,6 @@ namespace moe {
 namespace {
 
 constexpr int kGroup = 128;  // columns per scale group: a stage of the pipeline
-
-template <typename O>
-MOE_D O out_value(float v);
-template <>
-MOE_D float out_value<float>(float v) { return v; }
-template <>
-MOE_D __nv_bfloat16 out_value<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-template <>
-MOE_D __half out_value<__half>(float v) { return __float2half_rn(v); }
 
 MOE_D bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
   return __all_sync(0xFFFFFFFFu, wait_or_abort(bar, parity, abort, kLinearWaitError));
@@ -69,17 +61,8 @@ size_t rows_smem(int groups) {
   return 1024 + RowsShape<NT>::kPipeBytes + sizeof(float) * NT * groups + sizeof(RowsBarriers<NT>);
 }
 
-MOE_D uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-MOE_D void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-MOE_D float4 ld_cluster(uint32_t addr, uint32_t rank) {
-  uint32_t at;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(addr), "r"(rank));
+MOE_D float4 ld_cluster(const float* p, uint32_t rank) {
+  const uint32_t at = cluster_addr(p, rank);
   float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
                : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
@@ -214,7 +197,7 @@ __global__ void __launch_bounds__(kRowsThreads) linear_rows_kernel(const __grid_
     if (tid < 128 && n < a.outs) {
 #pragma unroll
       for (int j = 0; j < NT; ++j)
-        if (t0 + j < a.rows) out[(t0 + j) * a.outs + n] = out_value<O>(acc[j]);
+        if (t0 + j < a.rows) out[(t0 + j) * a.outs + n] = from_float<O>(acc[j]);
     }
     return;
   }
@@ -230,7 +213,7 @@ __global__ void __launch_bounds__(kRowsThreads) linear_rows_kernel(const __grid_
     const int e = i + rank * (NT * 32 / splits), t = e / 32, c = (e % 32) * 4;
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int r = 0; r < splits; ++r) {
-      const float4 v = ld_cluster(smem_addr(part + t * 128 + c), r);
+      const float4 v = ld_cluster(part + t * 128 + c, r);
       sum.x += v.x;
       sum.y += v.y;
       sum.z += v.z;
@@ -240,41 +223,55 @@ __global__ void __launch_bounds__(kRowsThreads) linear_rows_kernel(const __grid_
     const float v[4] = {sum.x, sum.y, sum.z, sum.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      if (n0 + c + j < a.outs) out[(t0 + t) * a.outs + n0 + c + j] = out_value<O>(v[j]);
+      if (n0 + c + j < a.outs) out[(t0 + t) * a.outs + n0 + c + j] = from_float<O>(v[j]);
   }
   cluster_sync();  // nobody leaves while its sums are being read
 }
 
 // ----------------------------------------------------------------- many rows
 
-constexpr int kTileM = 128, kTileN = 256, kTileStages = 4;
-constexpr int kTileABytes = kTileM * kGroup, kTileBBytes = kTileN * kGroup, kTileStageBytes = kTileABytes + kTileBBytes;
-constexpr int kSumWarps = 8;  // warp w: rows 32 (w % 4) .. + 31, columns 128 (w / 4) .. + 127
-constexpr int kTilesThreads = (kSumWarps + 2) * kWarp;
+// 128 tokens x TN outputs per CTA and tile.  (Pairs of CTAs sharing a 256-token
+// tile halve the bytes from L2, but a group's sums are handed over every 500
+// cycles, and across the pair the handshake alone took 1160: 912 us against 500
+// on 4000 x 7168 x 16384.)
+constexpr int kTileM = 128;  // tokens per CTA
+constexpr int kSumWarps = 8;  // warp w: tokens 32 (w % 4) .. + 31, half w / 4 of the TN columns
+constexpr int kTilesThreads = (kSumWarps + 3) * kWarp;  // .. 8: TMA; 9, 10: the products of even and odd groups
+template <int TN>
+struct TilesShape {
+  static constexpr int kABytes = kTileM * kGroup, kBBytes = TN * kGroup, kStageBytes = kABytes + kBBytes;
+  static constexpr int kStages = TN > 224 ? 4 : 5;
+};
+template <int TN>
 struct TilesBarriers {
-  uint64_t full[kTileStages], empty[kTileStages];
+  uint64_t full[TilesShape<TN>::kStages], empty[TilesShape<TN>::kStages];
   uint64_t sum_full[2], sum_empty[2];
   uint64_t drain;
   uint32_t tmem_base;
   int abort;
 };
-constexpr size_t kTilesSmem = 1024 + kTileStages * kTileStageBytes + sizeof(TilesBarriers);
-static_assert(kTilesSmem <= 232448, "shared memory per block");
+template <int TN>
+constexpr size_t tiles_smem() {
+  return 1024 + TilesShape<TN>::kStages * TilesShape<TN>::kStageBytes + sizeof(TilesBarriers<TN>);
+}
+static_assert(tiles_smem<256>() <= 232448 && tiles_smem<224>() <= 232448, "shared memory per block");
 
-template <typename O>
-__global__ void __launch_bounds__(kTilesThreads, 1) linear_tiles_kernel(const __grid_constant__ CUtensorMap map_x,
-                                                                        const __grid_constant__ CUtensorMap map_w,
-                                                                        LinearArgs a, int m_tiles, int n_tiles) {
+template <typename O, int TN>
+__global__ void __launch_bounds__(kTilesThreads, 1)
+    linear_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, LinearArgs a,
+                        int m_tiles, int n_tiles) {
+  using Shape = TilesShape<TN>;
+  constexpr int kStages = Shape::kStages, kHalf = TN / 2, kStageBytes = Shape::kStageBytes;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  TilesBarriers* bars = reinterpret_cast<TilesBarriers*>(smem + kTileStages * kTileStageBytes);
+  auto* bars = reinterpret_cast<TilesBarriers<TN>*>(smem + kStages * kStageBytes);
   const int tid = threadIdx.x, lane = tid % kWarp, warp = __shfl_sync(0xFFFFFFFFu, tid / kWarp, 0);
   volatile int* abort = &bars->abort;
   const int groups = static_cast<int>((a.cols + kGroup - 1) / kGroup);
   const int tiles = m_tiles * n_tiles;
 
   if (tid == 0) {
-    for (int s = 0; s < kTileStages; ++s) {
+    for (int s = 0; s < kStages; ++s) {
       mbar_init(&bars->full[s], 1);
       mbar_init(&bars->empty[s], 1);
     }
@@ -282,12 +279,12 @@ __global__ void __launch_bounds__(kTilesThreads, 1) linear_tiles_kernel(const __
       mbar_init(&bars->sum_full[b], 1);
       mbar_init(&bars->sum_empty[b], kSumWarps);
     }
-    mbar_init(&bars->drain, 1);
+    mbar_init(&bars->drain, 2);
     bars->abort = 0;
     fence_barrier_init();
   }
   if (warp == kSumWarps + 1) {
-    tmem_alloc(&bars->tmem_base, 2 * kTileN);
+    tmem_alloc(&bars->tmem_base, 512);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -299,100 +296,116 @@ __global__ void __launch_bounds__(kTilesThreads, 1) linear_tiles_kernel(const __
     const bool leader = elect_one();
     const uint32_t at = smem_addr(smem);
     uint32_t i = 0;
-    for (int t = blockIdx.x; t < tiles && !*abort; t += gridDim.x) {
-      const int m0 = t % m_tiles * kTileM, n0 = t / m_tiles * kTileN;
+    bool ok = true;
+    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      const int m0 = t % m_tiles * kTileM, n0 = t / m_tiles * TN;
       for (int g = 0; g < groups; ++g, ++i) {
-        const uint32_t s = i % kTileStages;
-        if (i >= kTileStages && !warp_wait(&bars->empty[s], ((i / kTileStages) - 1) & 1, abort)) break;
+        const uint32_t s = i % kStages;
+        if (i >= kStages && !warp_wait(&bars->empty[s], ((i / kStages) - 1) & 1, abort)) {
+          ok = false;
+          break;
+        }
         if (leader) {
-          mbar_arrive_expect_tx(&bars->full[s], kTileStageBytes);
-          tma_load_2d(at + s * kTileStageBytes, &map_x, g * kGroup, m0, &bars->full[s]);
-          tma_load_2d(at + s * kTileStageBytes + kTileABytes, &map_w, g * kGroup, n0, &bars->full[s]);
+          mbar_arrive_expect_tx(&bars->full[s], kStageBytes);
+          tma_load_2d(at + s * kStageBytes, &map_x, g * kGroup, m0, &bars->full[s]);
+          tma_load_2d(at + s * kStageBytes + Shape::kABytes, &map_w, g * kGroup, n0, &bars->full[s]);
         }
         __syncwarp();
       }
     }
-    for (uint32_t j = i > kTileStages ? i - kTileStages : 0; j < i; ++j)
-      mbar_wait(&bars->full[j % kTileStages], (j / kTileStages) & 1, kLinearWaitError);
-  } else if (warp == kSumWarps + 1) {
+    for (uint32_t j = i > kStages ? i - kStages : 0; j < i; ++j)  // every copy issued lands before the CTA leaves
+      mbar_wait(&bars->full[j % kStages], (j / kStages) & 1, kLinearWaitError);
+  } else if (warp == kSumWarps + 1 || warp == kSumWarps + 2) {
+    // one warp per accumulator: a group's hand-over hides behind the other's
     const bool leader = elect_one();
-    const uint32_t idesc = umma_idesc(kTileM, kTileN, 0, false);
-    const uint64_t x_desc = sw128_desc_k(smem_addr(smem)), w_desc = sw128_desc_k(smem_addr(smem) + kTileABytes);
-    uint32_t i = 0;
-    bool ok = true;
-    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-      for (int g = 0; g < groups; ++g, ++i) {
-        const uint32_t s = i % kTileStages, b = i % 2;
-        if (!warp_wait(&bars->full[s], (i / kTileStages) & 1, abort) ||
-            (i >= 2 && !warp_wait(&bars->sum_empty[b], ((i / 2) - 1) & 1, abort))) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        if (leader) {
-          const uint64_t step = static_cast<uint64_t>(s * (kTileStageBytes / 16));
+    const uint32_t b = warp - kSumWarps - 1, d = tmem + b * 256;
+    const uint32_t idesc = umma_idesc(kTileM, TN, 0, false);
+    const uint64_t x_desc = sw128_desc_k(smem_addr(smem)), w_desc = sw128_desc_k(smem_addr(smem) + Shape::kABytes);
+    const uint32_t mine = (tiles - blockIdx.x + gridDim.x - 1) / gridDim.x * static_cast<uint32_t>(groups);  // groups of this CTA's tiles
+    for (uint32_t i = b; i < mine; i += 2) {
+      const uint32_t s = i % kStages;
+      if (i >= 2 && !warp_wait(&bars->sum_empty[b], ((i / 2) - 1) & 1, abort)) break;
+      if (!warp_wait(&bars->full[s], (i / kStages) & 1, abort)) break;
+      tc_fence_after();
+      if (leader) {
+        const uint64_t step = static_cast<uint64_t>(s * (kStageBytes / 16));
 #pragma unroll
-          for (int k = 0; k < kGroup / 32; ++k)
-            umma_f8_ss(tmem + b * kTileN, x_desc + step + 2 * k, w_desc + step + 2 * k, idesc, k > 0);
-          umma_commit(&bars->empty[s]);
-          umma_commit(&bars->sum_full[b]);
-        }
-        __syncwarp();
+        for (int k = 0; k < kGroup / 32; ++k) umma_f8_ss(d, x_desc + step + 2 * k, w_desc + step + 2 * k, idesc, k > 0);
+        umma_commit(&bars->sum_full[b]);
+        umma_commit(&bars->empty[s]);
       }
+      __syncwarp();
     }
     if (leader) umma_commit(&bars->drain);
     __syncwarp();
     mbar_wait(&bars->drain, 0, kLinearWaitError);
-  } else {
+  } else if (warp < kSumWarps) {
     const int quad = warp % 4, half = warp / 4;
-    const uint32_t from = tmem + (static_cast<uint32_t>(quad * kWarp) << 16) + half * 128;
+    const uint32_t from = tmem + (static_cast<uint32_t>(quad * kWarp) << 16) + half * kHalf;
     uint32_t i = 0;
     bool ok = true;
     for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-      const int64_t row = t % m_tiles * kTileM + quad * kWarp + lane, n0 = t / m_tiles * kTileN + half * 128;
+      const int64_t row = t % m_tiles * kTileM + quad * kWarp + lane;
+      const int64_t n0 = static_cast<int64_t>(t / m_tiles) * TN + half * kHalf;
+      // the columns from `edge` (a multiple of 16) on belong to the next 128 of the weight's rows
+      const int edge = static_cast<int>(128 - n0 % 128);
+      const int64_t last = (a.outs - 1) / 128;
       const float* sx = a.x_scales + std::min<int64_t>(row, a.rows - 1) * groups;
-      const float* sw = a.w_scales + std::min<int64_t>(n0, a.outs - 1) / 128 * groups;
-      float acc[128];
+      const float* sw0 = a.w_scales + std::min<int64_t>(n0 / 128, last) * groups;
+      const float* sw1 = a.w_scales + std::min<int64_t>(n0 / 128 + 1, last) * groups;
+      float acc[kHalf];
 #pragma unroll
-      for (int j = 0; j < 128; ++j) acc[j] = 0.0f;
-      float next = __ldg(sx) * __ldg(sw);
+      for (int j = 0; j < kHalf; ++j) acc[j] = 0.0f;
+      float next0 = __ldg(sx) * __ldg(sw0), next1 = __ldg(sx) * __ldg(sw1);
       for (int g = 0; g < groups; ++g, ++i) {
         const uint32_t b = i % 2;
-        const float f = next;
-        if (g + 1 < groups) next = __ldg(sx + g + 1) * __ldg(sw + g + 1);
+        const float f0 = next0, f1 = next1;
+        if (g + 1 < groups) {
+          const float x = __ldg(sx + g + 1);
+          next0 = x * __ldg(sw0 + g + 1);
+          next1 = x * __ldg(sw1 + g + 1);
+        }
         if (!warp_wait(&bars->sum_full[b], (i / 2) & 1, abort)) {
           ok = false;
           break;
         }
         tc_fence_after();
 #pragma unroll
-        for (int c = 0; c < 128; c += 32) {
+        for (int c = 0; c < kHalf; c += 32) {
           uint32_t d[32];
-          tmem_ld32(from + b * kTileN + c, d);
+          const int width = kHalf - c < 32 ? 16 : 32;
+          if (width == 32) tmem_ld32(from + b * 256 + c, d);
+          else tmem_ld16(from + b * 256 + c, d);
           tmem_ld_wait();
+          if (c + 32 >= kHalf) {  // the last columns have left the accumulator
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars->sum_empty[b]);
+          }
 #pragma unroll
-          for (int j = 0; j < 32; ++j) acc[c + j] = fmaf(__uint_as_float(d[j]), f, acc[c + j]);
+          for (int j = 0; j < 32; ++j) {
+            if (j >= width) break;
+            acc[c + j] = fmaf(__uint_as_float(d[j]), c + j / 16 * 16 < edge ? f0 : f1, acc[c + j]);
+          }
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars->sum_empty[b]);
       }
       if (!ok) break;
       if (row < a.rows) {
         O* out = static_cast<O*>(a.out) + row * a.outs + n0;
         constexpr int kV = 16 / sizeof(O);
-        if (n0 + 128 <= a.outs && a.outs % kV == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15u) == 0) {
+        const bool whole = n0 + kHalf <= a.outs && a.outs % kV == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15u) == 0;
 #pragma unroll
-          for (int j = 0; j < 128; j += kV) {
-            __align__(16) O v[kV];
+        for (int j = 0; j < kHalf; j += kV) {
+          __align__(16) O v[kV];
 #pragma unroll
-            for (int k = 0; k < kV; ++k) v[k] = out_value<O>(acc[j + k]);
+          for (int k = 0; k < kV; ++k) v[k] = from_float<O>(acc[j + k]);
+          if (whole) {
             *reinterpret_cast<uint4*>(out + j) = *reinterpret_cast<const uint4*>(v);
-          }
-        } else {
+          } else {
 #pragma unroll
-          for (int j = 0; j < 128; ++j)
-            if (n0 + j < a.outs) out[j] = out_value<O>(acc[j]);
+            for (int k = 0; k < kV; ++k)
+              if (n0 + j + k < a.outs) out[j + k] = v[k];
+          }
         }
       }
     }
@@ -400,7 +413,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) linear_tiles_kernel(const __
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == kSumWarps + 1) tmem_dealloc(tmem, 2 * kTileN);
+  if (warp == kSumWarps + 1) tmem_dealloc(tmem, 512);
 }
 
 // [rows][cols] bytes with a box of one group's columns and `box` rows, 128B-swizzled.
@@ -447,19 +460,33 @@ cudaError_t launch_rows(const LinearArgs& a, cudaStream_t stream) {
   return cudaLaunchKernelEx(&config, kernel, mx, mw, a, splits, max_groups);
 }
 
+template <typename O, int TN>
+cudaError_t launch_tiles_n(const LinearArgs& a, cudaStream_t stream) {
+  CUtensorMap mx, mw;
+  if (!encode_codes(&mx, a.x, a.rows, a.cols, a.x_stride, kTileM) || !encode_codes(&mw, a.w, a.outs, a.cols, a.w_stride, TN))
+    return cudaErrorInvalidValue;
+  auto kernel = linear_tiles_kernel<O, TN>;
+  constexpr int kSmem = static_cast<int>(tiles_smem<TN>());
+  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  if (err != cudaSuccess) return err;
+  const int64_t m_tiles = ceil_div(a.rows, kTileM), n_tiles = ceil_div(a.outs, TN);
+  if (m_tiles * n_tiles > INT32_MAX / 2) return cudaErrorInvalidValue;
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(m_tiles * n_tiles, gemv_grid_ctas()));
+  kernel<<<grid, kTilesThreads, kSmem, stream>>>(mx, mw, a, static_cast<int>(m_tiles), static_cast<int>(n_tiles));
+  return cudaGetLastError();
+}
+
+// The tile width whose rounds of all SMs cover the outputs with the least work:
+// 4000 x 7168 outputs are 896 tiles of 256 (7 rounds of 148, the last one all
+// but empty) or 1024 of 224 (7 rounds, each an eighth shorter).
 template <typename O>
 cudaError_t launch_tiles(const LinearArgs& a, cudaStream_t stream) {
-  CUtensorMap mx, mw;
-  if (!encode_codes(&mx, a.x, a.rows, a.cols, a.x_stride, kTileM) || !encode_codes(&mw, a.w, a.outs, a.cols, a.w_stride, kTileN))
-    return cudaErrorInvalidValue;
-  auto kernel = linear_tiles_kernel<O>;
-  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kTilesSmem));
-  if (err != cudaSuccess) return err;
-  const int64_t m_tiles = ceil_div(a.rows, kTileM), n_tiles = ceil_div(a.outs, kTileN);
-  if (m_tiles * n_tiles > INT32_MAX) return cudaErrorInvalidValue;
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(m_tiles * n_tiles, gemv_grid_ctas()));
-  kernel<<<grid, kTilesThreads, kTilesSmem, stream>>>(mx, mw, a, static_cast<int>(m_tiles), static_cast<int>(n_tiles));
-  return cudaGetLastError();
+  auto cost = [&](int64_t tn) {
+    return ceil_div(ceil_div(a.rows, kTileM) * ceil_div(a.outs, tn), gemv_grid_ctas()) * tn;
+  };
+  if (cost(224) < cost(256) && cost(224) <= cost(192)) return launch_tiles_n<O, 224>(a, stream);
+  if (cost(192) < cost(256)) return launch_tiles_n<O, 192>(a, stream);
+  return launch_tiles_n<O, 256>(a, stream);
 }
 
 template <typename O>
@@ -467,8 +494,8 @@ cudaError_t launch_linear(const LinearArgs& a, cudaStream_t stream) {
   if (a.rows <= 16) return launch_rows<O, 16>(a, stream);
   if (a.rows <= 32) return launch_rows<O, 32>(a, stream);
   if (a.rows <= 64) return launch_rows<O, 64>(a, stream);
-  // 128 x 256 tiles once they fill the SMs, smaller and cut ones until then
-  if (ceil_div(a.rows, kTileM) * ceil_div(a.outs, kTileN) * 2 < gemv_grid_ctas()) return launch_rows<O, 128>(a, stream);
+  // tiles once they fill half of the SMs, smaller and cut ones until then
+  if (ceil_div(a.rows, kTileM) * ceil_div(a.outs, 256) * 2 < gemv_grid_ctas()) return launch_rows<O, 128>(a, stream);
   return launch_tiles<O>(a, stream);
 }
 

@@ -18,6 +18,7 @@
 
 #include "fp8_gemv.cuh"
 #include "router.cuh"
+#include "rows.cuh"
 #include "serving.cuh"
 
 namespace moe {
@@ -31,6 +32,11 @@ MOE_D float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+MOE_D float reciprocal(float a) {  // within 1 ulp; 0 of an infinity
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a));
+  return r;
+}
 // Two floats -> two e4m3 codes, a in the low byte.
 MOE_D uint32_t e4m3x2(float a, float b) {
   uint16_t r;
@@ -38,76 +44,52 @@ MOE_D uint32_t e4m3x2(float a, float b) {
   return r;
 }
 
-template <typename T>
-MOE_D T from_float(float v);
-template <>
-MOE_D float from_float<float>(float v) { return v; }
-template <>
-MOE_D __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-template <>
-MOE_D __half from_float<__half>(float v) { return __float2half_rn(v); }
-template <typename T>
-MOE_D float widen(T v) { return static_cast<float>(v); }
-
-// Eight columns of a row as they are stored: 16-byte accesses when VEC (whole
-// and aligned), else one element at a time, `n` of them present.
-template <typename T>
-struct alignas(16) Eight {
-  T v[8];
-};
-template <typename T, bool VEC>
-MOE_D void load8(const T* p, int n, Eight<T>& e) {
-  if (VEC) {
-#pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
-      reinterpret_cast<uint4*>(e.v)[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) e.v[i] = i < n ? p[i] : from_float<T>(0.0f);
-  }
-}
-template <typename T, bool VEC>
-MOE_D void store8(T* p, int n, const Eight<T>& e) {
-  if (VEC) {
-#pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
-      reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(e.v)[i];
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < n) p[i] = e.v[i];
-  }
-}
-template <typename T>
-MOE_D void clear8(Eight<T>& e) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) e.v[i] = from_float<T>(0.0f);
-}
-
 MOE_D int columns_from(int64_t c, int64_t cols) { return static_cast<int>(cols - c < 8 ? cols - c : 8); }
+
+// The largest size among eight stored values (NaN if one is).
+template <typename T>
+MOE_D float amax8(const Eight<T>& e) {
+  float m = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max_nan(m, fabsf(widen<T>(e.v[i])));
+  return m;
+}
+template <>
+MOE_D float amax8<__nv_bfloat16>(const Eight<__nv_bfloat16>& e) {
+  const __nv_bfloat162* p = reinterpret_cast<const __nv_bfloat162*>(e.v);
+  const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(__habs2(p[0]), __habs2(p[1])), __hmax2_nan(__habs2(p[2]), __habs2(p[3])));
+  return max_nan(__low2float(m), __high2float(m));
+}
+template <>
+MOE_D float amax8<__half>(const Eight<__half>& e) {
+  const __half2* p = reinterpret_cast<const __half2*>(e.v);
+  const __half2 m = __hmax2_nan(__hmax2_nan(__habs2(p[0]), __habs2(p[1])), __hmax2_nan(__habs2(p[2]), __habs2(p[3])));
+  return max_nan(__low2float(m), __high2float(m));
+}
 
 // The group's scale and this lane's eight codes; the sixteen lanes of a group
 // are neighbours and all take part.
 template <bool VEC>
-MOE_D void codes8(const float (&y)[8], int n, uint8_t* codes, float* scale, bool first) {
-  float amax = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) amax = max_nan(amax, fabsf(y[i]));
+MOE_D void codes8(const float2 (&y)[4], float amax, int n, uint8_t* codes, float* scale, bool first) {
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
-  const float s = max_nan(amax, kTinyAmax) / kE4m3Max;
-  const float inv = 1.0f / s;
+  // amax / 448 and its reciprocal: an approximation and one Newton step each are enough
+  amax = max_nan(amax, kTinyAmax);
+  const float p448 = amax * (1.0f / kE4m3Max);
+  const float s = p448 > kE4m3Max * 1e30f ? p448 : fmaf(fmaf(-p448, kE4m3Max, amax), 1.0f / kE4m3Max, p448);
+  const float inv = reciprocal(s);
   if (n <= 0) return;
-  // y / s: the product with the reciprocal and one Newton step on its remainder (an infinite scale's
-  // remainder is none: 0 * inf), so that a value on the border between two codes goes to the even one
-  float q[8];
+  // y / s: the product with the reciprocal and one Newton step on its remainder, so that a value on
+  // the border between two codes goes to the even one (an infinite scale has no remainder: 0 * inf)
+  const float rem = inv == 0.0f ? 0.0f : -s;
+  uint32_t c[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float p = y[i] * inv;
-    q[i] = inv == 0.0f ? p : fmaf(fmaf(-p, s, y[i]), inv, p);
+  for (int i = 0; i < 4; ++i) {
+    const float2 p = mul2(y[i], make_float2(inv, inv));
+    const float2 q = fma2(fma2(p, make_float2(rem, rem), y[i]), make_float2(inv, inv), p);
+    c[i] = e4m3x2(q.x, q.y);
   }
-  const uint32_t lo = e4m3x2(q[0], q[1]) | e4m3x2(q[2], q[3]) << 16;
-  const uint32_t hi = e4m3x2(q[4], q[5]) | e4m3x2(q[6], q[7]) << 16;
+  const uint32_t lo = c[0] | c[1] << 16, hi = c[2] | c[3] << 16;
   if (VEC) {
     *reinterpret_cast<uint2*>(codes) = make_uint2(lo, hi);
   } else {
@@ -122,7 +104,7 @@ MOE_D void codes8(const float (&y)[8], int n, uint8_t* codes, float* scale, bool
 // i < V, in the stored type.  All loads of a row are in flight before the first
 // is used; many narrow CTAs per SM overlap one row's sum with others' bytes.
 template <typename T, typename W, bool VEC, int V>
-__global__ void __launch_bounds__(V == 1 ? 1024 : 512) rmsnorm_fp8_kernel(NormArgs a) {
+__global__ void __launch_bounds__(V == 1 ? 1024 : 512, V == 4 ? 2 : 1) rmsnorm_fp8_kernel(NormArgs a) {
   __shared__ float part[2][32];
   const int t = threadIdx.x, nt = blockDim.x, lane = t % kWarp, warp = t / kWarp;
   const int64_t groups = ceil_div(a.cols, 128);
@@ -171,16 +153,21 @@ __global__ void __launch_bounds__(V == 1 ? 1024 : 512) rmsnorm_fp8_kernel(NormAr
       Eight<W> w;
       clear8(w);
       if (n > 0) load8<W, VEC>(static_cast<const W*>(a.weight) + c, n, w);
-      float y[8];
+      float2 y[4];
+      float amax = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = n > 0 ? widen<T>(h[i].v[j]) * inv * widen<W>(w.v[j]) : 0.0f;
+      for (int j = 0; j < 4; ++j) {
+        y[j].x = n > 0 ? widen<T>(h[i].v[2 * j]) * inv * widen<W>(w.v[2 * j]) : 0.0f;
+        y[j].y = n > 0 ? widen<T>(h[i].v[2 * j + 1]) * inv * widen<W>(w.v[2 * j + 1]) : 0.0f;
+        amax = max_nan(amax, max_nan(fabsf(y[j].x), fabsf(y[j].y)));
+      }
       if (a.normed_out && n > 0) {
         Eight<T> o;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) o.v[j] = from_float<T>(y[j]);
+        for (int j = 0; j < 8; ++j) o.v[j] = from_float<T>(j % 2 ? y[j / 2].y : y[j / 2].x);
         store8<T, VEC>(static_cast<T*>(a.normed_out) + r * a.cols + c, n, o);
       }
-      codes8<VEC>(y, n, a.codes + r * a.codes_stride + c, a.scales + r * groups + c / 128, c % 128 == 0);
+      codes8<VEC>(y, amax, n, a.codes + r * a.codes_stride + c, a.scales + r * groups + c / 128, c % 128 == 0);
     }
   }
 }
@@ -191,7 +178,8 @@ constexpr int kUnits = 4, kQuantThreads = 256, kCtaUnits = kQuantThreads / 16 * 
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(NormArgs a) {
   const int64_t groups = ceil_div(a.cols, 128), units = a.rows * groups;
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * kCtaUnits, row0 = first / groups;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * kCtaUnits;
+  const int64_t row0 = units <= UINT32_MAX ? static_cast<uint32_t>(first) / static_cast<uint32_t>(groups) : first / groups;
   const uint32_t rest = static_cast<uint32_t>(first - row0 * groups), per_row = static_cast<uint32_t>(groups);
   const int sub = threadIdx.x % 16;
   Eight<T> e[kUnits];
@@ -208,10 +196,10 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(NormArgs a
   }
 #pragma unroll
   for (int i = 0; i < kUnits; ++i) {
-    float y[8];
+    float2 y[4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = widen<T>(e[i].v[j]);
-    codes8<VEC>(y, n[i], a.codes + row[i] * a.codes_stride + col[i], a.scales + row[i] * groups + col[i] / 128, sub == 0);
+    for (int j = 0; j < 4; ++j) y[j] = make_float2(widen<T>(e[i].v[2 * j]), widen<T>(e[i].v[2 * j + 1]));
+    codes8<VEC>(y, amax8<T>(e[i]), n[i], a.codes + row[i] * a.codes_stride + col[i], a.scales + row[i] * groups + col[i] / 128, sub == 0);
   }
 }
 

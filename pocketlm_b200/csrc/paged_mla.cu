@@ -21,71 +21,47 @@
 #include "fp8_gemv.cuh"
 #include "plan.cuh"
 #include "router.cuh"
+#include "rows.cuh"
 #include "serving.cuh"
 #include "tcgen05.cuh"
 
 namespace moe {
 namespace {
 
-template <typename T>
-MOE_D T from_float(float v);
-template <>
-MOE_D float from_float<float>(float v) { return v; }
-template <>
-MOE_D __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-template <>
-MOE_D __half from_float<__half>(float v) { return __float2half_rn(v); }
-template <typename T>
-MOE_D float widen(T v) { return static_cast<float>(v); }
-
-// Eight values: 16-byte accesses when VEC, else the first n one at a time.
-template <typename T, bool VEC>
-MOE_D void load8(const T* p, int n, float (&f)[8]) {
-  if (VEC) {
-    constexpr int kV = 16 / sizeof(T);
-#pragma unroll
-    for (int i = 0; i < 8 / kV; ++i) unpack16<T>(__ldg(reinterpret_cast<const uint4*>(p) + i), f + i * kV);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = i < n ? widen<T>(p[i]) : 0.0f;
-  }
-}
-template <typename T, bool VEC>
-MOE_D void store8(T* p, int n, const float (&f)[8]) {
-  if (VEC) {
-    __align__(16) T v[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = from_float<T>(f[i]);
-    *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(v);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < n) p[i] = from_float<T>(f[i]);
-  }
-}
-
 constexpr int kAppendThreads = 256;
 constexpr int kAppendVectors = 4;  // 8-value vectors of a latent row per lane: latent <= 1024
 
-// Pairs (2p, 2p + 1) of eight values from column c of a rope group, turned.
-MOE_D void rotate8(float (&f)[8], int n, const float* cos, const float* sin, int64_t c) {
+// The angles of the pairs at columns c, c + 2, .. of a rope group of n more columns.
+struct Angles {
+  float cos[4], sin[4];
+};
+MOE_D Angles angles_at(const float* cos, const float* sin, int c, int n) {
+  Angles a;
 #pragma unroll
   for (int p = 0; p < 4; ++p) {
-    if (2 * p >= n) break;
-    const float cs = __ldg(cos + c / 2 + p), sn = __ldg(sin + c / 2 + p);
-    const float a = f[2 * p], b = f[2 * p + 1];
-    f[2 * p] = a * cs - b * sn;
-    f[2 * p + 1] = a * sn + b * cs;
+    a.cos[p] = 2 * p < n ? __ldg(cos + c / 2 + p) : 0.0f;
+    a.sin[p] = 2 * p < n ? __ldg(sin + c / 2 + p) : 0.0f;
   }
+  return a;
+}
+template <typename T, typename C>
+MOE_D Eight<C> rotated(const Eight<T>& e, const Angles& a) {
+  Eight<C> r;
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    const float x = widen<T>(e.v[2 * p]), y = widen<T>(e.v[2 * p + 1]);
+    r.v[2 * p] = from_float<C>(x * a.cos[p] - y * a.sin[p]);
+    r.v[2 * p + 1] = from_float<C>(x * a.sin[p] + y * a.cos[p]);
+  }
+  return r;
 }
 
 // A CTA per token (and step): its last warp the cache row, the others the
-// queries, eight values of one head's group per thread and up to kAppendLoads
-// of them in flight.  The thread's column within a head stays the same where
-// the threads are a multiple of a head's vectors, and its angles with it.
+// queries: a thread keeps its eight columns of a head, and their angles, over
+// the heads that it takes, kAppendLoads of them in flight.
 constexpr int kAppendLoads = 4;
 template <typename T, typename W, typename C, bool VEC>
-__global__ void __launch_bounds__(kAppendThreads + kWarp) paged_append_kernel(AppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads + kWarp, 5) paged_append_kernel(AppendArgs a) {
   const int tid = threadIdx.x, q_threads = blockDim.x - kWarp, lane = tid % kWarp;
   const int latent = static_cast<int>(a.latent), rope = static_cast<int>(a.rope);
   for (int64_t t = blockIdx.x; t < a.tokens; t += gridDim.x) {
@@ -103,57 +79,58 @@ __global__ void __launch_bounds__(kAppendThreads + kWarp) paged_append_kernel(Ap
       const T* src = static_cast<const T*>(a.kv) + t * a.kv_stride;
       const int64_t page = slot / a.page_size;
       C* dst = static_cast<C*>(a.cache) + page * a.page_stride + (slot - page * a.page_size) * a.row_stride;
-      float f[kAppendVectors][8];
+      Eight<T> e[kAppendVectors];
       float ss = 0.0f;
 #pragma unroll
       for (int v = 0; v < kAppendVectors; ++v) {
         const int c = 8 * (lane + v * kWarp), n = min(latent - c, 8);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) f[v][j] = 0.0f;
-        if (n > 0) load8<T, VEC>(src + c, n, f[v]);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) ss = fmaf(f[v][j], f[v][j], ss);
+        clear8(e[v]);
+        if (n > 0) load8<T, VEC>(src + c, n, e[v]);
       }
+#pragma unroll
+      for (int v = 0; v < kAppendVectors; ++v)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) ss = fmaf(widen<T>(e[v].v[j]), widen<T>(e[v].v[j]), ss);
       const float inv = 1.0f / sqrtf(warp_sum(ss) / static_cast<float>(latent) + a.eps);
 #pragma unroll
       for (int v = 0; v < kAppendVectors; ++v) {
         const int c = 8 * (lane + v * kWarp), n = min(latent - c, 8);
-        if (n <= 0) continue;
-        float w[8];
+        if (n <= 0) break;
+        Eight<W> w;
+        Eight<C> o;
         load8<W, VEC>(static_cast<const W*>(a.norm_w) + c, n, w);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[v][j] *= inv * w[j];
-        store8<C, VEC>(dst + c, n, f[v]);
+        for (int j = 0; j < 8; ++j) o.v[j] = from_float<C>(widen<T>(e[v].v[j]) * inv * widen<W>(w.v[j]));
+        store8<C, VEC>(dst + c, n, o);
       }
       for (int c = 8 * lane; c < rope; c += 8 * kWarp) {
         const int n = min(rope - c, 8);
-        load8<T, VEC>(src + latent + c, n, f[0]);
-        rotate8(f[0], n, cos, sin, c);
-        store8<C, VEC>(dst + latent + c, n, f[0]);
+        load8<T, VEC>(src + latent + c, n, e[0]);
+        store8<C, VEC>(dst + latent + c, n, rotated<T, C>(e[0], angles_at(cos, sin, c, n)));
       }
       continue;
     }
-    const int per_head = (rope + 7) / 8, vectors = static_cast<int>(a.heads) * per_head;
-    const C* q = static_cast<const C*>(a.q) + t * a.q_stride;
-    C* out = static_cast<C*>(a.q_out) + t * a.heads * rope;
-    for (int v0 = tid; v0 < vectors; v0 += q_threads * kAppendLoads) {
-      float f[kAppendLoads][8];
+    const int per_head = (rope + 7) / 8, at_once = q_threads / per_head;  // heads at once
+    if (tid >= at_once * per_head) continue;
+    const int h0 = tid / per_head, c = 8 * (tid - h0 * per_head), n = min(rope - c, 8);
+    const C* q = static_cast<const C*>(a.q) + t * a.q_stride + c;
+    C* out = static_cast<C*>(a.q_out) + t * a.heads * rope + c;
+    Eight<C> e[kAppendLoads];
+    auto load = [&](int h) {
+#pragma unroll
+      for (int i = 0; i < kAppendLoads; ++i)
+        if (h + i * at_once < a.heads) load8<C, VEC>(q + (h + i * at_once) * a.q_head_stride, n, e[i]);
+    };
+    load(h0);  // before the angles, which wait for the position
+    const Angles turn = angles_at(cos, sin, c, n);
+    for (int h = h0; h < a.heads; h += at_once * kAppendLoads) {
+      if (h != h0) load(h);
 #pragma unroll
       for (int i = 0; i < kAppendLoads; ++i) {
-        const int v = v0 + i * q_threads, h = v / per_head, c = 8 * (v - h * per_head);
-        if (v < vectors) load8<C, VEC>(q + h * a.q_head_stride + c, min(rope - c, 8), f[i]);
-      }
-#pragma unroll
-      for (int i = 0; i < kAppendLoads; ++i) {
-        const int v = v0 + i * q_threads, h = v / per_head, c = 8 * (v - h * per_head), n = min(rope - c, 8);
-        if (v >= vectors) break;
-        if (placed) {
-          rotate8(f[i], n, cos, sin, c);
-        } else {  // a row that has no place in the sequence: zeros
-#pragma unroll
-          for (int j = 0; j < 8; ++j) f[i][j] = 0.0f;
-        }
-        store8<C, VEC>(out + h * rope + c, n, f[i]);
+        if (h + i * at_once >= a.heads) break;
+        Eight<C> o = rotated<C, C>(e[i], turn);
+        if (!placed) clear8(o);  // a row that has no place in the sequence: zeros
+        store8<C, VEC>(out + (h + i * at_once) * rope, n, o);
       }
     }
   }
