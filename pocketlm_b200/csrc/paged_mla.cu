@@ -164,74 +164,75 @@ cudaError_t launch_append_types(const AppendArgs& a, int x_dtype, int norm_dtype
 
 // ------------------------------------------------------------- attention
 //
-// A CTA takes 128 heads of one row and half of the latent columns of the
-// result; the two CTAs of a pair compute the same scores.  Tensor memory holds
-// the 128 x 256 fp32 result, two 128 x 64 score tiles (the softmax of one while
-// the other is computed; its 16-bit probabilities replace the scores) and 256
-// columns of the queries: all 512 columns.  Shared memory holds the queries'
-// other columns (80 KiB) and the cache rows in chunks of 64 positions x 64
-// columns (8 KiB, 128B-swizzled): the chunks of this CTA's own columns stay
-// until the second product has read them (3 tiles of them), the others pass
-// through 6 slots as the scores are computed.
-//   scores  S = Q K^T:  M = 128 heads, N = 64 positions, k over the columns
-//   result  O += P V:   M = 128 heads, N = own columns, k over the positions;
-// V is the same shared memory as K, read as an MN-major operand.
-// Halving the columns costs the scores twice (832 instead of 544 multiply-adds
-// per head and position and CTA) but leaves room in tensor memory for the
-// overlap; the cache is read from memory once, the pair's second read hits L2.
+// A pair of CTAs takes 128 heads of one row, 64 each, as one tcgen05.mma
+// cta_group::2 product with M = 128 over the pair:
+//   scores  S = Q K^T:  N = 128 positions (64 from each CTA), k over the columns
+//   result  O += P V:   N = 256 latent columns (128 from each CTA), k over the
+//                       positions, twice for 512 columns
+// At M = 128 a pair's product costs N / 4 cycles (measured: 34 at N = 128, 66 at
+// N = 256), all of the tensor cores' rate; one CTA alone with M = 128 needs
+// 76 cycles at N = 64 and has no room in tensor memory for 512 columns of result.
+// In tensor memory a CTA's 64 heads lie in lanes 0-63 with the first half of N
+// and in lanes 64-127 with the second: a softmax thread holds 64 positions of
+// one head, and shares the head's maximum and sum with the thread 64 further.
+//
+// Shared memory: the queries (9 chunks of 64 heads x 64 columns, 8 KiB), two
+// buffers of probabilities (16-bit, 16 KiB each) and a ring of 16 KiB stages
+// that the cache's chunks (64 positions x 64 columns, 128B-swizzled) pass
+// through: for a tile, two chunks of K per stage, then V (the same rows again,
+// from L2, as an MN-major operand: own columns, all 128 positions).  Bytes bound
+// it: a position's 1152 bytes come from memory once per 128 heads.
 //
 // The softmax's reference maximum moves only when a tile's maximum exceeds it
 // by 2^8 (log2 domain): probabilities stay below 2^8 of the reference's 1, well
-// inside 16-bit range, and the 256 columns of the result are rescaled rarely.
-// Probabilities are rounded to the cache's type for the second product, half a
-// step each; their sum is of the unrounded fp32 values.
+// inside 16-bit range, and the result is rescaled rarely.  Probabilities are
+// rounded to the cache's type for the second product, half a step each; their
+// sum is of the unrounded fp32 values.
 //
-// Work: all rows' tiles of 64 positions in one sequence, cut into equal
-// ranges, one per CTA pair, so that lengths need not be alike.  A row inside
-// one range is finished there; a row that is cut leaves fp32 parts in the
-// workspace, which the second kernel joins.  A range has at most two parts.
+// Work: all rows' tiles of 128 positions in one sequence, cut into equal
+// ranges, one per pair of CTAs, so that lengths need not be alike.  A row
+// inside one range is finished there; a row that is cut leaves fp32 parts in
+// the workspace, which the second kernel joins.  A range has at most two parts.
 //
-// Warps 0-3: softmax, result (a thread per head).  4-7: the cache's rows.
-// 8: tensor memory and the products (the whole warp walks the work, so that
-// operand descriptors stay in uniform registers; one lane issues).
+// Rows arrive by TMA, one box per run of positions that no page border cuts (the
+// largest power of two, up to 64, that divides the page size).  Positions that
+// do not take part -- past the length, or on a page outside the cache -- arrive
+// as zeros, from coordinates outside the tensor, whatever their memory holds;
+// a run that the length cuts comes row by row.  Their scores are masked.
 //
-// Rows arrive by TMA, one box per chunk and run of positions that no page
-// border cuts (gcd(page size, 64) of them), or, where such runs are shorter than
-// 8, by 16-byte asynchronous copies of four warps.  Positions that do not take
-// part (past the length, or on a page outside the cache) are masked in the scores;
-// their rows may hold anything, NaN among it, so the softmax warps clear them
-// in shared memory before the second product reads them with probability 0.
-constexpr int kTile = 64;
-constexpr int kHeads = 128;
-constexpr int kChunkBytes = kTile * 128;
-constexpr int kQChunkBytes = kHeads * 128;
-constexpr int kQTmemChunks = 4, kQSmemChunks = 5;
-constexpr int kKeptStages = 3, kKeptChunks = 4;
-constexpr int kPassing = 6;
-constexpr int kSoftmaxThreads = 128, kCopyThreads = 128;
-constexpr int kAttnThreads = kSoftmaxThreads + kCopyThreads + kWarp;
-constexpr int kAttnWarps = kAttnThreads / kWarp;
-constexpr uint32_t kColO = 0, kColS = 256, kColQ = 384;
-constexpr int kMinTiles = 2;  // fewest tiles worth a range of their own
+// Warps 0-3: softmax, result.  4: TMA.  5: tensor memory and, in the first CTA,
+// the products (the whole warp walks the work, so that operand descriptors stay
+// in uniform registers; one lane issues).
+constexpr int kTile = 128, kHalfTile = 64;
+constexpr int kHeads = 128, kCtaHeads = 64;
+constexpr int kChunkBytes = 64 * 128;
+constexpr int kQChunks = 9;
+constexpr int kStages = 7, kStageBytes = 2 * kChunkBytes;
+constexpr int kPBytes = 2 * kChunkBytes;
+constexpr int kSoftmaxWarps = 4, kSoftmaxThreads = kSoftmaxWarps * kWarp;
+constexpr int kAttnWarps = kSoftmaxWarps + 2, kAttnThreads = kAttnWarps * kWarp;
+constexpr uint32_t kColO = 0, kColS = 256;
+constexpr int kMinTiles = 1;  // fewest tiles worth a range of their own
 constexpr float kMovesBy = 8.0f;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct AttnBarriers {
-  uint64_t kept_full[kKeptStages], kept_empty[kKeptStages];
-  uint64_t pass_full[kPassing], pass_empty[kPassing];
-  uint64_t s_full[2];    // scores complete
-  uint64_t p_ready[2];   // probabilities written (one arrival per softmax warp)
-  uint64_t q_ready;      // queries of the next part in place
-  uint64_t o_done;       // a tile's second product complete
-  uint64_t o_read;       // the part's result has been read
+  uint64_t full[kStages];   // of the first CTA: both CTAs' bytes of a stage
+  uint64_t empty[kStages];  // in both
+  uint64_t q_full;          // of the first CTA: both CTAs' queries of a part
+  uint64_t s_full[2];       // scores complete
+  uint64_t p_ready[2];      // of the first CTA: probabilities written (one arrival per softmax warp of both)
+  uint64_t pv_done[2];      // a tile's second product complete
+  uint64_t o_read;          // of the first CTA: the part's result has been read
   uint64_t drain;
   uint32_t tmem_base;
   int abort;
   int first_item, first_tile;
   long long sums[kAttnWarps];
+  float share[2][kSoftmaxThreads];  // what the two threads of a head tell each other
 };
-constexpr size_t kAttnSmem = 1024 + static_cast<size_t>(kQSmemChunks) * kQChunkBytes +
-                             static_cast<size_t>(kKeptStages * kKeptChunks + kPassing) * kChunkBytes + sizeof(AttnBarriers);
+constexpr size_t kAttnSmem = 1024 + static_cast<size_t>(kQChunks) * kChunkBytes + 2 * kPBytes +
+                             static_cast<size_t>(kStages) * kStageBytes + sizeof(AttnBarriers);
 static_assert(kAttnSmem <= 232448, "shared memory per block");
 
 struct AttnPlan {
@@ -309,37 +310,31 @@ MOE_D uint32_t pack2<__half>(float lo, float hi) {
   return r;
 }
 
-MOE_D void copy16(uint32_t dst, const void* src, bool present) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(present ? 16 : 0) : "memory");
-}
-MOE_D void copies_arrive(uint64_t* bar) {
-  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
-}
-
 // A wait of a whole warp: every lane sees the same answer.
-MOE_D bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int code) {
-  return __all_sync(0xFFFFFFFFu, wait_or_abort(bar, parity, abort, code));
+MOE_D bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  return __all_sync(0xFFFFFFFFu, wait_or_abort(bar, parity, abort, kPagedWaitError));
 }
 
-template <typename T, bool TMA>
-__global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const __grid_constant__ CUtensorMap map_cache,
-                                                                          const __grid_constant__ CUtensorMap map_ql,
-                                                                          const __grid_constant__ CUtensorMap map_qp,
-                                                                          PagedAttnArgs a, AttnPlan plan) {
+template <typename T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttnThreads, 1)
+    paged_attention_kernel(const __grid_constant__ CUtensorMap map_runs, const __grid_constant__ CUtensorMap map_rows,
+                           const __grid_constant__ CUtensorMap map_ql, const __grid_constant__ CUtensorMap map_qp,
+                           PagedAttnArgs a, AttnPlan plan) {
   extern __shared__ unsigned char smem_raw[];
+  // the same place in both CTAs (their shared memory starts alike)
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   unsigned char* q_smem = smem;
-  unsigned char* kept_smem = q_smem + kQSmemChunks * kQChunkBytes;
-  unsigned char* pass_smem = kept_smem + kKeptStages * kKeptChunks * kChunkBytes;
-  AttnBarriers* bars = reinterpret_cast<AttnBarriers*>(pass_smem + kPassing * kChunkBytes);
+  unsigned char* p_smem = q_smem + kQChunks * kChunkBytes;
+  unsigned char* ring = p_smem + 2 * kPBytes;
+  AttnBarriers* bars = reinterpret_cast<AttnBarriers*>(ring + kStages * kStageBytes);
   const int tid = threadIdx.x, lane = tid % kWarp, warp = __shfl_sync(0xFFFFFFFFu, tid / kWarp, 0);
   volatile int* abort = &bars->abort;
   const int latent = static_cast<int>(a.latent), rope = static_cast<int>(a.rope);
   const int lat_chunks = (latent + 63) / 64, chunks = lat_chunks + 1;  // the last one holds the rope part
-  const int halves = lat_chunks > 1 ? 2 : 1, per_half = (lat_chunks + halves - 1) / halves;
-  const int worker = blockIdx.x / halves, half = blockIdx.x % halves;
-  const int kept0 = half * per_half, kept_n = min(per_half, lat_chunks - kept0);
-  const int q_tmem = min(kQTmemChunks, lat_chunks);
+  const int own_chunks = (lat_chunks + 1) / 2;                         // latent chunks whose V each CTA brings
+  const int k_stages = (chunks + 1) / 2, v_pairs = (own_chunks + 1) / 2;
+  const uint32_t rank = cluster_rank();
+  const int worker = blockIdx.x / 2;
 
   // tiles before each thread's rows; the range's first item
   long long mine = 0;
@@ -368,7 +363,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const 
     if (tid == 0) plan.before[a.batch] = total;
   }
   const int64_t workers = used_workers(total, plan.workers);
-  if (worker >= workers || total == 0) return;
+  if (worker >= workers || total == 0) return;  // both CTAs of the pair alike
   const int64_t start = range_start(worker, total, workers), stop = range_start(worker + 1, total, workers);
   if (start >= before && start < before + mine) {
     long long at = before;
@@ -383,264 +378,228 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const 
     bars->first_tile = static_cast<int>(start - at);
   }
   if (tid == 0) {
-    for (int s = 0; s < kKeptStages; ++s) {
-      mbar_init(&bars->kept_full[s], TMA ? 1 : kCopyThreads);
-      mbar_init(&bars->kept_empty[s], 1);
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&bars->full[s], 1);
+      mbar_init(&bars->empty[s], 1);
     }
-    for (int s = 0; s < kPassing; ++s) {
-      mbar_init(&bars->pass_full[s], TMA ? 1 : kCopyThreads);
-      mbar_init(&bars->pass_empty[s], 1);
-    }
+    mbar_init(&bars->q_full, 1);
     for (int s = 0; s < 2; ++s) {
       mbar_init(&bars->s_full[s], 1);
-      mbar_init(&bars->p_ready[s], kSoftmaxThreads / kWarp);
+      mbar_init(&bars->p_ready[s], 2 * kSoftmaxWarps);
+      mbar_init(&bars->pv_done[s], 1);
     }
-    mbar_init(&bars->q_ready, kSoftmaxThreads / kWarp + 1);
-    mbar_init(&bars->o_done, 1);
-    mbar_init(&bars->o_read, kSoftmaxThreads / kWarp);
+    mbar_init(&bars->o_read, 2 * kSoftmaxWarps);
     mbar_init(&bars->drain, 1);
     bars->abort = 0;
     fence_barrier_init();
   }
-  if (warp == kAttnWarps - 1) {
-    tmem_alloc(&bars->tmem_base, 512);
-    tmem_relinquish();
-  }
+  if (warp == kAttnWarps - 1) pair_tmem_alloc(&bars->tmem_base, 512);
   tc_fence_before();
   __syncthreads();
+  cluster_sync();
   tc_fence_after();
   const uint32_t tmem = bars->tmem_base;
   Walk walk{bars->first_item, bars->first_tile, stop - start};
   Part p;
 
-  if (TMA && warp >= kSoftmaxThreads / kWarp && warp < kAttnWarps - 1) {
+  if (warp == kSoftmaxWarps) {
     // --------------------------------------------------------------- TMA
-    if (warp == kSoftmaxThreads / kWarp) {
-      const uint32_t kept_at = smem_addr(kept_smem), pass_at = smem_addr(pass_smem);
-      const int run = plan.run, runs = kTile / run, page_size = static_cast<int>(a.page_size);
-      const bool leader = elect_one();
-      uint32_t g = 0, pc = 0, kept = 0;
-      bool ok = true;
-      // lane r: the page of the tile's run r (-1: none) and its first row there
-      auto lookup = [&](int tile, int& page, int& row) {
-        const int pos = tile * kTile + lane * run;
-        page = -1;
-        row = 0;
-        if (lane < runs && pos < p.len) {
-          const int col = pos / page_size;
-          page = __ldg(a.table + p.b * a.table_stride + col);
-          row = pos - col * page_size;
-          if (page >= a.pages) page = -1;
-        }
-      };
-      while (ok && walk.next(a, plan.groups, worker, p)) {
-        int page, row, next_page = -1, next_row = 0;
-        lookup(p.tile0, page, row);
-        for (int i = 0; i < p.tiles && ok; ++i, ++g) {
-          if (i + 1 < p.tiles) lookup(p.tile0 + i + 1, next_page, next_row);
-          const int present = __popc(__ballot_sync(0xFFFFFFFFu, page >= 0));
-          auto fetch = [&](int c, uint32_t dst, uint64_t* bar) {
-            const int x = c < lat_chunks ? c * 64 : latent;
-            for (int r = 0; r < runs; ++r) {
-              const int pg = __shfl_sync(0xFFFFFFFFu, page, r), at = __shfl_sync(0xFFFFFFFFu, row, r);
-              if (pg >= 0 && leader) tma_load_3d(dst + r * run * 128, &map_cache, x, at, pg, bar);
-            }
-          };
-          const int s = g % kKeptStages;
-          if (g >= kKeptStages && !warp_wait(&bars->kept_empty[s], ((g / kKeptStages) - 1) & 1, abort, kPagedWaitError)) {
-            ok = false;
-            break;
-          }
-          if (leader) mbar_arrive_expect_tx(&bars->kept_full[s], present * run * 128 * kept_n);
-          __syncwarp();
-          ++kept;
-          for (int k = 0; k < kept_n; ++k) fetch(kept0 + k, kept_at + (s * kKeptChunks + k) * kChunkBytes, &bars->kept_full[s]);
-          for (int c = 0; c < chunks; ++c) {
-            if (c >= kept0 && c < kept0 + kept_n) continue;
-            const int slot = pc % kPassing;
-            if (pc >= kPassing && !warp_wait(&bars->pass_empty[slot], ((pc / kPassing) - 1) & 1, abort, kPagedWaitError)) {
-              ok = false;
-              break;
-            }
-            if (leader) mbar_arrive_expect_tx(&bars->pass_full[slot], present * run * 128);
-            __syncwarp();
-            fetch(c, pass_at + slot * kChunkBytes, &bars->pass_full[slot]);
-            ++pc;
-          }
-          page = next_page;
-          row = next_row;
-        }
-      }
-      // every copy issued lands before the CTA may exit
-      for (uint32_t j = kept > kKeptStages ? kept - kKeptStages : 0; j < kept; ++j)
-        mbar_wait(&bars->kept_full[j % kKeptStages], (j / kKeptStages) & 1, kPagedWaitError);
-      for (uint32_t j = pc > kPassing ? pc - kPassing : 0; j < pc; ++j)
-        mbar_wait(&bars->pass_full[j % kPassing], (j / kPassing) & 1, kPagedWaitError);
-    }
-  } else if (!TMA && warp >= kSoftmaxThreads / kWarp && warp < kAttnWarps - 1) {
-    // ------------------------------------------------------------ copies
-    const int ct = tid - kSoftmaxThreads, unit = ct % 8, row0 = ct / 8;
-    const uint32_t kept_at = smem_addr(kept_smem), pass_at = smem_addr(pass_smem);
-    uint32_t g = 0, pc = 0;
-    bool ok = true;
-    while (ok && walk.next(a, plan.groups, worker, p)) {
-      const int32_t* table = a.table + p.b * a.table_stride;
-      for (int i = 0; i < p.tiles && ok; ++i, ++g) {
-        const T* src[4];
-        bool live[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int pos = (p.tile0 + i) * kTile + row0 + 16 * j;
-          src[j] = static_cast<const T*>(a.cache);
-          live[j] = pos < p.len;
-          if (live[j]) {
-            const int col = pos / static_cast<int>(a.page_size);
-            const int page = __ldg(table + col);
-            live[j] = page >= 0 && page < a.pages;
-            if (live[j]) src[j] += page * a.page_stride + (pos - col * static_cast<int>(a.page_size)) * a.row_stride;
-          }
-        }
-        // chunk c: columns 64 c .. of the latent part, or the rope part
-        auto fetch = [&](int c, uint32_t dst) {
-          const int col = (c < lat_chunks ? c * 64 : latent) + unit * 8;
-          const bool in = c < lat_chunks ? col < latent : unit * 8 < rope;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int r = row0 + 16 * j;
-            copy16(dst + r * 128 + ((unit ^ (r % 8)) * 16), src[j] + (in ? col : 0), live[j] && in);
-          }
-        };
-        const int s = g % kKeptStages;
-        if (g >= kKeptStages && !wait_or_abort(&bars->kept_empty[s], ((g / kKeptStages) - 1) & 1, abort, kPagedWaitError)) {
-          ok = false;
-          break;
-        }
-        for (int k = 0; k < kept_n; ++k) fetch(kept0 + k, kept_at + (s * kKeptChunks + k) * kChunkBytes);
-        copies_arrive(&bars->kept_full[s]);
-        for (int c = 0; c < chunks; ++c) {
-          if (c >= kept0 && c < kept0 + kept_n) continue;
-          const int slot = pc % kPassing;
-          if (pc >= kPassing && !wait_or_abort(&bars->pass_empty[slot], ((pc / kPassing) - 1) & 1, abort, kPagedWaitError)) {
-            ok = false;
-            break;
-          }
-          fetch(c, pass_at + slot * kChunkBytes);
-          copies_arrive(&bars->pass_full[slot]);
-          ++pc;
-        }
-      }
-    }
-    asm volatile("cp.async.wait_all;" ::: "memory");
-  } else if (warp == kAttnWarps - 1) {
-    // ---------------------------------------------------------- products
+    const uint32_t ring_at = smem_addr(ring), q_at = smem_addr(q_smem);
+    const int run = plan.run, runs = kHalfTile / run, page_size = static_cast<int>(a.page_size);
+    const int outside = static_cast<int>(a.pages);  // a page that the cache does not have: zeros
     const bool leader = elect_one();
-    const int format = __is_same(T, __nv_bfloat16) ? 1 : 0;
-    const uint32_t idesc_s = umma_idesc(kHeads, kTile, format, false);
-    const uint32_t idesc_o = umma_idesc(kHeads, 64 * kept_n, format, true);
-    const uint64_t q_desc = sw128_desc_k(smem_addr(q_smem)), k_desc = sw128_desc_k(smem_addr(kept_smem));
-    const uint64_t pass_desc = sw128_desc_k(smem_addr(pass_smem)), v_desc = sw128_desc(smem_addr(kept_smem), kChunkBytes);
-    uint32_t g = 0, pc = 0, parts = 0;
+    uint32_t g = 0, it = 0, parts = 0;
     bool ok = true;
-    // descriptors advance in units of 16 bytes: 2 per 16 columns of a swizzled row
-    auto chunk_scores = [&](int c, uint64_t b, uint32_t d, bool first) {
-      if (c < q_tmem) {
+    // runs lane and lane + 32 of each half of a tile: page, row in it, positions that take part
+    struct Runs {
+      int page[2][2], row[2][2], live[2][2];
+    };
+    auto lookup = [&](int tile) {
+      Runs r;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) umma_f16_ts(d, tmem + kColQ + c * 32 + k * 8, b + 2 * k, idesc_s, !(first && k == 0));
-      } else {
-        const uint64_t q = q_desc + (c - q_tmem) * (kQChunkBytes / 16);
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) umma_f16_ss(d, q + 2 * k, b + 2 * k, idesc_s, !(first && k == 0));
+        for (int k = 0; k < 2; ++k) {
+          const int i = lane + k * kWarp, pos = tile * kTile + h * kHalfTile + i * run;
+          r.page[h][k] = outside;
+          r.row[h][k] = r.live[h][k] = 0;
+          if (i < runs && pos < p.len) {
+            const int col = pos / page_size, page = __ldg(a.table + p.b * a.table_stride + col);
+            if (page >= 0 && page < a.pages) {
+              r.page[h][k] = page;
+              r.row[h][k] = pos - col * page_size;
+              r.live[h][k] = min(run, p.len - pos);
+            }
+          }
+        }
+      return r;
+    };
+    // 64 positions (half h) x 64 columns from x into dst
+    auto fetch = [&](const Runs& r, int h, int x, uint32_t dst, uint32_t bar) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int i = lane + k * kWarp, live = r.live[h][k];
+        const bool cut = live > 0 && live < run;
+        if (i < runs && !cut) pair_tma_load_3d(dst + i * run * 128, &map_runs, x, r.row[h][k], r.page[h][k], bar);
+        uint32_t cuts = __ballot_sync(0xFFFFFFFFu, cut);  // at most one run of a row: its last
+        if (cuts) {
+          const int from = __ffs(cuts) - 1;
+          const int n = __shfl_sync(0xFFFFFFFFu, live, from), page = __shfl_sync(0xFFFFFFFFu, r.page[h][k], from);
+          const int row = __shfl_sync(0xFFFFFFFFu, r.row[h][k], from), first = (from + k * kWarp) * run;
+          for (int j = lane; j < run; j += kWarp)
+            pair_tma_load_3d(dst + (first + j) * 128, &map_rows, x, row + j, j < n ? page : outside, bar);
+        }
       }
     };
-    // the scores of the tile whose number is t
-    auto scores = [&](uint32_t t) {
-      const uint32_t s = t % kKeptStages, d = tmem + kColS + (t % 2) * kTile;
-      if (!warp_wait(&bars->kept_full[s], (t / kKeptStages) & 1, abort, kPagedWaitError)) return false;
-      if (!TMA) fence_proxy_async_shared();
-      tc_fence_after();
-      for (int k = 0; k < kept_n; ++k)
-        if (leader) chunk_scores(kept0 + k, k_desc + (s * kKeptChunks + k) * (kChunkBytes / 16), d, k == 0);
-      for (int c = 0; c < chunks; ++c) {
-        if (c >= kept0 && c < kept0 + kept_n) continue;
-        const uint32_t slot = pc % kPassing;
-        if (!warp_wait(&bars->pass_full[slot], (pc / kPassing) & 1, abort, kPagedWaitError)) return false;
-        if (!TMA) fence_proxy_async_shared();
-        tc_fence_after();
-        if (leader) {
-          chunk_scores(c, pass_desc + slot * (kChunkBytes / 16), d, false);
-          umma_commit(&bars->pass_empty[slot]);
-        }
-        __syncwarp();
-        ++pc;
-      }
-      if (leader) umma_commit(&bars->s_full[t % 2]);
+    // the next stage is free: its memory, and the first CTA's barrier armed with both CTAs' bytes
+    auto open = [&](int n_chunks, uint32_t& dst, uint32_t& bar) {
+      const uint32_t s = it % kStages;
+      if (it >= kStages && !warp_wait(&bars->empty[s], ((it / kStages) - 1) & 1, abort)) return false;
+      if (rank == 0 && leader) mbar_arrive_expect_tx(&bars->full[s], 2 * n_chunks * kChunkBytes);
       __syncwarp();
+      dst = ring_at + s * kStageBytes;
+      bar = cluster_addr(&bars->full[s], 0);
+      ++it;
+      return true;
+    };
+    auto fetch_k = [&](const Runs& r) {
+      for (int u = 0; u < k_stages; ++u) {
+        const int n = min(2, chunks - 2 * u);
+        uint32_t dst, bar;
+        if (!open(n, dst, bar)) return false;
+        for (int c = 2 * u; c < 2 * u + n; ++c)
+          fetch(r, rank, c < lat_chunks ? c * 64 : latent, dst + (c - 2 * u) * kChunkBytes, bar);
+      }
+      return true;
+    };
+    auto fetch_v = [&](const Runs& r) {
+      for (int h = 0; h < 2; ++h)
+        for (int j = 0; j < v_pairs; ++j) {
+          uint32_t dst, bar;
+          if (!open(2, dst, bar)) return false;
+          const int c = static_cast<int>(rank) * own_chunks + 2 * j;
+          fetch(r, h, c * 64, dst, bar);
+          fetch(r, h, (c + 1) * 64, dst + kChunkBytes, bar);
+        }
       return true;
     };
     while (ok && walk.next(a, plan.groups, worker, p)) {
-      const int tiles = __shfl_sync(0xFFFFFFFFu, p.tiles, 0);
-      if (!warp_wait(&bars->q_ready, parts & 1, abort, kPagedWaitError)) break;
-      tc_fence_after();
-      ok = scores(g);
-      for (int i = 0; i < tiles && ok; ++i, ++g) {
-        if (i + 1 < tiles && !(ok = scores(g + 1))) break;
-        if (!(ok = warp_wait(&bars->p_ready[g % 2], (g / 2) & 1, abort, kPagedWaitError))) break;
-        if (i == 0 && parts > 0 && !(ok = warp_wait(&bars->o_read, (parts - 1) & 1, abort, kPagedWaitError))) break;
-        tc_fence_after();
-        const uint32_t s = g % kKeptStages;
-        if (leader) {
-          const uint64_t v = v_desc + s * (kKeptChunks * kChunkBytes / 16);
-#pragma unroll
-          for (int k = 0; k < kTile / 16; ++k)
-            umma_f16_ts(tmem + kColO, tmem + kColS + (g % 2) * kTile + k * 8, v + k * (2048 / 16), idesc_o, i > 0 || k > 0);
-          umma_commit(&bars->kept_empty[s]);
-          umma_commit(&bars->o_done);
+      Runs now = lookup(p.tile0);
+      if (parts > 0 && !(ok = warp_wait(&bars->s_full[(g - 1) % 2], ((g - 1) / 2) & 1, abort))) break;  // the queries' last use
+      if (leader) {
+        const uint32_t bar = cluster_addr(&bars->q_full, 0);
+        if (rank == 0) mbar_arrive_expect_tx(&bars->q_full, 2 * chunks * kChunkBytes);
+        for (int c = 0; c < chunks; ++c)
+          pair_tma_load_3d(q_at + c * kChunkBytes, c < lat_chunks ? &map_ql : &map_qp, c < lat_chunks ? c * 64 : 0,
+                           p.group * kHeads + static_cast<int>(rank) * kCtaHeads, static_cast<int>(p.b), bar);
+      }
+      __syncwarp();
+      ok = fetch_k(now);
+      for (int i = 0; i < p.tiles && ok; ++i, ++g) {
+        Runs next = now;
+        if (i + 1 < p.tiles) {
+          next = lookup(p.tile0 + i + 1);
+          ok = fetch_k(next);
         }
-        __syncwarp();
+        ok = ok && fetch_v(now);
+        now = next;
       }
       ++parts;
     }
-    if (leader) umma_commit(&bars->drain);  // every product issued is complete before tensor memory is freed
-    __syncwarp();
-    mbar_wait(&bars->drain, 0, kPagedWaitError);
+    // the copies issued land before either CTA leaves: the first one's barriers count them all, and what
+    // the products have consumed had landed
+    for (uint32_t j = it > kStages ? it - kStages : 0; j < it; ++j)
+      mbar_wait(rank == 0 ? &bars->full[j % kStages] : &bars->empty[j % kStages], (j / kStages) & 1, kPagedWaitError);
+  } else if (warp == kAttnWarps - 1) {
+    // ---------------------------------------------------------- products
+    if (rank == 0) {
+      const bool leader = elect_one();
+      const int format = __is_same(T, __nv_bfloat16) ? 1 : 0;
+      const uint32_t idesc_s = umma_idesc(kHeads, kTile, format, false), idesc_o = umma_idesc(kHeads, 256, format, true);
+      const uint64_t q_desc = sw128_desc_k(smem_addr(q_smem)), p_desc = sw128_desc_k(smem_addr(p_smem));
+      const uint64_t k_desc = sw128_desc_k(smem_addr(ring)), v_desc = sw128_desc(smem_addr(ring), kChunkBytes);
+      uint32_t g = 0, it = 0, parts = 0;
+      bool ok = true;
+      // descriptors advance in units of 16 bytes
+      auto scores = [&](uint32_t t) {
+        const uint32_t d = tmem + kColS + (t % 2) * (kTile / 2);
+        for (int u = 0; u < k_stages; ++u, ++it) {
+          const uint32_t s = it % kStages;
+          if (!warp_wait(&bars->full[s], (it / kStages) & 1, abort)) return false;
+          tc_fence_after();
+          if (leader) {
+            const int n = min(2, chunks - 2 * u);
+            for (int c = 0; c < n; ++c) {
+              const uint64_t q = q_desc + (2 * u + c) * (kChunkBytes / 16), k = k_desc + s * (kStageBytes / 16) + c * (kChunkBytes / 16);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) pair_umma_f16_ss(d, q + 2 * i, k + 2 * i, idesc_s, u > 0 || c > 0 || i > 0);
+            }
+            pair_umma_commit(&bars->empty[s]);
+          }
+          __syncwarp();
+        }
+        if (leader) pair_umma_commit(&bars->s_full[t % 2]);
+        __syncwarp();
+        return true;
+      };
+      while (ok && walk.next(a, plan.groups, worker, p)) {
+        const int tiles = __shfl_sync(0xFFFFFFFFu, p.tiles, 0);
+        if (!warp_wait(&bars->q_full, parts & 1, abort)) break;
+        ok = scores(g);
+        for (int i = 0; i < tiles && ok; ++i, ++g) {
+          if (i + 1 < tiles && !(ok = scores(g + 1))) break;
+          if (!(ok = warp_wait(&bars->p_ready[g % 2], (g / 2) & 1, abort))) break;
+          if (i == 0 && parts > 0 && !(ok = warp_wait(&bars->o_read, (parts - 1) & 1, abort))) break;
+          for (int h = 0; h < 2 && ok; ++h)
+            for (int j = 0; j < v_pairs; ++j, ++it) {
+              const uint32_t s = it % kStages;
+              if (!(ok = warp_wait(&bars->full[s], (it / kStages) & 1, abort))) break;
+              tc_fence_after();
+              if (leader) {
+                const uint64_t pd = p_desc + (g % 2) * (kPBytes / 16) + h * (kChunkBytes / 16), v = v_desc + s * (kStageBytes / 16);
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                  pair_umma_f16_ss(tmem + kColO + j * 128, pd + 2 * k, v + k * (2048 / 16), idesc_o, i > 0 || h > 0 || k > 0);
+                pair_umma_commit(&bars->empty[s]);
+              }
+              __syncwarp();
+            }
+          if (leader) pair_umma_commit(&bars->pv_done[g % 2]);
+          __syncwarp();
+        }
+        ++parts;
+      }
+      if (leader) pair_umma_commit(&bars->drain);
+      __syncwarp();
+    }
+    mbar_wait(&bars->drain, 0, kPagedWaitError);  // in both CTAs: every product is complete
   } else {
     // ------------------------------------------------- softmax and result
     const float c2 = fmaxf(a.scale * kLog2e, 1e-37f);  // above 0: a masked score's -inf stays one
     const uint32_t my_lanes = static_cast<uint32_t>(warp * kWarp) << 16;
     const int page_size = static_cast<int>(a.page_size);
-    // the part's queries: columns from 64 q_tmem on by TMA (absent heads and columns arrive as zeros), the others a
-    // thread its own row, all loads in flight together
-    auto load_queries = [&](const Part& p) {
-      const int h0 = p.group * kHeads, nh = static_cast<int>(min(a.heads - h0, static_cast<int64_t>(kHeads)));
-      if (tid == 0) {
-        mbar_arrive_expect_tx(&bars->q_ready, (chunks - q_tmem) * kQChunkBytes);
-        for (int c = q_tmem; c < chunks; ++c)
-          tma_load_3d(smem_addr(q_smem) + (c - q_tmem) * kQChunkBytes, c < lat_chunks ? &map_ql : &map_qp,
-                      c < lat_chunks ? c * 64 : 0, h0, static_cast<int>(p.b), &bars->q_ready);
-      }
-      __syncwarp();
-      const T* ql = static_cast<const T*>(a.q_latent) + p.b * a.ql_stride + (h0 + tid) * a.ql_head_stride;
-      __align__(16) uint32_t v[kQTmemChunks][32];
-#pragma unroll
-      for (int c = 0; c < kQTmemChunks; ++c)
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const int col = c * 64 + u * 8;
-          *reinterpret_cast<uint4*>(v[c] + 4 * u) = tid < nh && c < q_tmem && col < latent
-                                                        ? __ldg(reinterpret_cast<const uint4*>(ql + col))
-                                                        : make_uint4(0, 0, 0, 0);
-        }
-#pragma unroll
-      for (int c = 0; c < kQTmemChunks; ++c) tmem_st32(tmem + my_lanes + kColQ + c * 32, v[c]);
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->q_ready);
+    const int head = tid % kCtaHeads, part_of = tid / kCtaHeads;  // the thread's head of the CTA, and half of N
+    const uint32_t ready_at[2] = {cluster_addr(&bars->p_ready[0], 0), cluster_addr(&bars->p_ready[1], 0)};
+    const uint32_t read_at = cluster_addr(&bars->o_read, 0);
+    int turn = 0;
+    // the value of this thread's head in the other half; `fine` becomes whether it is for all four warps, so
+    // that after a wait that ran out they leave together
+    auto other = [&](float v, bool& fine) {
+      bars->share[turn][tid] = v;
+      uint32_t all;
+      asm volatile(
+          "{\n .reg .pred p, q;\n setp.ne.u32 q, %1, 0;\n bar.red.and.pred p, 1, %2, q;\n selp.u32 %0, 1, 0, p;\n}"
+          : "=r"(all)
+          : "r"(static_cast<uint32_t>(fine)), "n"(kSoftmaxThreads)
+          : "memory");
+      fine = all != 0;
+      const float got = bars->share[turn][tid ^ kCtaHeads];
+      turn ^= 1;
+      return got;
     };
     uint32_t g = 0;
-    bool ok = true, more = walk.next(a, plan.groups, worker, p);
-    if (more) load_queries(p);
-    while (ok && more) {
+    bool ok = true;
+    while (ok && walk.next(a, plan.groups, worker, p)) {
       float m = -INFINITY, l = 0.0f;
       const int32_t* table = a.table + p.b * a.table_stride;
       for (int i = 0; i < p.tiles; ++i, ++g) {
@@ -648,7 +607,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const 
         uint32_t live[2];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const int pos = (p.tile0 + i) * kTile + k * kWarp + lane;
+          const int pos = (p.tile0 + i) * kTile + part_of * kHalfTile + k * kWarp + lane;
           bool in = pos < p.len;
           if (in) {
             const int page = __ldg(table + pos / page_size);
@@ -657,33 +616,30 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const 
           }
           live[k] = __ballot_sync(0xFFFFFFFFu, in);
         }
-        if (!warp_wait(&bars->s_full[g % 2], (g / 2) & 1, abort, kPagedWaitError)) {
-          ok = false;
-          break;
-        }
+        bool got = ok && warp_wait(&bars->s_full[g % 2], (g / 2) & 1, abort);
+        if (got && g >= 2) got = warp_wait(&bars->pv_done[g % 2], ((g / 2) - 1) & 1, abort);  // the buffer of probabilities
         tc_fence_after();
-        const uint32_t s_at = tmem + my_lanes + kColS + (g % 2) * kTile;
-        uint32_t r[kTile];
-        tmem_ld32(s_at, r);
-        tmem_ld32(s_at + 32, r + 32);
+        uint32_t r[kHalfTile];
+        tmem_ld32(tmem + my_lanes + kColS + (g % 2) * kHalfTile, r);
+        tmem_ld32(tmem + my_lanes + kColS + (g % 2) * kHalfTile + 32, r + 32);
         tmem_ld_wait();
         if ((live[0] & live[1]) != 0xFFFFFFFFu) {
 #pragma unroll
-          for (int j = 0; j < kTile; ++j)
+          for (int j = 0; j < kHalfTile; ++j)
             if (!(live[j / 32] >> (j % 32) & 1u)) r[j] = 0xFF800000u;  // -inf
-          if (TMA) {  // the scores are complete: nothing reads these rows now but the second product
-            unsigned char* v_at = kept_smem + (g % kKeptStages) * kKeptChunks * kChunkBytes;
-            for (int row = tid / 8; row < kTile; row += kSoftmaxThreads / 8)
-              if (!(live[row / 32] >> (row % 32) & 1u))
-                for (int k = 0; k < kept_n; ++k)
-                  *reinterpret_cast<uint4*>(v_at + k * kChunkBytes + row * 128 + (tid % 8) * 16) = make_uint4(0, 0, 0, 0);
-            fence_proxy_async_shared();
-          }
         }
-        float top = -INFINITY;
+        float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < kTile; ++j) top = fmaxf(top, __uint_as_float(r[j]));
-        top *= c2;
+        for (int j = 0; j < kHalfTile; j += 2) {
+          t0 = fmaxf(t0, __uint_as_float(r[j]));
+          t1 = fmaxf(t1, __uint_as_float(r[j + 1]));
+        }
+        float top = fmaxf(t0, t1);
+        top = fmaxf(top, other(top, got)) * c2;
+        if (!got) {
+          ok = false;
+          break;
+        }
         const bool moves = top > m + kMovesBy || (m == -INFINITY && top > m);
         if (__any_sync(0xFFFFFFFFu, moves)) {
           const float f = !moves ? 1.0f : m == -INFINITY ? 0.0f : exp2_fast(m - top);
@@ -692,12 +648,9 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const 
             m = top;
           }
           if (i > 0) {
-            if (!warp_wait(&bars->o_done, (g - 1) & 1, abort, kPagedWaitError)) {
-              ok = false;
-              break;
-            }
+            ok = warp_wait(&bars->pv_done[(g - 1) % 2], ((g - 1) / 2) & 1, abort);  // (a failure shows in the next wait of all)
             tc_fence_after();
-            for (int c = 0; c < 64 * kept_n; c += 32) {
+            for (int c = 0; c < v_pairs * 128; c += 32) {
               uint32_t o[32];
               tmem_ld32(tmem + my_lanes + kColO + c, o);
               tmem_ld_wait();
@@ -711,7 +664,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const 
         const float ref = m == -INFINITY ? 0.0f : m;
         float sum0 = 0.0f, sum1 = 0.0f;
 #pragma unroll
-        for (int j = 0; j < kTile; j += 2) {
+        for (int j = 0; j < kHalfTile; j += 2) {
           const float p0 = exp2_fast(fmaf(__uint_as_float(r[j]), c2, -ref));
           const float p1 = exp2_fast(fmaf(__uint_as_float(r[j + 1]), c2, -ref));
           sum0 += p0;
@@ -719,58 +672,70 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const 
           r[j / 2] = pack2<T>(p0, p1);
         }
         l += sum0 + sum1;
-        tmem_st32(s_at, r);
-        tmem_st_wait();
+        unsigned char* dst = p_smem + (g % 2) * kPBytes + part_of * kChunkBytes + head * 128;
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          *reinterpret_cast<uint4*>(dst + ((u ^ (head % 8)) * 16)) = make_uint4(r[4 * u], r[4 * u + 1], r[4 * u + 2], r[4 * u + 3]);
+        fence_proxy_async_shared();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bars->p_ready[g % 2]);
+        if (lane == 0) cluster_arrive(ready_at[g % 2]);
       }
+      ok = ok && warp_wait(&bars->pv_done[(g - 1) % 2], ((g - 1) / 2) & 1, abort);
+      const float sum = l + other(l, ok);
       if (!ok) break;
-      const Part done = p;
-      more = walk.next(a, plan.groups, worker, p);
-      if (more) load_queries(p);  // the last scores are complete: the queries' places are free
-      if (!warp_wait(&bars->o_done, (g - 1) & 1, abort, kPagedWaitError)) break;
       tc_fence_after();
-      const int64_t h = done.group * kHeads + tid;
-      const bool has = h < a.heads;
-      const int col0 = kept0 * 64, cols = min(64 * kept_n, latent - col0);
-      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-      T* out = static_cast<T*>(a.out) + (done.b * a.heads + h) * latent + col0;
-      float* part = plan.part_o + (static_cast<int64_t>(done.slot) * kHeads + tid) * latent + col0;
-      for (int c = 0; c < cols; c += 32) {
-        uint32_t o[32];
-        tmem_ld32(tmem + my_lanes + kColO + c, o);
-        tmem_ld_wait();
-        if (!has) continue;
+      // through the probabilities' buffers, which nothing uses now: 64 columns of the warp's 32 heads at a time, so
+      // that sixteen lanes write a head's columns side by side
+      float* stage = reinterpret_cast<float*>(p_smem) + warp * (kWarp * 64);
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      const int64_t h0 = p.group * kHeads + static_cast<int64_t>(rank) * kCtaHeads + (warp % 2) * kWarp;  // the warp's first head
+      for (int c = 0; c < own_chunks; ++c) {  // chunk c of this half of N
+        const int col0 = (part_of * own_chunks + c) * 64;
+        if (col0 >= latent) break;
 #pragma unroll
-        for (int j = 0; j < 32; j += 8) {
-          if (c + j >= cols) break;
-          if (done.whole) {
-            uint4 v;
-            v.x = pack2<T>(__uint_as_float(o[j]) * inv, __uint_as_float(o[j + 1]) * inv);
-            v.y = pack2<T>(__uint_as_float(o[j + 2]) * inv, __uint_as_float(o[j + 3]) * inv);
-            v.z = pack2<T>(__uint_as_float(o[j + 4]) * inv, __uint_as_float(o[j + 5]) * inv);
-            v.w = pack2<T>(__uint_as_float(o[j + 6]) * inv, __uint_as_float(o[j + 7]) * inv);
-            *reinterpret_cast<uint4*>(out + c + j) = v;
-          } else {
-            *reinterpret_cast<uint4*>(part + c + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
-            *reinterpret_cast<uint4*>(part + c + j + 4) = make_uint4(o[j + 4], o[j + 5], o[j + 6], o[j + 7]);
+        for (int k = 0; k < 64; k += 32) {
+          uint32_t o[32];
+          tmem_ld32(tmem + my_lanes + kColO + c * 64 + k, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            float4 v = make_float4(__uint_as_float(o[j]), __uint_as_float(o[j + 1]), __uint_as_float(o[j + 2]), __uint_as_float(o[j + 3]));
+            if (p.whole) v = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+            *reinterpret_cast<float4*>(stage + lane * 64 + (((k + j) / 4) ^ (lane % 8)) * 4) = v;
           }
         }
+        __syncwarp();
+        const int unit = lane % 16, col = col0 + unit * 4;
+#pragma unroll 4
+        for (int row = lane / 16; row < kWarp; row += 2) {
+          const int64_t h = h0 + row;
+          const float4 v = *reinterpret_cast<const float4*>(stage + row * 64 + ((unit ^ (row % 8)) * 4));
+          if (h >= a.heads || col >= latent) continue;
+          if (p.whole)
+            *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (p.b * a.heads + h) * latent + col) =
+                make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w));
+          else
+            *reinterpret_cast<float4*>(plan.part_o + (static_cast<int64_t>(p.slot) * kHeads + (h - p.group * kHeads)) * latent + col) = v;
+        }
+        __syncwarp();
       }
-      if (half == 0 && has) {
-        if (!done.whole) plan.part_ml[static_cast<int64_t>(done.slot) * kHeads + tid] = make_float2(m, l);
-        else if (a.lse) a.lse[done.b * a.heads + h] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+      const int64_t h = p.group * kHeads + static_cast<int64_t>(rank) * kCtaHeads + head;
+      if (part_of == 0 && h < a.heads) {
+        if (!p.whole) plan.part_ml[static_cast<int64_t>(p.slot) * kHeads + (h - p.group * kHeads)] = make_float2(m, sum);
+        else if (a.lse) a.lse[p.b * a.heads + h] = sum == 0.0f ? -INFINITY : (m + log2f(sum)) * kLn2;
       }
       tc_fence_before();
+      // (all four warps have left the staging before any writes probabilities: the next tile's exchange orders them)
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->o_read);
+      if (lane == 0) cluster_arrive(read_at);
     }
   }
   tc_fence_before();
   __syncthreads();
+  cluster_sync();  // nobody leaves while the other CTA may still signal or read here
   tc_fence_after();
-  if (warp == kAttnWarps - 1) tmem_dealloc(tmem, 512);
+  if (warp == kAttnWarps - 1) pair_tmem_dealloc(tmem, 512);
 }
 
 // Joins the parts of the rows that were cut, and writes the rows without
@@ -821,13 +786,12 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attention_join_kernel(Page
 
 AttnPlan attn_plan(Plan& p, int64_t batch, int64_t heads, int64_t latent, int64_t table_cols, int64_t page_size) {
   AttnPlan l{};
-  const int64_t halves = latent > 64 ? 2 : 1;
   l.groups = static_cast<int>(ceil_div(heads, kHeads));
   // at most one pair of CTAs per pair of SMs, and no more than there can be ranges
   const int64_t most = batch * l.groups * ceil_div(table_cols * page_size, kTile);
-  l.workers = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(gemv_grid_ctas() / halves, ceil_div(most, kMinTiles))));
+  l.workers = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(gemv_grid_ctas() / 2, ceil_div(most, kMinTiles))));
   l.run = 1;
-  while (l.run < kTile && page_size % (2 * l.run) == 0) l.run *= 2;
+  while (l.run < kHalfTile && page_size % (2 * l.run) == 0) l.run *= 2;
   l.part_o = p.take<float>(2 * l.workers * kHeads * latent);
   l.part_ml = p.take<float2>(2 * l.workers * kHeads);
   l.before = p.take<int64_t>(batch + 1);
@@ -854,17 +818,17 @@ bool encode_rows(CUtensorMap* map, const void* base, int64_t x, int64_t y, int64
 
 template <typename T>
 cudaError_t launch_attention(const PagedAttnArgs& a, const AttnPlan& plan, cudaStream_t stream) {
-  const bool tma = plan.run >= 8;
-  CUtensorMap cache{}, ql, qp;
-  if (!encode_rows<T>(&ql, a.q_latent, a.latent, a.heads, a.batch, a.ql_head_stride, a.ql_stride, kHeads) ||
-      !encode_rows<T>(&qp, a.q_pe, a.rope, a.heads, a.batch, a.qp_head_stride, a.qp_stride, kHeads) ||
-      (tma && !encode_rows<T>(&cache, a.cache, a.latent + a.rope, a.page_size, a.pages, a.row_stride, a.page_stride, plan.run)))
+  CUtensorMap runs, rows, ql, qp;
+  const int64_t width = a.latent + a.rope;
+  if (!encode_rows<T>(&ql, a.q_latent, a.latent, a.heads, a.batch, a.ql_head_stride, a.ql_stride, kCtaHeads) ||
+      !encode_rows<T>(&qp, a.q_pe, a.rope, a.heads, a.batch, a.qp_head_stride, a.qp_stride, kCtaHeads) ||
+      !encode_rows<T>(&runs, a.cache, width, a.page_size, a.pages, a.row_stride, a.page_stride, plan.run) ||
+      !encode_rows<T>(&rows, a.cache, width, a.page_size, a.pages, a.row_stride, a.page_stride, 1))
     return cudaErrorInvalidValue;
-  auto kernel = tma ? paged_attention_kernel<T, true> : paged_attention_kernel<T, false>;
+  auto kernel = paged_attention_kernel<T>;
   cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kAttnSmem));
   if (err != cudaSuccess) return err;
-  const unsigned ctas = static_cast<unsigned>(plan.workers * (a.latent > 64 ? 2 : 1));
-  kernel<<<ctas, kAttnThreads, kAttnSmem, stream>>>(cache, ql, qp, a, plan);
+  kernel<<<static_cast<unsigned>(2 * plan.workers), kAttnThreads, kAttnSmem, stream>>>(runs, rows, ql, qp, a, plan);
   err = cudaGetLastError();
   if (err != cudaSuccess) return err;
   paged_attention_join_kernel<T><<<static_cast<unsigned>(a.batch * ceil_div(a.heads, 2)), kJoinThreads, 0, stream>>>(a, plan);
