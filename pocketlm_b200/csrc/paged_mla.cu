@@ -176,12 +176,14 @@ cudaError_t launch_append_types(const AppendArgs& a, int x_dtype, int norm_dtype
 // and in lanes 64-127 with the second: a softmax thread holds 64 positions of
 // one head, and shares the head's maximum and sum with the thread 64 further.
 //
-// Shared memory: the queries (9 chunks of 64 heads x 64 columns, 8 KiB), two
-// buffers of probabilities (16-bit, 16 KiB each) and a ring of 16 KiB stages
-// that the cache's chunks (64 positions x 64 columns, 128B-swizzled) pass
-// through: for a tile, two chunks of K per stage, then V (the same rows again,
-// from L2, as an MN-major operand: own columns, all 128 positions).  Bytes bound
-// it: a position's 1152 bytes come from memory once per 128 heads.
+// Shared memory: the queries (9 chunks of 64 heads x 64 columns, 8 KiB), the
+// probabilities (16-bit, 16 KiB), and a buffer for each of a tile's five loads,
+// in chunks of 64 positions x 64 columns (128B-swizzled): K's columns 0-255,
+// 256-511 and rope (64 positions, half of the tile), V's own 256 columns of the
+// tile's first and second half (the same rows again, from L2, as an MN-major
+// operand).  Each is loaded again as soon as the products have read it, a whole
+// tile ahead of its next use.  Bytes bound it: a position's 1152 bytes come from
+// memory once per 128 heads.
 //
 // The softmax's reference maximum moves only when a tile's maximum exceeds it
 // by 2^8 (log2 domain): probabilities stay below 2^8 of the reference's 1, well
@@ -198,31 +200,36 @@ cudaError_t launch_append_types(const AppendArgs& a, int x_dtype, int norm_dtype
 // largest power of two, up to 64, that divides the page size).  Positions that
 // do not take part -- past the length, or on a page outside the cache -- arrive
 // as zeros, from coordinates outside the tensor, whatever their memory holds;
-// a run that the length cuts comes row by row.  Their scores are masked.
+// a run that the length cuts comes row by row.  Their scores are masked.  Runs
+// of 64 bring up to four chunks with one copy (a copy takes the issuing warp
+// about 50 cycles, and a tile has 17 chunks).
 //
-// Warps 0-3: softmax, result.  4: TMA.  5: tensor memory and, in the first CTA,
-// the products (the whole warp walks the work, so that operand descriptors stay
-// in uniform registers; one lane issues).
+// Warps 0-3: softmax, result.  4: copies of queries and K.  5: copies of V.  6:
+// tensor memory and, in the first CTA, the products (the whole warp walks the
+// work, so that operand descriptors stay in uniform registers; one lane issues).
 constexpr int kTile = 128, kHalfTile = 64;
 constexpr int kHeads = 128, kCtaHeads = 64;
 constexpr int kChunkBytes = 64 * 128;
 constexpr int kQChunks = 9;
-constexpr int kStages = 7, kStageBytes = 2 * kChunkBytes;
+constexpr int kBuffers = 5;  // K columns 0-255, 256-511, rope; V of the first and the second half of the tile
+constexpr int kBufferChunk[kBuffers] = {0, 4, 8, 9, 13};  // where each starts, in chunks
+constexpr int kBufferChunks = 17;
 constexpr int kPBytes = 2 * kChunkBytes;
 constexpr int kSoftmaxWarps = 4, kSoftmaxThreads = kSoftmaxWarps * kWarp;
-constexpr int kAttnWarps = kSoftmaxWarps + 2, kAttnThreads = kAttnWarps * kWarp;
+constexpr int kKeysWarp = 4, kValuesWarp = 5, kProductsWarp = 6;
+constexpr int kAttnWarps = 7, kAttnThreads = kAttnWarps * kWarp;
 constexpr uint32_t kColO = 0, kColS = 256;
 constexpr int kMinTiles = 1;  // fewest tiles worth a range of their own
 constexpr float kMovesBy = 8.0f;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct AttnBarriers {
-  uint64_t full[kStages];   // of the first CTA: both CTAs' bytes of a stage
-  uint64_t empty[kStages];  // in both
+  uint64_t full[kBuffers];   // of the first CTA: both CTAs' bytes of a buffer
+  uint64_t empty[kBuffers];  // in both
   uint64_t q_full;          // of the first CTA: both CTAs' queries of a part
   uint64_t s_full[2];       // scores complete
-  uint64_t p_ready[2];      // of the first CTA: probabilities written (one arrival per softmax warp of both)
-  uint64_t pv_done[2];      // a tile's second product complete
+  uint64_t p_ready;         // of the first CTA: probabilities written (one arrival per softmax warp of both)
+  uint64_t pv_done;         // a tile's second product complete
   uint64_t o_read;          // of the first CTA: the part's result has been read
   uint64_t drain;
   uint32_t tmem_base;
@@ -231,8 +238,8 @@ struct AttnBarriers {
   long long sums[kAttnWarps];
   float share[2][kSoftmaxThreads];  // what the two threads of a head tell each other
 };
-constexpr size_t kAttnSmem = 1024 + static_cast<size_t>(kQChunks) * kChunkBytes + 2 * kPBytes +
-                             static_cast<size_t>(kStages) * kStageBytes + sizeof(AttnBarriers);
+constexpr size_t kAttnSmem = 1024 + static_cast<size_t>(kQChunks + kBufferChunks) * kChunkBytes + kPBytes +
+                             sizeof(AttnBarriers);
 static_assert(kAttnSmem <= 232448, "shared memory per block");
 
 struct AttnPlan {
@@ -241,6 +248,7 @@ struct AttnPlan {
   int64_t* before;     // [batch + 1]: tiles before each row
   int workers;         // pairs of CTAs
   int run;             // positions per TMA box
+  bool wide;           // boxes of four chunks: runs of 64, latent columns in whole chunks
   int groups;          // groups of 128 heads: an item is a row's group
 };
 
@@ -317,22 +325,22 @@ MOE_D bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
 
 template <typename T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttnThreads, 1)
-    paged_attention_kernel(const __grid_constant__ CUtensorMap map_runs, const __grid_constant__ CUtensorMap map_rows,
-                           const __grid_constant__ CUtensorMap map_ql, const __grid_constant__ CUtensorMap map_qp,
+    paged_attention_kernel(const __grid_constant__ CUtensorMap map_wide, const __grid_constant__ CUtensorMap map_runs,
+                           const __grid_constant__ CUtensorMap map_rows, const __grid_constant__ CUtensorMap map_ql, const __grid_constant__ CUtensorMap map_qp,
                            PagedAttnArgs a, AttnPlan plan) {
   extern __shared__ unsigned char smem_raw[];
   // the same place in both CTAs (their shared memory starts alike)
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   unsigned char* q_smem = smem;
   unsigned char* p_smem = q_smem + kQChunks * kChunkBytes;
-  unsigned char* ring = p_smem + 2 * kPBytes;
-  AttnBarriers* bars = reinterpret_cast<AttnBarriers*>(ring + kStages * kStageBytes);
+  unsigned char* buffers = p_smem + kPBytes;
+  AttnBarriers* bars = reinterpret_cast<AttnBarriers*>(buffers + kBufferChunks * kChunkBytes);
   const int tid = threadIdx.x, lane = tid % kWarp, warp = __shfl_sync(0xFFFFFFFFu, tid / kWarp, 0);
   volatile int* abort = &bars->abort;
   const int latent = static_cast<int>(a.latent), rope = static_cast<int>(a.rope);
   const int lat_chunks = (latent + 63) / 64, chunks = lat_chunks + 1;  // the last one holds the rope part
   const int own_chunks = (lat_chunks + 1) / 2;                         // latent chunks whose V each CTA brings
-  const int k_stages = (chunks + 1) / 2, v_pairs = (own_chunks + 1) / 2;
+  const int v_pairs = (own_chunks + 1) / 2;                            // .. two at a time: a product of N = 256
   const uint32_t rank = cluster_rank();
   const int worker = blockIdx.x / 2;
 
@@ -378,22 +386,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttnThreads, 1)
     bars->first_tile = static_cast<int>(start - at);
   }
   if (tid == 0) {
-    for (int s = 0; s < kStages; ++s) {
+    for (int s = 0; s < kBuffers; ++s) {
       mbar_init(&bars->full[s], 1);
       mbar_init(&bars->empty[s], 1);
     }
     mbar_init(&bars->q_full, 1);
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(&bars->s_full[s], 1);
-      mbar_init(&bars->p_ready[s], 2 * kSoftmaxWarps);
-      mbar_init(&bars->pv_done[s], 1);
-    }
+    mbar_init(&bars->s_full[0], 1);
+    mbar_init(&bars->s_full[1], 1);
+    mbar_init(&bars->p_ready, 2 * kSoftmaxWarps);
+    mbar_init(&bars->pv_done, 1);
     mbar_init(&bars->o_read, 2 * kSoftmaxWarps);
     mbar_init(&bars->drain, 1);
     bars->abort = 0;
     fence_barrier_init();
   }
-  if (warp == kAttnWarps - 1) pair_tmem_alloc(&bars->tmem_base, 512);
+  if (warp == kProductsWarp) pair_tmem_alloc(&bars->tmem_base, 512);
   tc_fence_before();
   __syncthreads();
   cluster_sync();
@@ -402,144 +409,145 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttnThreads, 1)
   Walk walk{bars->first_item, bars->first_tile, stop - start};
   Part p;
 
-  if (warp == kSoftmaxWarps) {
-    // --------------------------------------------------------------- TMA
-    const uint32_t ring_at = smem_addr(ring), q_at = smem_addr(q_smem);
+  if (warp == kKeysWarp || warp == kValuesWarp) {
+    // ------------------------------------------------------------ copies
+    const uint32_t buffers_at = smem_addr(buffers), q_at = smem_addr(q_smem), full_at = cluster_addr(&bars->full[0], 0);
     const int run = plan.run, runs = kHalfTile / run, page_size = static_cast<int>(a.page_size);
     const int outside = static_cast<int>(a.pages);  // a page that the cache does not have: zeros
-    const bool leader = elect_one();
-    uint32_t g = 0, it = 0, parts = 0;
+    const bool leader = elect_one(), wide = plan.wide;
+    uint32_t g = 0, parts = 0;
     bool ok = true;
-    // runs lane and lane + 32 of each half of a tile: page, row in it, positions that take part
-    struct Runs {
-      int page[2][2], row[2][2], live[2][2];
+    // Where 64 positions lie: run `lane` (and lane + 32, where there are 64 runs of one position), absent ones
+    // outside the cache, and the run that the length cuts (all lanes know it; `cut` positions of it take part).
+    struct Half {
+      int page, row, page2, row2;
+      bool mine;
+      int cut, cut_page, cut_row, cut_first;
     };
-    auto lookup = [&](int tile) {
-      Runs r;
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const int i = lane + k * kWarp, pos = tile * kTile + h * kHalfTile + i * run;
-          r.page[h][k] = outside;
-          r.row[h][k] = r.live[h][k] = 0;
-          if (i < runs && pos < p.len) {
-            const int col = pos / page_size, page = __ldg(a.table + p.b * a.table_stride + col);
-            if (page >= 0 && page < a.pages) {
-              r.page[h][k] = page;
-              r.row[h][k] = pos - col * page_size;
-              r.live[h][k] = min(run, p.len - pos);
-            }
+    auto lookup = [&](int pos0) {
+      Half r;
+      int live;
+      auto find = [&](int i, int& page, int& row) {
+        const int pos = pos0 + i * run;
+        page = outside;
+        row = live = 0;
+        if (i < runs && pos < p.len) {
+          const int col = pos / page_size, pg = __ldg(a.table + p.b * a.table_stride + col);
+          if (pg >= 0 && pg < a.pages) {
+            page = pg;
+            row = pos - col * page_size;
+            live = min(run, p.len - pos);
           }
         }
+      };
+      r.page2 = outside;
+      r.row2 = 0;
+      if (runs > kWarp) find(lane + kWarp, r.page2, r.row2);
+      find(lane, r.page, r.row);
+      const bool cut = live > 0 && live < run;
+      const uint32_t cuts = __ballot_sync(0xFFFFFFFFu, cut);  // at most one run of a row: its last
+      const int from = cuts ? __ffs(cuts) - 1 : 0;
+      r.mine = lane < runs && !cut;
+      r.cut = cuts ? __shfl_sync(0xFFFFFFFFu, live, from) : 0;
+      r.cut_page = __shfl_sync(0xFFFFFFFFu, r.page, from);
+      r.cut_row = __shfl_sync(0xFFFFFFFFu, r.row, from);
+      r.cut_first = from * run;
       return r;
     };
-    // 64 positions (half h) x 64 columns from x into dst
-    auto fetch = [&](const Runs& r, int h, int x, uint32_t dst, uint32_t bar) {
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const int i = lane + k * kWarp, live = r.live[h][k];
-        const bool cut = live > 0 && live < run;
-        if (i < runs && !cut) pair_tma_load_3d(dst + i * run * 128, &map_runs, x, r.row[h][k], r.page[h][k], bar);
-        uint32_t cuts = __ballot_sync(0xFFFFFFFFu, cut);  // at most one run of a row: its last
-        if (cuts) {
-          const int from = __ffs(cuts) - 1;
-          const int n = __shfl_sync(0xFFFFFFFFu, live, from), page = __shfl_sync(0xFFFFFFFFu, r.page[h][k], from);
-          const int row = __shfl_sync(0xFFFFFFFFu, r.row[h][k], from), first = (from + k * kWarp) * run;
+    // buffer i gets 64 positions of `n` chunks from the c-th on, in tile g: its memory is free, and the first CTA's
+    // barrier expects both CTAs' bytes
+    auto fill = [&](int i, int first_chunk, const Half& r, int c, int n) {
+      if (g >= 1 && !warp_wait(&bars->empty[i], (g - 1) & 1, abort)) return false;
+      if (rank == 0 && leader) mbar_arrive_expect_tx(&bars->full[i], 2 * n * kChunkBytes);
+      __syncwarp();
+      const uint32_t dst = buffers_at + first_chunk * kChunkBytes, bar = full_at + i * 8;
+      const bool rope_part = c == lat_chunks;
+      if (wide && !rope_part && n == 4 && !r.cut) {
+        if (lane == 0) pair_tma_load_4d(dst, &map_wide, 0, r.row, c, r.page, bar);  // its run is the only one
+        __syncwarp();
+        return true;
+      }
+      for (int k = 0; k < n; ++k) {
+        const int x = rope_part ? latent : (c + k) * 64;
+        const uint32_t to = dst + k * kChunkBytes;
+        if (r.mine) pair_tma_load_3d(to + lane * run * 128, &map_runs, x, r.row, r.page, bar);
+        if (runs > kWarp) pair_tma_load_3d(to + (lane + kWarp) * 128, &map_runs, x, r.row2, r.page2, bar);
+        if (r.cut)
           for (int j = lane; j < run; j += kWarp)
-            pair_tma_load_3d(dst + (first + j) * 128, &map_rows, x, row + j, j < n ? page : outside, bar);
-        }
-      }
-    };
-    // the next stage is free: its memory, and the first CTA's barrier armed with both CTAs' bytes
-    auto open = [&](int n_chunks, uint32_t& dst, uint32_t& bar) {
-      const uint32_t s = it % kStages;
-      if (it >= kStages && !warp_wait(&bars->empty[s], ((it / kStages) - 1) & 1, abort)) return false;
-      if (rank == 0 && leader) mbar_arrive_expect_tx(&bars->full[s], 2 * n_chunks * kChunkBytes);
-      __syncwarp();
-      dst = ring_at + s * kStageBytes;
-      bar = cluster_addr(&bars->full[s], 0);
-      ++it;
-      return true;
-    };
-    auto fetch_k = [&](const Runs& r) {
-      for (int u = 0; u < k_stages; ++u) {
-        const int n = min(2, chunks - 2 * u);
-        uint32_t dst, bar;
-        if (!open(n, dst, bar)) return false;
-        for (int c = 2 * u; c < 2 * u + n; ++c)
-          fetch(r, rank, c < lat_chunks ? c * 64 : latent, dst + (c - 2 * u) * kChunkBytes, bar);
-      }
-      return true;
-    };
-    auto fetch_v = [&](const Runs& r) {
-      for (int h = 0; h < 2; ++h)
-        for (int j = 0; j < v_pairs; ++j) {
-          uint32_t dst, bar;
-          if (!open(2, dst, bar)) return false;
-          const int c = static_cast<int>(rank) * own_chunks + 2 * j;
-          fetch(r, h, c * 64, dst, bar);
-          fetch(r, h, (c + 1) * 64, dst + kChunkBytes, bar);
-        }
-      return true;
-    };
-    while (ok && walk.next(a, plan.groups, worker, p)) {
-      Runs now = lookup(p.tile0);
-      if (parts > 0 && !(ok = warp_wait(&bars->s_full[(g - 1) % 2], ((g - 1) / 2) & 1, abort))) break;  // the queries' last use
-      if (leader) {
-        const uint32_t bar = cluster_addr(&bars->q_full, 0);
-        if (rank == 0) mbar_arrive_expect_tx(&bars->q_full, 2 * chunks * kChunkBytes);
-        for (int c = 0; c < chunks; ++c)
-          pair_tma_load_3d(q_at + c * kChunkBytes, c < lat_chunks ? &map_ql : &map_qp, c < lat_chunks ? c * 64 : 0,
-                           p.group * kHeads + static_cast<int>(rank) * kCtaHeads, static_cast<int>(p.b), bar);
+            pair_tma_load_3d(to + (r.cut_first + j) * 128, &map_rows, x, r.cut_row + j, j < r.cut ? r.cut_page : outside, bar);
       }
       __syncwarp();
-      ok = fetch_k(now);
-      for (int i = 0; i < p.tiles && ok; ++i, ++g) {
-        Runs next = now;
-        if (i + 1 < p.tiles) {
-          next = lookup(p.tile0 + i + 1);
-          ok = fetch_k(next);
+      return true;
+    };
+    if (warp == kKeysWarp) {
+      const int half = static_cast<int>(rank) * kHalfTile, k0 = min(4, lat_chunks);
+      while (ok && walk.next(a, plan.groups, worker, p)) {
+        Half now = lookup(p.tile0 * kTile + half);
+        if (parts > 0 && !(ok = warp_wait(&bars->s_full[(g - 1) % 2], ((g - 1) / 2) & 1, abort))) break;  // the queries' last use
+        if (leader) {
+          const uint32_t bar = cluster_addr(&bars->q_full, 0);
+          if (rank == 0) mbar_arrive_expect_tx(&bars->q_full, 2 * chunks * kChunkBytes);
+          for (int c = 0; c < chunks; ++c)
+            pair_tma_load_3d(q_at + c * kChunkBytes, c < lat_chunks ? &map_ql : &map_qp, c < lat_chunks ? c * 64 : 0,
+                             p.group * kHeads + static_cast<int>(rank) * kCtaHeads, static_cast<int>(p.b), bar);
         }
-        ok = ok && fetch_v(now);
-        now = next;
+        __syncwarp();
+        for (int i = 0; i < p.tiles && ok; ++i, ++g) {
+          ok = fill(0, 0, now, 0, k0) && (lat_chunks <= 4 || fill(1, 4, now, 4, lat_chunks - 4)) && fill(2, 8, now, lat_chunks, 1);
+          if (i + 1 < p.tiles) now = lookup((p.tile0 + i + 1) * kTile + half);
+        }
+        ++parts;
       }
-      ++parts;
+    } else {
+      const int c = static_cast<int>(rank) * own_chunks;
+      while (ok && walk.next(a, plan.groups, worker, p)) {
+        Half first = lookup(p.tile0 * kTile), second = lookup(p.tile0 * kTile + kHalfTile);
+        for (int i = 0; i < p.tiles && ok; ++i, ++g) {
+          ok = fill(3, 9, first, c, own_chunks) && fill(4, 13, second, c, own_chunks);
+          if (i + 1 < p.tiles) {
+            first = lookup((p.tile0 + i + 1) * kTile);
+            second = lookup((p.tile0 + i + 1) * kTile + kHalfTile);
+          }
+        }
+      }
     }
     // the copies issued land before either CTA leaves: the first one's barriers count them all, and what
     // the products have consumed had landed
-    for (uint32_t j = it > kStages ? it - kStages : 0; j < it; ++j)
-      mbar_wait(rank == 0 ? &bars->full[j % kStages] : &bars->empty[j % kStages], (j / kStages) & 1, kPagedWaitError);
-  } else if (warp == kAttnWarps - 1) {
+    if (g > 0)
+      for (int i = warp == kKeysWarp ? 0 : 3; i < (warp == kKeysWarp ? 3 : 5); ++i)
+        if (i != 1 || lat_chunks > 4)
+          mbar_wait(rank == 0 ? &bars->full[i] : &bars->empty[i], (g - 1) & 1, kPagedWaitError);
+  } else if (warp == kProductsWarp) {
     // ---------------------------------------------------------- products
     if (rank == 0) {
       const bool leader = elect_one();
       const int format = __is_same(T, __nv_bfloat16) ? 1 : 0;
       const uint32_t idesc_s = umma_idesc(kHeads, kTile, format, false), idesc_o = umma_idesc(kHeads, 256, format, true);
       const uint64_t q_desc = sw128_desc_k(smem_addr(q_smem)), p_desc = sw128_desc_k(smem_addr(p_smem));
-      const uint64_t k_desc = sw128_desc_k(smem_addr(ring)), v_desc = sw128_desc(smem_addr(ring), kChunkBytes);
-      uint32_t g = 0, it = 0, parts = 0;
+      const uint64_t k_desc = sw128_desc_k(smem_addr(buffers));
+      const uint64_t v_desc = sw128_desc(smem_addr(buffers) + kBufferChunk[3] * kChunkBytes, kChunkBytes);
+      constexpr int kStep = kChunkBytes / 16;  // descriptors advance in units of 16 bytes
+      uint32_t g = 0, parts = 0;
       bool ok = true;
-      // descriptors advance in units of 16 bytes
+      // the scores of the tile whose number is t
       auto scores = [&](uint32_t t) {
         const uint32_t d = tmem + kColS + (t % 2) * (kTile / 2);
-        for (int u = 0; u < k_stages; ++u, ++it) {
-          const uint32_t s = it % kStages;
-          if (!warp_wait(&bars->full[s], (it / kStages) & 1, abort)) return false;
+        for (int i = 0; i < 3; ++i) {
+          if (i == 1 && lat_chunks <= 4) continue;
+          const int c0 = i == 2 ? lat_chunks : 4 * i, n = i == 2 ? 1 : min(4, lat_chunks - c0);
+          if (!warp_wait(&bars->full[i], t & 1, abort)) return false;
           tc_fence_after();
           if (leader) {
-            const int n = min(2, chunks - 2 * u);
             for (int c = 0; c < n; ++c) {
-              const uint64_t q = q_desc + (2 * u + c) * (kChunkBytes / 16), k = k_desc + s * (kStageBytes / 16) + c * (kChunkBytes / 16);
+              const uint64_t q = q_desc + (c0 + c) * kStep, k = k_desc + (kBufferChunk[0] + 4 * i + c) * kStep;
 #pragma unroll
-              for (int i = 0; i < 4; ++i) pair_umma_f16_ss(d, q + 2 * i, k + 2 * i, idesc_s, u > 0 || c > 0 || i > 0);
+              for (int j = 0; j < 4; ++j) pair_umma_f16_ss(d, q + 2 * j, k + 2 * j, idesc_s, i > 0 || c > 0 || j > 0);
             }
-            pair_umma_commit(&bars->empty[s]);
+            pair_umma_commit(&bars->empty[i]);
+            if (i == 2) pair_umma_commit(&bars->s_full[t % 2]);
           }
           __syncwarp();
         }
-        if (leader) pair_umma_commit(&bars->s_full[t % 2]);
-        __syncwarp();
         return true;
       };
       while (ok && walk.next(a, plan.groups, worker, p)) {
@@ -548,24 +556,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttnThreads, 1)
         ok = scores(g);
         for (int i = 0; i < tiles && ok; ++i, ++g) {
           if (i + 1 < tiles && !(ok = scores(g + 1))) break;
-          if (!(ok = warp_wait(&bars->p_ready[g % 2], (g / 2) & 1, abort))) break;
+          if (!(ok = warp_wait(&bars->p_ready, g & 1, abort))) break;
           if (i == 0 && parts > 0 && !(ok = warp_wait(&bars->o_read, (parts - 1) & 1, abort))) break;
-          for (int h = 0; h < 2 && ok; ++h)
-            for (int j = 0; j < v_pairs; ++j, ++it) {
-              const uint32_t s = it % kStages;
-              if (!(ok = warp_wait(&bars->full[s], (it / kStages) & 1, abort))) break;
-              tc_fence_after();
-              if (leader) {
-                const uint64_t pd = p_desc + (g % 2) * (kPBytes / 16) + h * (kChunkBytes / 16), v = v_desc + s * (kStageBytes / 16);
+          for (int h = 0; h < 2; ++h) {
+            if (!(ok = warp_wait(&bars->full[3 + h], g & 1, abort))) break;
+            tc_fence_after();
+            if (leader) {
+              for (int j = 0; j < v_pairs; ++j) {
+                const uint64_t pd = p_desc + h * kStep, v = v_desc + (4 * h + 2 * j) * kStep;
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
                   pair_umma_f16_ss(tmem + kColO + j * 128, pd + 2 * k, v + k * (2048 / 16), idesc_o, i > 0 || h > 0 || k > 0);
-                pair_umma_commit(&bars->empty[s]);
               }
-              __syncwarp();
+              pair_umma_commit(&bars->empty[3 + h]);
+              if (h == 1) pair_umma_commit(&bars->pv_done);
             }
-          if (leader) pair_umma_commit(&bars->pv_done[g % 2]);
-          __syncwarp();
+            __syncwarp();
+          }
         }
         ++parts;
       }
@@ -579,7 +586,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttnThreads, 1)
     const uint32_t my_lanes = static_cast<uint32_t>(warp * kWarp) << 16;
     const int page_size = static_cast<int>(a.page_size);
     const int head = tid % kCtaHeads, part_of = tid / kCtaHeads;  // the thread's head of the CTA, and half of N
-    const uint32_t ready_at[2] = {cluster_addr(&bars->p_ready[0], 0), cluster_addr(&bars->p_ready[1], 0)};
+    const uint32_t ready_at = cluster_addr(&bars->p_ready, 0);
     const uint32_t read_at = cluster_addr(&bars->o_read, 0);
     int turn = 0;
     // the value of this thread's head in the other half; `fine` becomes whether it is for all four warps, so
@@ -617,7 +624,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttnThreads, 1)
           live[k] = __ballot_sync(0xFFFFFFFFu, in);
         }
         bool got = ok && warp_wait(&bars->s_full[g % 2], (g / 2) & 1, abort);
-        if (got && g >= 2) got = warp_wait(&bars->pv_done[g % 2], ((g / 2) - 1) & 1, abort);  // the buffer of probabilities
         tc_fence_after();
         uint32_t r[kHalfTile];
         tmem_ld32(tmem + my_lanes + kColS + (g % 2) * kHalfTile, r);
@@ -648,7 +654,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttnThreads, 1)
             m = top;
           }
           if (i > 0) {
-            ok = warp_wait(&bars->pv_done[(g - 1) % 2], ((g - 1) / 2) & 1, abort);  // (a failure shows in the next wait of all)
+            ok = warp_wait(&bars->pv_done, (g - 1) & 1, abort);  // (a failure shows in the next wait of all)
             tc_fence_after();
             for (int c = 0; c < v_pairs * 128; c += 32) {
               uint32_t o[32];
@@ -672,45 +678,43 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttnThreads, 1)
           r[j / 2] = pack2<T>(p0, p1);
         }
         l += sum0 + sum1;
-        unsigned char* dst = p_smem + (g % 2) * kPBytes + part_of * kChunkBytes + head * 128;
+        if (g > 0) ok = warp_wait(&bars->pv_done, (g - 1) & 1, abort) && ok;  // the last probabilities have been read
+        unsigned char* dst = p_smem + part_of * kChunkBytes + head * 128;
 #pragma unroll
         for (int u = 0; u < 8; ++u)
           *reinterpret_cast<uint4*>(dst + ((u ^ (head % 8)) * 16)) = make_uint4(r[4 * u], r[4 * u + 1], r[4 * u + 2], r[4 * u + 3]);
         fence_proxy_async_shared();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) cluster_arrive(ready_at[g % 2]);
+        if (lane == 0) cluster_arrive(ready_at);
       }
-      ok = ok && warp_wait(&bars->pv_done[(g - 1) % 2], ((g - 1) / 2) & 1, abort);
+      ok = ok && warp_wait(&bars->pv_done, (g - 1) & 1, abort);
       const float sum = l + other(l, ok);
       if (!ok) break;
       tc_fence_after();
-      // through the probabilities' buffers, which nothing uses now: 64 columns of the warp's 32 heads at a time, so
-      // that sixteen lanes write a head's columns side by side
-      float* stage = reinterpret_cast<float*>(p_smem) + warp * (kWarp * 64);
+      // through the probabilities' buffer, which nothing uses now: 32 columns of the warp's 32 heads at a time, so
+      // that eight lanes write a head's columns side by side
+      float* stage = reinterpret_cast<float*>(p_smem) + warp * (kWarp * 32);
       const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
       const int64_t h0 = p.group * kHeads + static_cast<int64_t>(rank) * kCtaHeads + (warp % 2) * kWarp;  // the warp's first head
-      for (int c = 0; c < own_chunks; ++c) {  // chunk c of this half of N
-        const int col0 = (part_of * own_chunks + c) * 64;
+      for (int c = 0; c < 2 * own_chunks; ++c) {  // 32 columns c of this half of N
+        const int col0 = part_of * own_chunks * 64 + c * 32;
         if (col0 >= latent) break;
+        uint32_t o[32];
+        tmem_ld32(tmem + my_lanes + kColO + c * 32, o);
+        tmem_ld_wait();
 #pragma unroll
-        for (int k = 0; k < 64; k += 32) {
-          uint32_t o[32];
-          tmem_ld32(tmem + my_lanes + kColO + c * 64 + k, o);
-          tmem_ld_wait();
-#pragma unroll
-          for (int j = 0; j < 32; j += 4) {
-            float4 v = make_float4(__uint_as_float(o[j]), __uint_as_float(o[j + 1]), __uint_as_float(o[j + 2]), __uint_as_float(o[j + 3]));
-            if (p.whole) v = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
-            *reinterpret_cast<float4*>(stage + lane * 64 + (((k + j) / 4) ^ (lane % 8)) * 4) = v;
-          }
+        for (int j = 0; j < 32; j += 4) {
+          float4 v = make_float4(__uint_as_float(o[j]), __uint_as_float(o[j + 1]), __uint_as_float(o[j + 2]), __uint_as_float(o[j + 3]));
+          if (p.whole) v = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+          *reinterpret_cast<float4*>(stage + lane * 32 + ((j / 4) ^ (lane % 8)) * 4) = v;
         }
         __syncwarp();
-        const int unit = lane % 16, col = col0 + unit * 4;
-#pragma unroll 4
-        for (int row = lane / 16; row < kWarp; row += 2) {
+        const int unit = lane % 8, col = col0 + unit * 4;
+#pragma unroll
+        for (int row = lane / 8; row < kWarp; row += 4) {
           const int64_t h = h0 + row;
-          const float4 v = *reinterpret_cast<const float4*>(stage + row * 64 + ((unit ^ (row % 8)) * 4));
+          const float4 v = *reinterpret_cast<const float4*>(stage + row * 32 + ((unit ^ (row % 8)) * 4));
           if (h >= a.heads || col >= latent) continue;
           if (p.whole)
             *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (p.b * a.heads + h) * latent + col) =
@@ -735,7 +739,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttnThreads, 1)
   __syncthreads();
   cluster_sync();  // nobody leaves while the other CTA may still signal or read here
   tc_fence_after();
-  if (warp == kAttnWarps - 1) pair_tmem_dealloc(tmem, 512);
+  if (warp == kProductsWarp) pair_tmem_dealloc(tmem, 512);
 }
 
 // Joins the parts of the rows that were cut, and writes the rows without
@@ -792,43 +796,48 @@ AttnPlan attn_plan(Plan& p, int64_t batch, int64_t heads, int64_t latent, int64_
   l.workers = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(gemv_grid_ctas() / 2, ceil_div(most, kMinTiles))));
   l.run = 1;
   while (l.run < kHalfTile && page_size % (2 * l.run) == 0) l.run *= 2;
+  l.wide = l.run == kHalfTile && latent % 64 == 0;
   l.part_o = p.take<float>(2 * l.workers * kHeads * latent);
   l.part_ml = p.take<float2>(2 * l.workers * kHeads);
   l.before = p.take<int64_t>(batch + 1);
   return l;
 }
 
-// A tensor [z][y][x] of 16-bit values with a box of 64 columns and `rows` rows, 128B-swizzled.
+// A tensor [z][y][x] of 16-bit values with a box of 64 columns and `rows` rows, 128B-swizzled; or, with
+// `chunks`, its first 64 chunks columns as [z][chunk][y][64] and a box of 64 columns, `rows` rows and 4 chunks.
 template <typename T>
 bool encode_rows(CUtensorMap* map, const void* base, int64_t x, int64_t y, int64_t z, int64_t y_stride, int64_t z_stride,
-                 int rows) {
+                 int rows, int64_t chunks = 0) {
   const auto encode = tensor_map_encoder();
   if (!encode) return false;
   // a dimension of one has no stride of its own, but the map wants one
   if (y == 1) y_stride = 64;
   if (z == 1) z_stride = 64;
-  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(x), static_cast<cuuint64_t>(y), static_cast<cuuint64_t>(z)};
-  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(y_stride) * 2, static_cast<cuuint64_t>(z_stride) * 2};
-  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(rows), 1}, steps[3] = {1, 1, 1};
-  return encode(map, __is_same(T, __nv_bfloat16) ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
-                const_cast<void*>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  auto u = [](int64_t v) { return static_cast<cuuint64_t>(v); };
+  const bool wide = chunks > 0;
+  const cuuint64_t dims[4] = {u(wide ? 64 : x), u(y), u(wide ? chunks : z), u(z)};
+  const cuuint64_t strides[3] = {u(y_stride * 2), u(wide ? 128 : z_stride * 2), u(z_stride * 2)};
+  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(rows), wide ? 4u : 1u, 1}, steps[4] = {1, 1, 1, 1};
+  return encode(map, __is_same(T, __nv_bfloat16) ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                wide ? 4 : 3, const_cast<void*>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
                 CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <typename T>
 cudaError_t launch_attention(const PagedAttnArgs& a, const AttnPlan& plan, cudaStream_t stream) {
-  CUtensorMap runs, rows, ql, qp;
+  CUtensorMap wide{}, runs, rows, ql, qp;
   const int64_t width = a.latent + a.rope;
   if (!encode_rows<T>(&ql, a.q_latent, a.latent, a.heads, a.batch, a.ql_head_stride, a.ql_stride, kCtaHeads) ||
       !encode_rows<T>(&qp, a.q_pe, a.rope, a.heads, a.batch, a.qp_head_stride, a.qp_stride, kCtaHeads) ||
       !encode_rows<T>(&runs, a.cache, width, a.page_size, a.pages, a.row_stride, a.page_stride, plan.run) ||
-      !encode_rows<T>(&rows, a.cache, width, a.page_size, a.pages, a.row_stride, a.page_stride, 1))
+      !encode_rows<T>(&rows, a.cache, width, a.page_size, a.pages, a.row_stride, a.page_stride, 1) ||
+      (plan.wide && !encode_rows<T>(&wide, a.cache, width, a.page_size, a.pages, a.row_stride, a.page_stride, kHalfTile, a.latent / 64)))
     return cudaErrorInvalidValue;
   auto kernel = paged_attention_kernel<T>;
   cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kAttnSmem));
   if (err != cudaSuccess) return err;
-  kernel<<<static_cast<unsigned>(2 * plan.workers), kAttnThreads, kAttnSmem, stream>>>(runs, rows, ql, qp, a, plan);
+  kernel<<<static_cast<unsigned>(2 * plan.workers), kAttnThreads, kAttnSmem, stream>>>(wide, runs, rows, ql, qp, a, plan);
   err = cudaGetLastError();
   if (err != cudaSuccess) return err;
   paged_attention_join_kernel<T><<<static_cast<unsigned>(a.batch * ceil_div(a.heads, 2)), kJoinThreads, 0, stream>>>(a, plan);

@@ -151,6 +151,14 @@ MOE_D void pair_tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, 
       : "memory");
 }
 
+MOE_D void pair_tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, "
+      "%5}], [%6];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+      : "memory");
+}
+
 // One lane of a converged warp, the same one every time.
 MOE_D bool elect_one() {
   uint32_t is;
