@@ -197,12 +197,14 @@ cudaError_t launch_append_types(const AppendArgs& a, int x_dtype, int norm_dtype
 // the workspace, which the second kernel joins.  A range has at most two parts.
 //
 // Rows arrive by TMA, one box per run of positions that no page border cuts (the
-// largest power of two, up to 64, that divides the page size).  Positions that
-// do not take part -- past the length, or on a page outside the cache -- arrive
-// as zeros, from coordinates outside the tensor, whatever their memory holds;
-// a run that the length cuts comes row by row.  Their scores are masked.  Runs
-// of 64 bring up to four chunks with one copy (a copy takes the issuing warp
-// about 50 cycles, and a tile has 17 chunks).
+// largest power of two, up to 64, that divides the page size); runs of 64 bring
+// four chunks with one copy.  The scores of positions that do not take part are
+// masked; their rows of V must not hold a NaN all the same.  Runs without a
+// position, or on a page outside the cache, arrive as zeros, from coordinates
+// outside the tensor; the rows of a run behind the length that cuts it (whatever
+// their memory holds) are cleared in shared memory before the products may read.
+// K is asked into L2 two tiles ahead: a buffer's reload would otherwise show
+// memory's latency in every tile.
 //
 // Warps 0-3: softmax, result.  4: copies of queries and K.  5: copies of V.  6:
 // tensor memory and, in the first CTA, the products (the whole warp walks the
@@ -224,13 +226,14 @@ constexpr float kMovesBy = 8.0f;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct AttnBarriers {
-  uint64_t full[kBuffers];   // of the first CTA: both CTAs' bytes of a buffer
+  uint64_t full[kBuffers];   // of the first CTA: both CTAs' copies of a buffer have been issued, and their bytes
   uint64_t empty[kBuffers];  // in both
   uint64_t q_full;          // of the first CTA: both CTAs' queries of a part
   uint64_t s_full[2];       // scores complete
   uint64_t p_ready;         // of the first CTA: probabilities written (one arrival per softmax warp of both)
   uint64_t pv_done;         // a tile's second product complete
   uint64_t o_read;          // of the first CTA: the part's result has been read
+  uint64_t cut;             // the bytes of a half of V that the length cuts
   uint64_t drain;
   uint32_t tmem_base;
   int abort;
@@ -298,6 +301,7 @@ struct Walk {
   }
 };
 
+MOE_D void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 MOE_D float exp2_fast(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -326,7 +330,7 @@ MOE_D bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
 template <typename T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttnThreads, 1)
     paged_attention_kernel(const __grid_constant__ CUtensorMap map_wide, const __grid_constant__ CUtensorMap map_runs,
-                           const __grid_constant__ CUtensorMap map_rows, const __grid_constant__ CUtensorMap map_ql, const __grid_constant__ CUtensorMap map_qp,
+                           const __grid_constant__ CUtensorMap map_ql, const __grid_constant__ CUtensorMap map_qp,
                            PagedAttnArgs a, AttnPlan plan) {
   extern __shared__ unsigned char smem_raw[];
   // the same place in both CTAs (their shared memory starts alike)
@@ -387,9 +391,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttnThreads, 1)
   }
   if (tid == 0) {
     for (int s = 0; s < kBuffers; ++s) {
-      mbar_init(&bars->full[s], 1);
+      mbar_init(&bars->full[s], 2);
       mbar_init(&bars->empty[s], 1);
     }
+    mbar_init(&bars->cut, 1);
     mbar_init(&bars->q_full, 1);
     mbar_init(&bars->s_full[0], 1);
     mbar_init(&bars->s_full[1], 1);
@@ -418,25 +423,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttnThreads, 1)
     uint32_t g = 0, parts = 0;
     bool ok = true;
     // Where 64 positions lie: run `lane` (and lane + 32, where there are 64 runs of one position), absent ones
-    // outside the cache, and the run that the length cuts (all lanes know it; `cut` positions of it take part).
+    // outside the cache; the run that the length cuts is whole here, and positions from `dead` on do not take part.
     struct Half {
-      int page, row, page2, row2;
-      bool mine;
-      int cut, cut_page, cut_row, cut_first;
+      int page, row, page2, row2, dead;
     };
     auto lookup = [&](int pos0) {
       Half r;
-      int live;
       auto find = [&](int i, int& page, int& row) {
         const int pos = pos0 + i * run;
         page = outside;
-        row = live = 0;
+        row = 0;
         if (i < runs && pos < p.len) {
           const int col = pos / page_size, pg = __ldg(a.table + p.b * a.table_stride + col);
           if (pg >= 0 && pg < a.pages) {
             page = pg;
             row = pos - col * page_size;
-            live = min(run, p.len - pos);
           }
         }
       };
@@ -444,45 +445,70 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttnThreads, 1)
       r.row2 = 0;
       if (runs > kWarp) find(lane + kWarp, r.page2, r.row2);
       find(lane, r.page, r.row);
-      const bool cut = live > 0 && live < run;
-      const uint32_t cuts = __ballot_sync(0xFFFFFFFFu, cut);  // at most one run of a row: its last
-      const int from = cuts ? __ffs(cuts) - 1 : 0;
-      r.mine = lane < runs && !cut;
-      r.cut = cuts ? __shfl_sync(0xFFFFFFFFu, live, from) : 0;
-      r.cut_page = __shfl_sync(0xFFFFFFFFu, r.page, from);
-      r.cut_row = __shfl_sync(0xFFFFFFFFu, r.row, from);
-      r.cut_first = from * run;
+      r.dead = max(0, p.len - pos0);
       return r;
     };
-    // buffer i gets 64 positions of `n` chunks from the c-th on, in tile g: its memory is free, and the first CTA's
-    // barrier expects both CTAs' bytes
+    // 64 positions of `n` chunks from the c-th on into dst
+    auto copy = [&](uint32_t dst, const Half& r, int c, int n, uint32_t bar) {
+      if (wide && n == 4) {
+        if (lane == 0) pair_tma_load_4d(dst, &map_wide, 0, r.row, c, r.page, bar);  // its run is the only one
+        return;
+      }
+      for (int k = 0; k < n; ++k) {
+        const int x = c == lat_chunks ? latent : (c + k) * 64;
+        const uint32_t to = dst + k * kChunkBytes;
+        if (lane < runs) pair_tma_load_3d(to + lane * run * 128, &map_runs, x, r.row, r.page, bar);
+        if (runs > kWarp) pair_tma_load_3d(to + (lane + kWarp) * 128, &map_runs, x, r.row2, r.page2, bar);
+      }
+    };
+    uint32_t cuts = 0;
+    // buffer i (chunks from first_chunk on) gets chunks c .. c + n - 1 of 64 positions, in tile g, once its memory is
+    // free; each CTA tells the first one's barrier, which expects both CTAs' bytes
     auto fill = [&](int i, int first_chunk, const Half& r, int c, int n) {
       if (g >= 1 && !warp_wait(&bars->empty[i], (g - 1) & 1, abort)) return false;
-      if (rank == 0 && leader) mbar_arrive_expect_tx(&bars->full[i], 2 * n * kChunkBytes);
-      __syncwarp();
       const uint32_t dst = buffers_at + first_chunk * kChunkBytes, bar = full_at + i * 8;
-      const bool rope_part = c == lat_chunks;
-      if (wide && !rope_part && n == 4 && !r.cut) {
-        if (lane == 0) pair_tma_load_4d(dst, &map_wide, 0, r.row, c, r.page, bar);  // its run is the only one
+      const uint32_t bytes = static_cast<uint32_t>(n) * kChunkBytes;
+      const bool clear = i >= 3 && r.dead > 0 && r.dead % run != 0 && r.dead < kHalfTile;
+      if (!clear) {
+        // (each CTA adds its own bytes: a remote arrival may come before or after the bytes that it announces)
+        if (leader) cluster_arrive_expect_tx(bar, bytes);
+        __syncwarp();
+        copy(dst, r, c, n, bar);
         __syncwarp();
         return true;
       }
-      for (int k = 0; k < n; ++k) {
-        const int x = rope_part ? latent : (c + k) * 64;
-        const uint32_t to = dst + k * kChunkBytes;
-        if (r.mine) pair_tma_load_3d(to + lane * run * 128, &map_runs, x, r.row, r.page, bar);
-        if (runs > kWarp) pair_tma_load_3d(to + (lane + kWarp) * 128, &map_runs, x, r.row2, r.page2, bar);
-        if (r.cut)
-          for (int j = lane; j < run; j += kWarp)
-            pair_tma_load_3d(to + (r.cut_first + j) * 128, &map_rows, x, r.cut_row + j, j < r.cut ? r.cut_page : outside, bar);
-      }
+      const uint32_t mine = cluster_addr(&bars->cut, rank);
+      if (leader) mbar_arrive_expect_tx(&bars->cut, bytes);
+      __syncwarp();
+      copy(dst, r, c, n, mine);
+      __syncwarp();
+      if (!warp_wait(&bars->cut, cuts & 1, abort)) return false;
+      ++cuts;
+      unsigned char* at = buffers + first_chunk * kChunkBytes;
+      for (int row = r.dead + lane / 8; row < (r.dead + run - 1) / run * run; row += 4)
+        for (int k = 0; k < n; ++k) *reinterpret_cast<uint4*>(at + k * kChunkBytes + row * 128 + (lane % 8) * 16) = make_uint4(0, 0, 0, 0);
+      fence_proxy_async_shared();
+      __syncwarp();
+      if (leader) cluster_arrive(bar);
       __syncwarp();
       return true;
+    };
+    // ask 64 positions into L2, a line at a time (by the load unit: one bulk prefetch would queue in front of the copies)
+    const int lines = static_cast<int>(ceil_div((a.latent + a.rope) * static_cast<int64_t>(sizeof(T)), 128));
+    auto prefetch = [&](const Half& r) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int i = lane + k * kWarp, from = i / run;
+        const int page = runs > kWarp ? (k ? r.page2 : r.page) : __shfl_sync(0xFFFFFFFFu, r.page, from);
+        const int row = runs > kWarp ? (k ? r.row2 : r.row) : __shfl_sync(0xFFFFFFFFu, r.row, from) + i % run;
+        if (page == outside || i >= r.dead) continue;
+        const char* at = reinterpret_cast<const char*>(static_cast<const T*>(a.cache) + page * a.page_stride + row * a.row_stride);
+        for (int l = 0; l < lines; ++l) prefetch_l2(at + l * 128);
+      }
     };
     if (warp == kKeysWarp) {
       const int half = static_cast<int>(rank) * kHalfTile, k0 = min(4, lat_chunks);
       while (ok && walk.next(a, plan.groups, worker, p)) {
-        Half now = lookup(p.tile0 * kTile + half);
         if (parts > 0 && !(ok = warp_wait(&bars->s_full[(g - 1) % 2], ((g - 1) / 2) & 1, abort))) break;  // the queries' last use
         if (leader) {
           const uint32_t bar = cluster_addr(&bars->q_full, 0);
@@ -492,9 +518,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttnThreads, 1)
                              p.group * kHeads + static_cast<int>(rank) * kCtaHeads, static_cast<int>(p.b), bar);
         }
         __syncwarp();
+        auto at = [&](int i) { return lookup((p.tile0 + i) * kTile + half); };  // (past the part: rows are there, or nothing)
+        Half now = at(0), next = at(1);
         for (int i = 0; i < p.tiles && ok; ++i, ++g) {
           ok = fill(0, 0, now, 0, k0) && (lat_chunks <= 4 || fill(1, 4, now, 4, lat_chunks - 4)) && fill(2, 8, now, lat_chunks, 1);
-          if (i + 1 < p.tiles) now = lookup((p.tile0 + i + 1) * kTile + half);
+          now = next;
+          next = at(i + 2);
         }
         ++parts;
       }
@@ -696,7 +725,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttnThreads, 1)
       // that eight lanes write a head's columns side by side
       float* stage = reinterpret_cast<float*>(p_smem) + warp * (kWarp * 32);
       const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-      const int64_t h0 = p.group * kHeads + static_cast<int64_t>(rank) * kCtaHeads + (warp % 2) * kWarp;  // the warp's first head
+      const int first_row = static_cast<int>(rank) * kCtaHeads + (warp % 2) * kWarp + lane / 8;  // of the group's 128 heads
+      const int rows = static_cast<int>(min(a.heads - p.group * kHeads, static_cast<int64_t>(kHeads)));
+      const int unit = lane % 8;
+      T* out = static_cast<T*>(a.out) + (p.b * a.heads + p.group * kHeads + first_row) * latent + unit * 4;
+      float* part = plan.part_o + (static_cast<int64_t>(p.slot) * kHeads + first_row) * latent + unit * 4;
+      const float scale = p.whole ? inv : 1.0f;
       for (int c = 0; c < 2 * own_chunks; ++c) {  // 32 columns c of this half of N
         const int col0 = part_of * own_chunks * 64 + c * 32;
         if (col0 >= latent) break;
@@ -704,26 +738,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttnThreads, 1)
         tmem_ld32(tmem + my_lanes + kColO + c * 32, o);
         tmem_ld_wait();
 #pragma unroll
-        for (int j = 0; j < 32; j += 4) {
-          float4 v = make_float4(__uint_as_float(o[j]), __uint_as_float(o[j + 1]), __uint_as_float(o[j + 2]), __uint_as_float(o[j + 3]));
-          if (p.whole) v = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
-          *reinterpret_cast<float4*>(stage + lane * 32 + ((j / 4) ^ (lane % 8)) * 4) = v;
-        }
+        for (int j = 0; j < 32; j += 4)
+          *reinterpret_cast<float4*>(stage + lane * 32 + ((j / 4) ^ (lane % 8)) * 4) =
+              make_float4(__uint_as_float(o[j]) * scale, __uint_as_float(o[j + 1]) * scale, __uint_as_float(o[j + 2]) * scale,
+                          __uint_as_float(o[j + 3]) * scale);
         __syncwarp();
-        const int unit = lane % 8, col = col0 + unit * 4;
+        float4 v[8];
 #pragma unroll
-        for (int row = lane / 8; row < kWarp; row += 4) {
-          const int64_t h = h0 + row;
-          const float4 v = *reinterpret_cast<const float4*>(stage + row * 32 + ((unit ^ (row % 8)) * 4));
-          if (h >= a.heads || col >= latent) continue;
-          if (p.whole)
-            *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (p.b * a.heads + h) * latent + col) =
-                make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w));
-          else
-            *reinterpret_cast<float4*>(plan.part_o + (static_cast<int64_t>(p.slot) * kHeads + (h - p.group * kHeads)) * latent + col) = v;
+        for (int i = 0; i < 8; ++i) {
+          const int row = lane / 8 + 4 * i;
+          v[i] = *reinterpret_cast<const float4*>(stage + row * 32 + ((unit ^ (row % 8)) * 4));
         }
         __syncwarp();
+        if (col0 + unit * 4 >= latent) continue;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (first_row + 4 * i >= rows) break;
+          if (p.whole) *reinterpret_cast<uint2*>(out + 4 * i * latent + col0) = make_uint2(pack2<T>(v[i].x, v[i].y), pack2<T>(v[i].z, v[i].w));
+          else *reinterpret_cast<float4*>(part + 4 * i * latent + col0) = v[i];
+        }
       }
+      __syncwarp();
       const int64_t h = p.group * kHeads + static_cast<int64_t>(rank) * kCtaHeads + head;
       if (part_of == 0 && h < a.heads) {
         if (!p.whole) plan.part_ml[static_cast<int64_t>(p.slot) * kHeads + (h - p.group * kHeads)] = make_float2(m, sum);
@@ -742,50 +777,99 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttnThreads, 1)
   if (warp == kProductsWarp) pair_tmem_dealloc(tmem, 512);
 }
 
+MOE_D void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // Joins the parts of the rows that were cut, and writes the rows without
-// positions.  A CTA takes two heads of a row; a thread four columns.
-constexpr int kJoinThreads = 256;
-template <typename T>
+// positions.  A CTA takes kJoinHeads heads of a row (of one group), a thread four
+// columns of each; the parts' weights first, all at once, then their columns
+// with eight loads in flight: eight heads' where there are many rows, each cut
+// into two or three parts, and eight parts of one head where there are few.
+constexpr int kJoinThreads = 128, kMostWorkers = 128;
+template <typename T, int kJoinHeads>
 __global__ void __launch_bounds__(kJoinThreads) paged_attention_join_kernel(PagedAttnArgs a, AttnPlan plan) {
-  const int64_t pairs = ceil_div(a.heads, 2);
-  const int64_t b = blockIdx.x / pairs, h = (blockIdx.x - b * pairs) * 2 + threadIdx.x / (kJoinThreads / 2);
-  if (h >= a.heads) return;
-  const int64_t c = 4 * (threadIdx.x % (kJoinThreads / 2));
+  __shared__ float weight[kJoinHeads][kMostWorkers], total_of[kJoinHeads], ref_of[kJoinHeads];
+  const int per_row = static_cast<int>(ceil_div(a.heads, kJoinHeads));
+  const int64_t b = blockIdx.x / per_row, h0 = static_cast<int64_t>(blockIdx.x - b * per_row) * kJoinHeads;
+  const int heads = static_cast<int>(min(a.heads - h0, static_cast<int64_t>(kJoinHeads)));
+  const int lane = threadIdx.x % kWarp, warp = threadIdx.x / kWarp, c = 4 * threadIdx.x;
   const bool in = c < a.latent;
-  const int64_t total = plan.before[a.batch], tiles = (plan.before[b + 1] - plan.before[b]) / plan.groups;
-  T* out = static_cast<T*>(a.out) + (b * a.heads + h) * a.latent + c;
-  if (tiles == 0) {
-    if (in) *reinterpret_cast<uint2*>(out) = make_uint2(0, 0);
-    if (a.lse && c == 0) a.lse[b * a.heads + h] = -INFINITY;
+  wait_for_previous_kernel();
+  const int64_t total = plan.before[a.batch], first = plan.before[b], next = plan.before[b + 1];
+  T* out = static_cast<T*>(a.out) + (b * a.heads + h0) * a.latent + c;
+  if (first == next) {
+    for (int h = 0; h < heads; ++h) {
+      if (in) *reinterpret_cast<uint2*>(out + h * a.latent) = make_uint2(0, 0);
+      if (a.lse && c == 0) a.lse[b * a.heads + h0 + h] = -INFINITY;
+    }
     return;
   }
-  const int64_t workers = used_workers(total, plan.workers), group = h / kHeads;
-  const int64_t t0 = plan.before[b] + group * tiles, t1 = t0 + tiles - 1;  // the item's first and last tile
-  const int64_t w0 = ((t0 + 1) * workers - 1) / total, w1 = ((t1 + 1) * workers - 1) / total;
+  const int64_t workers = used_workers(total, plan.workers), group = h0 / kHeads, tiles = (next - first) / plan.groups;
+  const int64_t t0 = first + group * tiles, t1 = t0 + tiles - 1;  // the item's first and last tile
+  const int w0 = static_cast<int>(((t0 + 1) * workers - 1) / total), w1 = static_cast<int>(((t1 + 1) * workers - 1) / total);
   if (w0 == w1) return;  // finished where it was computed
-  // the first part is its range's last (unless the range starts with the row), the others open theirs
-  auto at = [&](int64_t w) { return (2 * w + (w == w0 ? 1 : 0)) * kHeads + (h - group * kHeads); };
-  float top = -INFINITY;
-  for (int64_t w = w0; w <= w1; ++w) top = fmaxf(top, plan.part_ml[at(w)].x);
-  if (top == -INFINITY) top = 0.0f;
-  float sum = 0.0f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-  for (int64_t w = w0; w <= w1; ++w) {
-    const float2 ml = plan.part_ml[at(w)];
-    const float f = exp2_fast(ml.x - top);
-    sum = fmaf(ml.y, f, sum);
-    if (in) {
-      const float4 o = *reinterpret_cast<const float4*>(plan.part_o + at(w) * a.latent + c);
-      acc.x = fmaf(o.x, f, acc.x);
-      acc.y = fmaf(o.y, f, acc.y);
-      acc.z = fmaf(o.z, f, acc.z);
-      acc.w = fmaf(o.w, f, acc.w);
+  // the first part is its range's last, the others open theirs
+  const int64_t row0 = h0 - group * kHeads;
+  auto at = [&](int w) { return (2 * static_cast<int64_t>(w) + (w == w0 ? 1 : 0)) * kHeads + row0; };
+  for (int h = warp; h < heads; h += kJoinThreads / kWarp) {
+    float2 ml[kMostWorkers / kWarp];
+    float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kMostWorkers / kWarp; ++k) {
+      const int w = w0 + k * kWarp + lane;
+      ml[k] = w <= w1 ? plan.part_ml[at(w) + h] : make_float2(-INFINITY, 0.0f);
+      top = fmaxf(top, ml[k].x);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    const float ref = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+    for (int k = 0; k < kMostWorkers / kWarp; ++k) {
+      const float e = exp2_fast(ml[k].x - ref);
+      weight[h][k * kWarp + lane] = e;
+      sum += e * ml[k].y;
+    }
+    sum = warp_sum(sum);
+    if (lane == 0) {
+      total_of[h] = sum;
+      ref_of[h] = ref;
     }
   }
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  if (in) *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
-  if (a.lse && c == 0) a.lse[b * a.heads + h] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
+  __syncthreads();
+  float4 acc[kJoinHeads];
+#pragma unroll
+  for (int h = 0; h < kJoinHeads; ++h) acc[h] = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (in) {
+    constexpr int kAtOnce = 8 / kJoinHeads;  // parts
+    for (int w = w0; w <= w1; w += kAtOnce) {
+      float4 o[kAtOnce][kJoinHeads];
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k)
+#pragma unroll
+        for (int h = 0; h < kJoinHeads; ++h)
+          o[k][h] = h < heads && w + k <= w1 ? __ldcg(reinterpret_cast<const float4*>(plan.part_o + (at(w + k) + h) * a.latent + c))
+                                             : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k)
+#pragma unroll
+        for (int h = 0; h < kJoinHeads; ++h) {
+          if (h >= heads || w + k > w1) break;
+          const float e = weight[h][w + k - w0];
+          acc[h].x = fmaf(o[k][h].x, e, acc[h].x);
+          acc[h].y = fmaf(o[k][h].y, e, acc[h].y);
+          acc[h].z = fmaf(o[k][h].z, e, acc[h].z);
+          acc[h].w = fmaf(o[k][h].w, e, acc[h].w);
+        }
+    }
+#pragma unroll
+    for (int h = 0; h < kJoinHeads; ++h) {
+      if (h >= heads) break;
+      const float inv = total_of[h] == 0.0f ? 0.0f : 1.0f / total_of[h];
+      *reinterpret_cast<uint2*>(out + h * a.latent) = make_uint2(pack2<T>(acc[h].x * inv, acc[h].y * inv), pack2<T>(acc[h].z * inv, acc[h].w * inv));
+    }
+  }
+  if (a.lse && threadIdx.x < heads)
+    a.lse[b * a.heads + h0 + threadIdx.x] =
+        total_of[threadIdx.x] == 0.0f ? -INFINITY : (ref_of[threadIdx.x] + log2f(total_of[threadIdx.x])) * kLn2;
 }
 
 AttnPlan attn_plan(Plan& p, int64_t batch, int64_t heads, int64_t latent, int64_t table_cols, int64_t page_size) {
@@ -793,7 +877,7 @@ AttnPlan attn_plan(Plan& p, int64_t batch, int64_t heads, int64_t latent, int64_
   l.groups = static_cast<int>(ceil_div(heads, kHeads));
   // at most one pair of CTAs per pair of SMs, and no more than there can be ranges
   const int64_t most = batch * l.groups * ceil_div(table_cols * page_size, kTile);
-  l.workers = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(gemv_grid_ctas() / 2, ceil_div(most, kMinTiles))));
+  l.workers = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({gemv_grid_ctas() / 2, kMostWorkers, ceil_div(most, kMinTiles)})));
   l.run = 1;
   while (l.run < kHalfTile && page_size % (2 * l.run) == 0) l.run *= 2;
   l.wide = l.run == kHalfTile && latent % 64 == 0;
@@ -824,24 +908,40 @@ bool encode_rows(CUtensorMap* map, const void* base, int64_t x, int64_t y, int64
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// A kernel that may be set up while the one before it in the stream still runs (it waits for its end by
+// itself, wait_for_previous_kernel).
+template <typename K, typename... Args>
+cudaError_t launch_dependent(K kernel, unsigned grid, int threads, cudaStream_t stream, Args... args) {
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(grid);
+  config.blockDim = dim3(static_cast<unsigned>(threads));
+  config.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, kernel, args...);
+}
+
 template <typename T>
 cudaError_t launch_attention(const PagedAttnArgs& a, const AttnPlan& plan, cudaStream_t stream) {
-  CUtensorMap wide{}, runs, rows, ql, qp;
+  CUtensorMap wide{}, runs, ql, qp;
   const int64_t width = a.latent + a.rope;
   if (!encode_rows<T>(&ql, a.q_latent, a.latent, a.heads, a.batch, a.ql_head_stride, a.ql_stride, kCtaHeads) ||
       !encode_rows<T>(&qp, a.q_pe, a.rope, a.heads, a.batch, a.qp_head_stride, a.qp_stride, kCtaHeads) ||
       !encode_rows<T>(&runs, a.cache, width, a.page_size, a.pages, a.row_stride, a.page_stride, plan.run) ||
-      !encode_rows<T>(&rows, a.cache, width, a.page_size, a.pages, a.row_stride, a.page_stride, 1) ||
       (plan.wide && !encode_rows<T>(&wide, a.cache, width, a.page_size, a.pages, a.row_stride, a.page_stride, kHalfTile, a.latent / 64)))
     return cudaErrorInvalidValue;
   auto kernel = paged_attention_kernel<T>;
   cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kAttnSmem));
   if (err != cudaSuccess) return err;
-  kernel<<<static_cast<unsigned>(2 * plan.workers), kAttnThreads, kAttnSmem, stream>>>(wide, runs, rows, ql, qp, a, plan);
+  kernel<<<static_cast<unsigned>(2 * plan.workers), kAttnThreads, kAttnSmem, stream>>>(wide, runs, ql, qp, a, plan);
   err = cudaGetLastError();
   if (err != cudaSuccess) return err;
-  paged_attention_join_kernel<T><<<static_cast<unsigned>(a.batch * ceil_div(a.heads, 2)), kJoinThreads, 0, stream>>>(a, plan);
-  return cudaGetLastError();
+  if (a.batch * a.heads >= 16 * gemv_grid_ctas())
+    return launch_dependent(paged_attention_join_kernel<T, 8>, static_cast<unsigned>(a.batch * ceil_div(a.heads, 8)), kJoinThreads, stream, a, plan);
+  return launch_dependent(paged_attention_join_kernel<T, 1>, static_cast<unsigned>(a.batch * a.heads), kJoinThreads, stream, a, plan);
 }
 
 }  // namespace

@@ -101,7 +101,7 @@ static int attention_supported(int64_t batch, int64_t heads, int64_t latent, int
     return fail(kBadDims, "bad dimensions");
   if (latent > 512 || latent % 8 || rope > 64 || rope % 8)
     return fail(kUnsupported, "kv_lora_rank up to 512 and qk_rope_dim up to 64, multiples of 8");
-  if (batch > 65535 || heads > (1 << 16) || table_cols > INT32_MAX / page_size)
+  if (batch > 65535 || heads > (1 << 16) || batch * heads > INT32_MAX || table_cols > INT32_MAX / page_size)
     return fail(kUnsupported, "dimension too large");
   return kOk;
 }

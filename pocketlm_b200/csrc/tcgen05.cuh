@@ -132,8 +132,14 @@ MOE_D uint32_t cluster_addr(const void* p, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_addr(p)), "r"(rank));
   return at;
 }
+// (At the default scope: what these barriers hand over are this CTA's shared
+// memory, fenced towards the async proxy, and tensor memory; a release of
+// cluster scope would wait some 1300 cycles for everything else besides.)
 MOE_D void cluster_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+MOE_D void cluster_arrive_expect_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 // Loads into this CTA's memory that report to a barrier of either CTA of the pair (its cluster address).
 MOE_D void pair_tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
