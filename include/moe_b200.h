@@ -624,7 +624,7 @@ int moe_paged_mla_append(const void* kv_rows, int64_t kv_stride, int kv_dtype, c
  * the table is skipped and sets code 512 in moe_b200_device_error.
  * kv_lora_rank <= 512 and qk_rope_dim <= 64, both multiples of 8; rows of
  * queries and cache start on 16-byte boundaries, strides positive; batch <=
- * 65535.  workspace:
+ * 65535.  workspace (on a 32-byte boundary):
  * moe_paged_mla_attention_workspace_bytes (-1 for dimensions it rejects). */
 int64_t moe_paged_mla_attention_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_lora_rank,
                                                 int64_t qk_rope_dim, int64_t table_cols, int64_t page_size);

@@ -206,9 +206,10 @@ cudaError_t launch_append_types(const AppendArgs& a, int x_dtype, int norm_dtype
 // K is asked into L2 two tiles ahead: a buffer's reload would otherwise show
 // memory's latency in every tile.
 //
-// Warps 0-3: softmax, result.  4: copies of queries and K.  5: copies of V.  6:
-// tensor memory and, in the first CTA, the products (the whole warp walks the
-// work, so that operand descriptors stay in uniform registers; one lane issues).
+// Warps 0-3: softmax, result.  4: copies of queries and K.  5, 6: copies of V's
+// halves.  7: tensor memory and, in the first CTA, the products (the whole warp
+// walks the work, so that operand descriptors stay in uniform registers; one
+// lane issues).
 constexpr int kTile = 128, kHalfTile = 64;
 constexpr int kHeads = 128, kCtaHeads = 64;
 constexpr int kChunkBytes = 64 * 128;
@@ -218,8 +219,8 @@ constexpr int kBufferChunk[kBuffers] = {0, 4, 8, 9, 13};  // where each starts, 
 constexpr int kBufferChunks = 17;
 constexpr int kPBytes = 2 * kChunkBytes;
 constexpr int kSoftmaxWarps = 4, kSoftmaxThreads = kSoftmaxWarps * kWarp;
-constexpr int kKeysWarp = 4, kValuesWarp = 5, kProductsWarp = 6;
-constexpr int kAttnWarps = 7, kAttnThreads = kAttnWarps * kWarp;
+constexpr int kKeysWarp = 4, kValuesWarp = 5, kProductsWarp = 7;
+constexpr int kAttnWarps = 8, kAttnThreads = kAttnWarps * kWarp;
 constexpr uint32_t kColO = 0, kColS = 256;
 constexpr int kMinTiles = 1;  // fewest tiles worth a range of their own
 constexpr float kMovesBy = 8.0f;
@@ -233,7 +234,7 @@ struct AttnBarriers {
   uint64_t p_ready;         // of the first CTA: probabilities written (one arrival per softmax warp of both)
   uint64_t pv_done;         // a tile's second product complete
   uint64_t o_read;          // of the first CTA: the part's result has been read
-  uint64_t cut;             // the bytes of a half of V that the length cuts
+  uint64_t cut[2];          // the bytes of a half of V that the length cuts
   uint64_t drain;
   uint32_t tmem_base;
   int abort;
@@ -251,9 +252,12 @@ struct AttnPlan {
   int64_t* before;     // [batch + 1]: tiles before each row
   int workers;         // pairs of CTAs
   int run;             // positions per TMA box
+  int shift, page_size;  // log2 of the page size where it has one, else -1
   bool wide;           // boxes of four chunks: runs of 64, latent columns in whole chunks
   int groups;          // groups of 128 heads: an item is a row's group
 };
+
+MOE_D int page_of(const AttnPlan& plan, int pos) { return plan.shift >= 0 ? pos >> plan.shift : pos / plan.page_size; }
 
 MOE_HD int64_t range_start(int64_t w, int64_t total, int64_t workers) { return w * total / workers; }
 MOE_D int64_t used_workers(int64_t total, int64_t workers) {
@@ -301,7 +305,12 @@ struct Walk {
   }
 };
 
-MOE_D void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+// 32 bytes, 32-byte aligned.
+MOE_D void store_sector(void* p, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+               "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
 MOE_D float exp2_fast(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -394,7 +403,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttnThreads, 1)
       mbar_init(&bars->full[s], 2);
       mbar_init(&bars->empty[s], 1);
     }
-    mbar_init(&bars->cut, 1);
+    mbar_init(&bars->cut[0], 1);
+    mbar_init(&bars->cut[1], 1);
     mbar_init(&bars->q_full, 1);
     mbar_init(&bars->s_full[0], 1);
     mbar_init(&bars->s_full[1], 1);
@@ -414,51 +424,49 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttnThreads, 1)
   Walk walk{bars->first_item, bars->first_tile, stop - start};
   Part p;
 
-  if (warp == kKeysWarp || warp == kValuesWarp) {
+  if (warp >= kKeysWarp && warp < kProductsWarp) {
     // ------------------------------------------------------------ copies
     const uint32_t buffers_at = smem_addr(buffers), q_at = smem_addr(q_smem), full_at = cluster_addr(&bars->full[0], 0);
-    const int run = plan.run, runs = kHalfTile / run, page_size = static_cast<int>(a.page_size);
+    const int run = plan.run, runs = kHalfTile / run;
     const int outside = static_cast<int>(a.pages);  // a page that the cache does not have: zeros
     const bool leader = elect_one(), wide = plan.wide;
     uint32_t g = 0, parts = 0;
     bool ok = true;
-    // Where 64 positions lie: run `lane` (and lane + 32, where there are 64 runs of one position), absent ones
-    // outside the cache; the run that the length cuts is whole here, and positions from `dead` on do not take part.
+    // Where 64 positions lie: run `lane` (and lane + 32, where there are 64 runs of one position), its page as the
+    // table has it (-1: none; looked at when it is used, a tile later); the run that the length cuts is whole here, and
+    // positions from `dead` on do not take part.
     struct Half {
       int page, row, page2, row2, dead;
     };
     auto lookup = [&](int pos0) {
       Half r;
       auto find = [&](int i, int& page, int& row) {
-        const int pos = pos0 + i * run;
-        page = outside;
-        row = 0;
-        if (i < runs && pos < p.len) {
-          const int col = pos / page_size, pg = __ldg(a.table + p.b * a.table_stride + col);
-          if (pg >= 0 && pg < a.pages) {
-            page = pg;
-            row = pos - col * page_size;
-          }
-        }
+        const int pos = pos0 + i * run, col = page_of(plan, pos);
+        page = -1;
+        row = pos - col * static_cast<int>(a.page_size);
+        if (i < runs && pos < p.len) page = __ldg(a.table + p.b * a.table_stride + col);
       };
-      r.page2 = outside;
+      r.page2 = -1;
       r.row2 = 0;
       if (runs > kWarp) find(lane + kWarp, r.page2, r.row2);
       find(lane, r.page, r.row);
       r.dead = max(0, p.len - pos0);
       return r;
     };
+    // absent runs: a page that the cache does not have, zeros
+    auto known = [&](int page) { return static_cast<uint32_t>(page) < static_cast<uint32_t>(outside) ? page : outside; };
     // 64 positions of `n` chunks from the c-th on into dst
     auto copy = [&](uint32_t dst, const Half& r, int c, int n, uint32_t bar) {
       if (wide && n == 4) {
-        if (lane == 0) pair_tma_load_4d(dst, &map_wide, 0, r.row, c, r.page, bar);  // its run is the only one
+        if (lane == 0) pair_tma_load_4d(dst, &map_wide, 0, r.row, c, known(r.page), bar);  // its run is the only one
         return;
       }
+      const int page = known(r.page), page2 = known(r.page2);
       for (int k = 0; k < n; ++k) {
         const int x = c == lat_chunks ? latent : (c + k) * 64;
         const uint32_t to = dst + k * kChunkBytes;
-        if (lane < runs) pair_tma_load_3d(to + lane * run * 128, &map_runs, x, r.row, r.page, bar);
-        if (runs > kWarp) pair_tma_load_3d(to + (lane + kWarp) * 128, &map_runs, x, r.row2, r.page2, bar);
+        if (lane < runs) pair_tma_load_3d(to + lane * run * 128, &map_runs, x, r.row, page, bar);
+        if (runs > kWarp) pair_tma_load_3d(to + (lane + kWarp) * 128, &map_runs, x, r.row2, page2, bar);
       }
     };
     uint32_t cuts = 0;
@@ -477,12 +485,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttnThreads, 1)
         __syncwarp();
         return true;
       }
-      const uint32_t mine = cluster_addr(&bars->cut, rank);
-      if (leader) mbar_arrive_expect_tx(&bars->cut, bytes);
+      uint64_t* own = &bars->cut[i - 3];
+      if (leader) mbar_arrive_expect_tx(own, bytes);
       __syncwarp();
-      copy(dst, r, c, n, mine);
+      copy(dst, r, c, n, cluster_addr(own, rank));
       __syncwarp();
-      if (!warp_wait(&bars->cut, cuts & 1, abort)) return false;
+      if (!warp_wait(own, cuts & 1, abort)) return false;
       ++cuts;
       unsigned char* at = buffers + first_chunk * kChunkBytes;
       for (int row = r.dead + lane / 8; row < (r.dead + run - 1) / run * run; row += 4)
@@ -492,19 +500,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttnThreads, 1)
       if (leader) cluster_arrive(bar);
       __syncwarp();
       return true;
-    };
-    // ask 64 positions into L2, a line at a time (by the load unit: one bulk prefetch would queue in front of the copies)
-    const int lines = static_cast<int>(ceil_div((a.latent + a.rope) * static_cast<int64_t>(sizeof(T)), 128));
-    auto prefetch = [&](const Half& r) {
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const int i = lane + k * kWarp, from = i / run;
-        const int page = runs > kWarp ? (k ? r.page2 : r.page) : __shfl_sync(0xFFFFFFFFu, r.page, from);
-        const int row = runs > kWarp ? (k ? r.row2 : r.row) : __shfl_sync(0xFFFFFFFFu, r.row, from) + i % run;
-        if (page == outside || i >= r.dead) continue;
-        const char* at = reinterpret_cast<const char*>(static_cast<const T*>(a.cache) + page * a.page_stride + row * a.row_stride);
-        for (int l = 0; l < lines; ++l) prefetch_l2(at + l * 128);
-      }
     };
     if (warp == kKeysWarp) {
       const int half = static_cast<int>(rank) * kHalfTile, k0 = min(4, lat_chunks);
@@ -518,32 +513,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttnThreads, 1)
                              p.group * kHeads + static_cast<int>(rank) * kCtaHeads, static_cast<int>(p.b), bar);
         }
         __syncwarp();
-        auto at = [&](int i) { return lookup((p.tile0 + i) * kTile + half); };  // (past the part: rows are there, or nothing)
-        Half now = at(0), next = at(1);
+        Half now = lookup(p.tile0 * kTile + half);
         for (int i = 0; i < p.tiles && ok; ++i, ++g) {
           ok = fill(0, 0, now, 0, k0) && (lat_chunks <= 4 || fill(1, 4, now, 4, lat_chunks - 4)) && fill(2, 8, now, lat_chunks, 1);
-          now = next;
-          next = at(i + 2);
+          if (i + 1 < p.tiles) now = lookup((p.tile0 + i + 1) * kTile + half);
         }
         ++parts;
       }
     } else {
-      const int c = static_cast<int>(rank) * own_chunks;
+      const int c = static_cast<int>(rank) * own_chunks, h = warp - kValuesWarp;
       while (ok && walk.next(a, plan.groups, worker, p)) {
-        Half first = lookup(p.tile0 * kTile), second = lookup(p.tile0 * kTile + kHalfTile);
+        Half now = lookup(p.tile0 * kTile + h * kHalfTile);
         for (int i = 0; i < p.tiles && ok; ++i, ++g) {
-          ok = fill(3, 9, first, c, own_chunks) && fill(4, 13, second, c, own_chunks);
-          if (i + 1 < p.tiles) {
-            first = lookup((p.tile0 + i + 1) * kTile);
-            second = lookup((p.tile0 + i + 1) * kTile + kHalfTile);
-          }
+          ok = fill(3 + h, 9 + 4 * h, now, c, own_chunks);
+          if (i + 1 < p.tiles) now = lookup((p.tile0 + i + 1) * kTile + h * kHalfTile);
         }
       }
     }
     // the copies issued land before either CTA leaves: the first one's barriers count them all, and what
     // the products have consumed had landed
     if (g > 0)
-      for (int i = warp == kKeysWarp ? 0 : 3; i < (warp == kKeysWarp ? 3 : 5); ++i)
+      for (int i = warp == kKeysWarp ? 0 : warp - kValuesWarp + 3, n = warp == kKeysWarp ? 3 : i + 1; i < n; ++i)
         if (i != 1 || lat_chunks > 4)
           mbar_wait(rank == 0 ? &bars->full[i] : &bars->empty[i], (g - 1) & 1, kPagedWaitError);
   } else if (warp == kProductsWarp) {
@@ -613,7 +603,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttnThreads, 1)
     // ------------------------------------------------- softmax and result
     const float c2 = fmaxf(a.scale * kLog2e, 1e-37f);  // above 0: a masked score's -inf stays one
     const uint32_t my_lanes = static_cast<uint32_t>(warp * kWarp) << 16;
-    const int page_size = static_cast<int>(a.page_size);
     const int head = tid % kCtaHeads, part_of = tid / kCtaHeads;  // the thread's head of the CTA, and half of N
     const uint32_t ready_at = cluster_addr(&bars->p_ready, 0);
     const uint32_t read_at = cluster_addr(&bars->o_read, 0);
@@ -646,7 +635,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttnThreads, 1)
           const int pos = (p.tile0 + i) * kTile + part_of * kHalfTile + k * kWarp + lane;
           bool in = pos < p.len;
           if (in) {
-            const int page = __ldg(table + pos / page_size);
+            const int page = __ldg(table + page_of(plan, pos));
             in = page >= 0 && page < a.pages;
             if (!in) atomicOr(&g_device_error, kPagedRangeError);
           }
@@ -721,51 +710,45 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttnThreads, 1)
       const float sum = l + other(l, ok);
       if (!ok) break;
       tc_fence_after();
-      // through the probabilities' buffer, which nothing uses now: 32 columns of the warp's 32 heads at a time, so
-      // that eight lanes write a head's columns side by side
-      float* stage = reinterpret_cast<float*>(p_smem) + warp * (kWarp * 32);
-      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-      const int first_row = static_cast<int>(rank) * kCtaHeads + (warp % 2) * kWarp + lane / 8;  // of the group's 128 heads
-      const int rows = static_cast<int>(min(a.heads - p.group * kHeads, static_cast<int64_t>(kHeads)));
-      const int unit = lane % 8;
-      T* out = static_cast<T*>(a.out) + (p.b * a.heads + p.group * kHeads + first_row) * latent + unit * 4;
-      float* part = plan.part_o + (static_cast<int64_t>(p.slot) * kHeads + first_row) * latent + unit * 4;
-      const float scale = p.whole ? inv : 1.0f;
-      for (int c = 0; c < 2 * own_chunks; ++c) {  // 32 columns c of this half of N
+      // a thread its head's columns of this half of N, whole 32-byte sectors at a time
+      const float scale = p.whole ? (sum == 0.0f ? 0.0f : 1.0f / sum) : 1.0f;
+      const int row = static_cast<int>(rank) * kCtaHeads + head;  // of the group's 128 heads
+      const bool has = row < a.heads - p.group * kHeads;
+      T* out = static_cast<T*>(a.out) + (p.b * a.heads + p.group * kHeads + row) * latent;
+      const bool sectors = latent % 16 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 31u) == 0;
+      float* part = plan.part_o + (static_cast<int64_t>(p.slot) * kHeads + row) * latent;
+      for (int c = 0; c < 2 * own_chunks; ++c) {  // 32 columns
         const int col0 = part_of * own_chunks * 64 + c * 32;
         if (col0 >= latent) break;
         uint32_t o[32];
         tmem_ld32(tmem + my_lanes + kColO + c * 32, o);
         tmem_ld_wait();
+        if (!has) continue;
 #pragma unroll
-        for (int j = 0; j < 32; j += 4)
-          *reinterpret_cast<float4*>(stage + lane * 32 + ((j / 4) ^ (lane % 8)) * 4) =
-              make_float4(__uint_as_float(o[j]) * scale, __uint_as_float(o[j + 1]) * scale, __uint_as_float(o[j + 2]) * scale,
-                          __uint_as_float(o[j + 3]) * scale);
-        __syncwarp();
-        float4 v[8];
+        for (int j = 0; j < 32; j += 16) {
+          if (col0 + j >= latent) break;
+          if (!p.whole) {
+            store_sector(part + col0 + j, o + j);
+            if (col0 + j + 8 < latent) store_sector(part + col0 + j + 8, o + j + 8);
+            continue;
+          }
+          uint32_t v[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int row = lane / 8 + 4 * i;
-          v[i] = *reinterpret_cast<const float4*>(stage + row * 32 + ((unit ^ (row % 8)) * 4));
-        }
-        __syncwarp();
-        if (col0 + unit * 4 >= latent) continue;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (first_row + 4 * i >= rows) break;
-          if (p.whole) *reinterpret_cast<uint2*>(out + 4 * i * latent + col0) = make_uint2(pack2<T>(v[i].x, v[i].y), pack2<T>(v[i].z, v[i].w));
-          else *reinterpret_cast<float4*>(part + 4 * i * latent + col0) = v[i];
+          for (int k = 0; k < 8; ++k)
+            v[k] = pack2<T>(__uint_as_float(o[j + 2 * k]) * scale, __uint_as_float(o[j + 2 * k + 1]) * scale);
+          if (sectors && col0 + j + 16 <= latent) store_sector(out + col0 + j, v);
+          else {
+            *reinterpret_cast<uint4*>(out + col0 + j) = make_uint4(v[0], v[1], v[2], v[3]);
+            if (col0 + j + 8 < latent) *reinterpret_cast<uint4*>(out + col0 + j + 8) = make_uint4(v[4], v[5], v[6], v[7]);
+          }
         }
       }
-      __syncwarp();
       const int64_t h = p.group * kHeads + static_cast<int64_t>(rank) * kCtaHeads + head;
       if (part_of == 0 && h < a.heads) {
         if (!p.whole) plan.part_ml[static_cast<int64_t>(p.slot) * kHeads + (h - p.group * kHeads)] = make_float2(m, sum);
         else if (a.lse) a.lse[p.b * a.heads + h] = sum == 0.0f ? -INFINITY : (m + log2f(sum)) * kLn2;
       }
       tc_fence_before();
-      // (all four warps have left the staging before any writes probabilities: the next tile's exchange orders them)
       __syncwarp();
       if (lane == 0) cluster_arrive(read_at);
     }
@@ -880,6 +863,10 @@ AttnPlan attn_plan(Plan& p, int64_t batch, int64_t heads, int64_t latent, int64_
   l.workers = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({gemv_grid_ctas() / 2, kMostWorkers, ceil_div(most, kMinTiles)})));
   l.run = 1;
   while (l.run < kHalfTile && page_size % (2 * l.run) == 0) l.run *= 2;
+  l.page_size = static_cast<int>(page_size);
+  l.shift = -1;
+  for (int i = 0; i < 31; ++i)
+    if (page_size == int64_t(1) << i) l.shift = i;
   l.wide = l.run == kHalfTile && latent % 64 == 0;
   l.part_o = p.take<float>(2 * l.workers * kHeads * latent);
   l.part_ml = p.take<float2>(2 * l.workers * kHeads);

@@ -132,6 +132,7 @@ int moe_paged_mla_attention(const void* q_latent, int64_t ql_stride, int64_t ql_
   if ((batch > 1 && (ql_stride <= 0 || qp_stride <= 0)) || (heads > 1 && (ql_head_stride <= 0 || qp_head_stride <= 0)) ||
       (pages > 1 && page_stride <= 0) || (page_size > 1 && row_stride <= 0))
     return fail(kUnsupported, "strides must be positive");
+  if (reinterpret_cast<uintptr_t>(workspace) & 31u) return fail(kUnsupported, "the workspace must start on a 32-byte boundary");
   if (batch == 0) return kOk;
   PagedAttnArgs a{};
   a.q_latent = q_latent; a.q_pe = q_pe; a.cache = cache; a.table = page_table; a.lengths = lengths; a.out = out;
