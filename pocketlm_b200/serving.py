@@ -44,30 +44,26 @@ class NormedRows(NamedTuple):
     normed: torch.Tensor | None  # the normed rows in x's type, when asked for
 
 
-def _need(ok: bool, message: str) -> None:
-    if not ok:
-        raise ValueError(message)
-
-
-def _call(name: str, device: torch.device, *args) -> None:
-    fn, index = getattr(native.load_library(), name), device.index
+def _call(fn, index: int, *args) -> None:
+    """fn(*args, stream) on device `index`, on its current stream."""
     if index == torch.cuda.current_device():
         code = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
             code = fn(*args, _raw_stream(index))
     if code:
-        native._check(code, name)
+        native._check(code, fn.__name__)
 
 
-def _one_device(*tensors: torch.Tensor | None) -> torch.device:
-    device = tensors[0].device
-    if device.type != "cuda":
+def _one_device(*tensors: torch.Tensor | None) -> int:
+    """The index of the CUDA device that all of them are on."""
+    index = tensors[0].get_device()
+    if index < 0:
         raise ValueError("tensors must be on a CUDA device")
     for t in tensors:
-        if t is not None and t.device != device:
+        if t is not None and t.get_device() != index:
             raise ValueError("tensors must be on one device")
-    return device
+    return index
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -80,7 +76,7 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 def _new_codes(flat: torch.Tensor, rows: int, cols: int) -> torch.Tensor:
     """Codes [rows, cols] whose rows start on 16-byte boundaries, as fp8_block_linear reads them."""
     if cols % 16 == 0:
-        return flat.new_empty((rows, cols), dtype=torch.float8_e4m3fn)
+        return torch.empty_like(flat, dtype=torch.float8_e4m3fn) if flat.is_contiguous() else flat.new_empty((rows, cols), dtype=torch.float8_e4m3fn)
     return flat.new_empty((rows, (cols + 15) // 16 * 16), dtype=torch.float8_e4m3fn)[:, :cols]
 
 
@@ -95,12 +91,18 @@ def rmsnorm_fp8(x: torch.Tensor, weight: torch.Tensor, *, residual: torch.Tensor
     shape, dtype = x.shape, x.dtype
     cols = shape[-1] if shape else 0
     code = _CODE.get(dtype)
-    _need(code is not None, "x must be bf16, fp16 or fp32")
-    _need(cols > 0, "x must be [..., cols]")
-    _need(weight.shape == (cols,), "weight must be [cols]")
-    _need(weight.dtype == dtype or weight.dtype == torch.float32, "weight must be of x's type or fp32")
-    _need(residual is None or (residual.shape == shape and residual.dtype == dtype), "residual must be like x")
-    _need(cols <= 32768, "x has more than 32768 columns")
+    if not (code is not None):
+        raise ValueError("x must be bf16, fp16 or fp32")
+    if not (cols > 0):
+        raise ValueError("x must be [..., cols]")
+    if not (weight.shape == (cols,)):
+        raise ValueError("weight must be [cols]")
+    if not (weight.dtype == dtype or weight.dtype == torch.float32):
+        raise ValueError("weight must be of x's type or fp32")
+    if not (residual is None or (residual.shape == shape and residual.dtype == dtype)):
+        raise ValueError("residual must be like x")
+    if not (cols <= 32768):
+        raise ValueError("x has more than 32768 columns")
     device = _one_device(x, weight, residual)
     flat, weight = _rows(x), weight.contiguous()
     rows = flat.shape[0]
@@ -109,11 +111,11 @@ def rmsnorm_fp8(x: torch.Tensor, weight: torch.Tensor, *, residual: torch.Tensor
     normed = flat.new_empty((rows, cols)) if return_normed else None
     stream = res = None
     if residual is not None:
-        res, stream = _rows(residual), flat.new_empty((rows, cols))
+        res, stream = _rows(residual), torch.empty_like(flat) if flat.is_contiguous() else flat.new_empty((rows, cols))
     if rows:
-        _call("moe_rmsnorm_fp8", device, flat.data_ptr(), flat.stride(0), code, None if res is None else res.data_ptr(),
+        _call(native.load_library().moe_rmsnorm_fp8, device, flat.data_ptr(), flat.stride(0), code, None if res is None else res.data_ptr(),
               0 if res is None else res.stride(0), weight.data_ptr(), code if weight.dtype == dtype else native.DTYPE_F32,
-              rows, cols, eps, codes.data_ptr(), codes.stride(0), scales.data_ptr(),
+              rows, cols, eps, codes.data_ptr(), codes.stride(0) if rows > 1 else cols, scales.data_ptr(),
               None if stream is None else stream.data_ptr(), None if normed is None else normed.data_ptr())
     if len(shape) != 2:
         codes, scales = codes.view(shape), scales.view(*shape[:-1], scales.shape[1])
@@ -128,16 +130,18 @@ def quantize_fp8_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     shape = x.shape
     cols = shape[-1] if shape else 0
     code = _CODE.get(x.dtype)
-    _need(code is not None, "x must be bf16, fp16 or fp32")
-    _need(cols > 0, "x must be [..., cols]")
+    if not (code is not None):
+        raise ValueError("x must be bf16, fp16 or fp32")
+    if not (cols > 0):
+        raise ValueError("x must be [..., cols]")
     device = _one_device(x)
     flat = _rows(x)
     rows = flat.shape[0]
     codes = _new_codes(flat, rows, cols)
     scales = flat.new_empty((rows, (cols + 127) // 128), dtype=torch.float32)
     if rows:
-        _call("moe_fp8_quantize_rows", device, flat.data_ptr(), flat.stride(0), code, rows, cols, codes.data_ptr(),
-              codes.stride(0), scales.data_ptr())
+        _call(native.load_library().moe_fp8_quantize_rows, device, flat.data_ptr(), flat.stride(0), code, rows, cols, codes.data_ptr(),
+              codes.stride(0) if rows > 1 else cols, scales.data_ptr())
     if len(shape) != 2:
         codes, scales = codes.view(shape), scales.view(*shape[:-1], scales.shape[1])
     return codes, scales
@@ -159,27 +163,45 @@ def fp8_block_linear(codes: torch.Tensor, scales: torch.Tensor, fp8_weight: torc
     [out, in] e4m3 (or its bytes) and scale_inv [ceil(out / 128), ceil(in / 128)] as the checkpoints hold them.
     Sums in fp32, one rounding to out_dtype (bf16, fp16 or fp32).  NaN codes are NaN (the fp32-activation linears
     of `native` read them as 0).  Rows that do not start on 16-byte boundaries are copied first."""
-    _need(codes.dtype in _FP8 and fp8_weight.dtype in _FP8, "codes and fp8_weight must be e4m3")
-    _need(scales.dtype == torch.float32 and scale_inv.dtype == torch.float32, "scales must be fp32")
-    _need(out_dtype in _CODE, "out_dtype must be bf16, fp16 or fp32")
-    _need(fp8_weight.ndim == 2, "fp8_weight must have shape [out_rows, in_cols]")
-    _need(scale_inv.ndim == 2, "scale_inv must have shape [scale_rows, scale_cols]")
+    if not (codes.dtype in _FP8 and fp8_weight.dtype in _FP8):
+        raise ValueError("codes and fp8_weight must be e4m3")
+    if not (scales.dtype == torch.float32 and scale_inv.dtype == torch.float32):
+        raise ValueError("scales must be fp32")
+    if not (out_dtype in _CODE):
+        raise ValueError("out_dtype must be bf16, fp16 or fp32")
+    if not (fp8_weight.ndim == 2):
+        raise ValueError("fp8_weight must have shape [out_rows, in_cols]")
+    if not (scale_inv.ndim == 2):
+        raise ValueError("scale_inv must have shape [scale_rows, scale_cols]")
     outs, cols = fp8_weight.shape
     blocks = (cols + 127) // 128
-    _need(outs > 0 and cols > 0, "fp8_weight must not be empty")
-    _need(codes.ndim >= 1 and codes.shape[-1] == cols, "hidden input size does not match FP8 weight columns")
-    _need(scale_inv.shape == ((outs + 127) // 128, blocks), "scale_inv shape does not match FP8 128x128 block layout")
+    if not (outs > 0 and cols > 0):
+        raise ValueError("fp8_weight must not be empty")
+    if not (codes.ndim >= 1 and codes.shape[-1] == cols):
+        raise ValueError("hidden input size does not match FP8 weight columns")
+    if not (scale_inv.shape == ((outs + 127) // 128, blocks)):
+        raise ValueError("scale_inv shape does not match FP8 128x128 block layout")
     lead = codes.shape[:-1]
-    _need(scales.shape == (*lead, blocks), "scales must be [..., ceil(in_cols / 128)]")
+    if not (scales.shape == (*lead, blocks)):
+        raise ValueError("scales must be [..., ceil(in_cols / 128)]")
     device = _one_device(codes, scales, fp8_weight, scale_inv)
     x, w = codes if codes.ndim == 2 else codes.reshape(-1, cols), _code_rows(fp8_weight)
     rows = x.shape[0]
     x, scales, scale_inv = _code_rows(x), scales.contiguous(), scale_inv.contiguous()
     out = scales.new_empty((rows, outs), dtype=out_dtype)
     if rows:
-        _call("moe_fp8_block_linear", device, x.data_ptr(), x.stride(0), scales.data_ptr(), w.data_ptr(), w.stride(0),
+        _call(native.load_library().moe_fp8_block_linear, device, x.data_ptr(), x.stride(0), scales.data_ptr(), w.data_ptr(), w.stride(0),
               scale_inv.data_ptr(), rows, outs, cols, out.data_ptr(), _CODE[out_dtype])
     return out if len(lead) == 1 else out.reshape(*lead, outs)
+
+
+def _cache_layout(cache: torch.Tensor):
+    shape, strides, dtype = cache.shape, cache.stride(), cache.dtype
+    if len(shape) != 3 or strides[2] != 1 or 0 in shape:
+        raise ValueError("cache must be [pages, page_size, latent + rope]")
+    if dtype != torch.bfloat16 and dtype != torch.float16:
+        raise ValueError("cache must be bf16 or fp16")
+    return *shape, dtype, strides
 
 
 def paged_mla_append(kv_rows: torch.Tensor, kv_norm_weight: torch.Tensor, cache: torch.Tensor, slots: torch.Tensor,
@@ -194,38 +216,48 @@ def paged_mla_append(kv_rows: torch.Tensor, kv_norm_weight: torch.Tensor, cache:
     [tokens] into rope_cos / rope_sin fp32 [max_positions, rope / 2], pairs (2p, 2p + 1); q_pe [tokens, heads,
     rope] of the cache's type (a slice of the q_b projection's output needs no copy).  A position outside the
     tables gives zero queries and stores no row."""
-    _need(cache.ndim == 3 and cache.stride(2) == 1 and cache.numel() > 0, "cache must be [pages, page_size, latent + rope]")
-    _need(cache.dtype in (torch.bfloat16, torch.float16), "cache must be bf16 or fp16")
-    pages, page_size, width = cache.shape
-    _need(kv_norm_weight.ndim == 1 and rope_cos.ndim == 2 and rope_cos.shape == rope_sin.shape,
-          "kv_norm_weight must be [latent], rope_cos and rope_sin [max_positions, rope / 2]")
-    latent, rope, tokens = kv_norm_weight.shape[0], 2 * rope_cos.shape[1], kv_rows.shape[0]
-    _need(kv_rows.ndim == 2 and kv_rows.shape[1] == latent + rope == width, "kv_rows, cache and norm weight sizes do not match")
-    _need(latent > 0 and rope > 0 and rope_cos.shape[0] > 0, "latent, rope and the tables must not be empty")
-    _need(slots.shape == (tokens,) and positions.shape == (tokens,), "slots and positions must be [tokens]")
-    _need(slots.dtype == torch.int64 and positions.dtype == torch.int64, "slots and positions must be int64")
-    _need(kv_rows.dtype in (cache.dtype, torch.float32), "kv_rows must be of the cache's type or fp32")
-    _need(kv_norm_weight.dtype in (cache.dtype, torch.float32), "kv_norm_weight must be of the cache's type or fp32")
-    _need(rope_cos.dtype == torch.float32 and rope_sin.dtype == torch.float32, "rope tables must be fp32")
-    _need(q_pe is None or (q_pe.ndim == 3 and q_pe.shape[0] == tokens and q_pe.shape[1] > 0 and q_pe.shape[2] == rope),
-          "q_pe must be [tokens, heads, rope]")
-    _need(q_pe is None or q_pe.dtype == cache.dtype, "q_pe must be of the cache's type")
-    device = _one_device(cache, kv_rows, kv_norm_weight, slots, positions, rope_cos, rope_sin, q_pe)
-    kv = _rows(kv_rows)
-    q_out, heads, q_strides = None, 0, (0, 0)
+    pages, page_size, width, dtype, strides = _cache_layout(cache)
+    code, kv_shape, table = _CODE[dtype], kv_rows.shape, rope_cos.shape
+    if kv_norm_weight.ndim != 1 or len(table) != 2 or table != rope_sin.shape:
+        raise ValueError("kv_norm_weight must be [latent], rope_cos and rope_sin [max_positions, rope / 2]")
+    latent, rope, tokens = kv_norm_weight.shape[0], 2 * table[1], kv_shape[0]
+    if len(kv_shape) != 2 or kv_shape[1] != width or latent + rope != width:
+        raise ValueError("kv_rows, cache and norm weight sizes do not match")
+    if latent == 0 or rope == 0 or table[0] == 0:
+        raise ValueError("latent, rope and the tables must not be empty")
+    if slots.shape != (tokens,) or positions.shape != (tokens,):
+        raise ValueError("slots and positions must be [tokens]")
+    if slots.dtype != torch.int64 or positions.dtype != torch.int64:
+        raise ValueError("slots and positions must be int64")
+    kv_code, norm_code = _CODE.get(kv_rows.dtype), _CODE.get(kv_norm_weight.dtype)
+    if kv_code != code and kv_code != native.DTYPE_F32:
+        raise ValueError("kv_rows must be of the cache's type or fp32")
+    if norm_code != code and norm_code != native.DTYPE_F32:
+        raise ValueError("kv_norm_weight must be of the cache's type or fp32")
+    if rope_cos.dtype != torch.float32 or rope_sin.dtype != torch.float32:
+        raise ValueError("rope tables must be fp32")
+    heads, q_ptr, q_strides, q_out = 0, None, (0, 0), None
     if q_pe is not None:
-        if q_pe.stride(2) != 1:
+        q_shape = q_pe.shape
+        if len(q_shape) != 3 or q_shape[0] != tokens or q_shape[1] == 0 or q_shape[2] != rope:
+            raise ValueError("q_pe must be [tokens, heads, rope]")
+        if q_pe.dtype != dtype:
+            raise ValueError("q_pe must be of the cache's type")
+        heads = q_shape[1]
+    device = _one_device(cache, kv_rows, kv_norm_weight, slots, positions, rope_cos, rope_sin, q_pe)
+    if q_pe is not None:
+        q_strides = q_pe.stride()
+        if q_strides[2] != 1:
             q_pe = q_pe.contiguous()
-        heads, q_strides = q_pe.shape[1], q_pe.stride()[:2]
-        q_out = cache.new_empty((tokens, heads, rope))
+            q_strides = q_pe.stride()
+        q_ptr, q_out = q_pe.data_ptr(), cache.new_empty((tokens, heads, rope))
     if tokens:
-        norm_w, slots, positions = kv_norm_weight.contiguous(), slots.contiguous(), positions.contiguous()
+        kv, norm_w, slots, positions = _rows(kv_rows), kv_norm_weight.contiguous(), slots.contiguous(), positions.contiguous()
         cos, sin = rope_cos.contiguous(), rope_sin.contiguous()
-        _call("moe_paged_mla_append", device, kv.data_ptr(), kv.stride(0), _CODE[kv.dtype], norm_w.data_ptr(),
-              _CODE[norm_w.dtype], slots.data_ptr(), positions.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0],
-              cache.data_ptr(), _CODE[cache.dtype], pages, page_size, cache.stride(0), cache.stride(1),
-              None if q_pe is None else q_pe.data_ptr(), *q_strides, heads, None if q_out is None else q_out.data_ptr(),
-              tokens, latent, rope, float(eps))
+        _call(native.load_library().moe_paged_mla_append, device, kv.data_ptr(), kv.stride(0), kv_code, norm_w.data_ptr(),
+              norm_code, slots.data_ptr(), positions.data_ptr(), cos.data_ptr(), sin.data_ptr(), table[0], cache.data_ptr(),
+              code, pages, page_size, strides[0], strides[1], q_ptr, q_strides[0], q_strides[1], heads,
+              None if q_out is None else q_out.data_ptr(), tokens, latent, rope, eps)
     return q_out
 
 
@@ -234,12 +266,14 @@ def _attention_workspace(*dims: int) -> int:
     return max(int(native.load_library().moe_paged_mla_attention_workspace_bytes(*dims)), 256)
 
 
-def _query(t: torch.Tensor) -> torch.Tensor:
-    """Queries whose rows start on 16-byte boundaries and are stored one by one (a copy where they are not)."""
-    s0, s1, s2 = t.stride()
-    if s2 == 1 and s0 > 0 and s1 > 0 and s0 % 8 == 0 and s1 % 8 == 0 and t.data_ptr() % 16 == 0:
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
+def _query(t: torch.Tensor) -> tuple[torch.Tensor, int, tuple[int, ...]]:
+    """Queries whose rows start on 16-byte boundaries and are stored one by one (a copy where they are not), with their
+    address and strides."""
+    strides, ptr = t.stride(), t.data_ptr()
+    if strides[2] != 1 or strides[0] <= 0 or strides[1] <= 0 or strides[0] % 8 or strides[1] % 8 or ptr % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+        strides, ptr = t.stride(), t.data_ptr()
+    return t, ptr, strides
 
 
 def paged_mla_attention(q_latent: torch.Tensor, q_pe: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor,
@@ -253,32 +287,38 @@ def paged_mla_attention(q_latent: torch.Tensor, q_pe: torch.Tensor, cache: torch
     return_lse also log(sum exp(score)) fp32 [batch, heads].  A row of length 0 gives zeros (and -inf); entries of
     page_table past a row's last page are not read.  Several tokens of one sequence are rows with the same pages and
     lengths one apart.  latent <= 512 and rope <= 64, multiples of 8; any page size."""
-    _need(cache.ndim == 3 and cache.stride(2) == 1 and cache.numel() > 0, "cache must be [pages, page_size, latent + rope]")
-    _need(cache.dtype in (torch.bfloat16, torch.float16), "cache must be bf16 or fp16")
-    _need(q_latent.ndim == 3 and q_pe.ndim == 3, "q_latent and q_pe must be [batch, heads, dim]")
-    batch, heads, latent = q_latent.shape
-    rope = q_pe.shape[2]
-    pages, page_size, width = cache.shape
-    _need(q_pe.shape[:2] == q_latent.shape[:2] and heads > 0, "batch or head count mismatch")
-    _need(latent > 0 and rope > 0 and latent + rope == width, "query and cache sizes do not match")
-    _need(q_latent.dtype == cache.dtype and q_pe.dtype == cache.dtype, "queries must be of the cache's type")
-    _need(page_table.ndim == 2 and page_table.shape[0] == batch and page_table.shape[1] > 0,
-          "page_table must be [batch, max_pages]")
-    _need(lengths.shape == (batch,), "lengths must be [batch]")
-    _need(page_table.dtype == torch.int32 and lengths.dtype == torch.int32, "page_table and lengths must be int32")
-    _need(cache.stride(0) % 8 == 0 and cache.stride(1) % 8 == 0 and cache.data_ptr() % 16 == 0,
-          "cache rows must start on 16-byte boundaries")
+    pages, page_size, width, dtype, strides = _cache_layout(cache)
+    q_shape, pe_shape, table_shape = q_latent.shape, q_pe.shape, page_table.shape
+    if len(q_shape) != 3 or len(pe_shape) != 3:
+        raise ValueError("q_latent and q_pe must be [batch, heads, dim]")
+    batch, heads, latent = q_shape
+    rope = pe_shape[2]
+    if pe_shape[0] != batch or pe_shape[1] != heads or heads == 0:
+        raise ValueError("batch or head count mismatch")
+    if latent == 0 or rope == 0 or latent + rope != width:
+        raise ValueError("query and cache sizes do not match")
+    if q_latent.dtype != dtype or q_pe.dtype != dtype:
+        raise ValueError("queries must be of the cache's type")
+    if len(table_shape) != 2 or table_shape[0] != batch or table_shape[1] == 0:
+        raise ValueError("page_table must be [batch, max_pages]")
+    if lengths.shape != (batch,):
+        raise ValueError("lengths must be [batch]")
+    if page_table.dtype != torch.int32 or lengths.dtype != torch.int32:
+        raise ValueError("page_table and lengths must be int32")
+    cache_ptr = cache.data_ptr()
+    if strides[0] % 8 or strides[1] % 8 or cache_ptr % 16:
+        raise ValueError("cache rows must start on 16-byte boundaries")
     device = _one_device(cache, q_latent, q_pe, page_table, lengths)
-    q_latent, q_pe = _query(q_latent), _query(q_pe)
-    out = cache.new_empty((batch, heads, latent))
+    out = torch.empty_like(q_latent) if q_latent.is_contiguous() else cache.new_empty(q_shape)
     lse = cache.new_empty((batch, heads), dtype=torch.float32) if return_lse else None
     if batch:
+        (ql, ql_ptr, ql_strides), (qp, qp_ptr, qp_strides) = _query(q_latent), _query(q_pe)
         table = page_table if page_table.stride(1) == 1 else page_table.contiguous()
         lengths = lengths.contiguous()
-        work = cache.new_empty((_attention_workspace(batch, heads, latent, rope, table.shape[1], page_size),), dtype=torch.uint8)
-        _call("moe_paged_mla_attention", device, q_latent.data_ptr(), q_latent.stride(0), q_latent.stride(1),
-              q_pe.data_ptr(), q_pe.stride(0), q_pe.stride(1), cache.data_ptr(), _CODE[cache.dtype], pages, page_size,
-              cache.stride(0), cache.stride(1), table.data_ptr(), table.stride(0), table.shape[1], lengths.data_ptr(),
-              batch, heads, latent, rope, float(softmax_scale), out.data_ptr(), None if lse is None else lse.data_ptr(),
-              work.data_ptr(), work.numel())
+        need = _attention_workspace(batch, heads, latent, rope, table_shape[1], page_size)
+        work = cache.new_empty((need,), dtype=torch.uint8)
+        _call(native.load_library().moe_paged_mla_attention, device, ql_ptr, ql_strides[0], ql_strides[1], qp_ptr,
+              qp_strides[0], qp_strides[1], cache_ptr, _CODE[dtype], pages, page_size, strides[0], strides[1],
+              table.data_ptr(), table.stride(0), table_shape[1], lengths.data_ptr(), batch, heads, latent, rope,
+              softmax_scale, out.data_ptr(), None if lse is None else lse.data_ptr(), work.data_ptr(), need)
     return (out, lse) if return_lse else out
