@@ -14,9 +14,9 @@
 // sums are added through distributed shared memory in rank order (the same
 // result on every run).
 //
-// Many rows (linear_tiles_kernel): the tensor cores bound it.  128 tokens x up
-// to 256 outputs per CTA and tile, two accumulators so that the sums of one
-// group are read while the next is computed; persistent CTAs.
+// Many rows (linear_tiles_kernel): the tensor cores bound it.  256 tokens x up
+// to 256 outputs per pair of CTAs and tile, two accumulators so that the sums
+// of one group are read while the next is computed; persistent.
 #include <algorithm>
 
 #include "fp8_gemv.cuh"
@@ -40,8 +40,9 @@ constexpr int kRowsThreads = 192;  // warps 0-3: sums (a thread per weight row);
 constexpr int kWTileBytes = 128 * kGroup;
 template <int NT>
 struct RowsShape {
-  static constexpr int kStages = NT <= 32 ? 5 : NT <= 64 ? 4 : 3;
-  static constexpr int kBufs = NT <= 64 ? 4 : 2;  // accumulators in tensor memory
+  static constexpr int kStages = NT <= 32 ? 5 : NT <= 64 ? 4 : 6;
+  static constexpr int kPerSm = NT <= 64 ? 2 : 1;  // CTAs that fit an SM
+  static constexpr int kBufs = 4;                  // accumulators in tensor memory
   static constexpr int kCols = NT * kBufs < 32 ? 32 : NT * kBufs;
   static constexpr int kStageBytes = kWTileBytes + NT * kGroup;
   static constexpr int kPipeBytes = kStages * kStageBytes;
@@ -230,122 +231,159 @@ __global__ void __launch_bounds__(kRowsThreads) linear_rows_kernel(const __grid_
 
 // ----------------------------------------------------------------- many rows
 
-// 128 tokens x TN outputs per CTA and tile.  (Pairs of CTAs sharing a 256-token
-// tile halve the bytes from L2, but a group's sums are handed over every 500
-// cycles, and across the pair the handshake alone took 1160: 912 us against 500
-// on 4000 x 7168 x 16384.)
+// PAIR: two CTAs (cta_group::2) take 256 tokens x TN outputs, each holding its
+// 128 tokens' rows and half of the weight rows.  That halves the weights' bytes
+// from L2 and runs the products faster (four steps of M = 256, N = 256 take 520
+// cycles over the pair, of M = 128, N = 256 on one CTA 690).  Otherwise one CTA
+// takes 128 tokens x TN.  In both a group's sums must leave tensor memory every
+// 500 cycles, and the two come within a twentieth of each other per round of all
+// SMs (4000 x 7168 x 16384: 458 us in pairs, 483 alone); the finer tiles of one
+// CTA fill the SMs where a pair's do not (600 x 7168 x 7168: 36 us against 63).
 constexpr int kTileM = 128;  // tokens per CTA
 constexpr int kSumWarps = 8;  // warp w: tokens 32 (w % 4) .. + 31, half w / 4 of the TN columns
-constexpr int kTilesThreads = (kSumWarps + 3) * kWarp;  // .. 8: TMA; 9, 10: the products of even and odd groups
-template <int TN>
+constexpr int kTilesThreads = (kSumWarps + 4) * kWarp;  // .. 8: TMA; 9, 10: the products of even and odd groups
+template <int TN, bool PAIR>
 struct TilesShape {
-  static constexpr int kABytes = kTileM * kGroup, kBBytes = TN * kGroup, kStageBytes = kABytes + kBBytes;
-  static constexpr int kStages = TN > 224 ? 4 : 5;
+  static constexpr int kCtas = PAIR ? 2 : 1;
+  static constexpr int kABytes = kTileM * kGroup, kBBytes = TN / kCtas * kGroup, kStageBytes = kABytes + kBBytes;
+  static constexpr int kStages = PAIR ? 6 : 4;
 };
-template <int TN>
+template <int TN, bool PAIR>
 struct TilesBarriers {
-  uint64_t full[TilesShape<TN>::kStages], empty[TilesShape<TN>::kStages];
+  uint64_t full[TilesShape<TN, PAIR>::kStages], empty[TilesShape<TN, PAIR>::kStages];
   uint64_t sum_full[2], sum_empty[2];
   uint64_t drain;
   uint32_t tmem_base;
   int abort;
 };
-template <int TN>
+template <int TN, bool PAIR>
 constexpr size_t tiles_smem() {
-  return 1024 + TilesShape<TN>::kStages * TilesShape<TN>::kStageBytes + sizeof(TilesBarriers<TN>);
+  return 1024 + TilesShape<TN, PAIR>::kStages * TilesShape<TN, PAIR>::kStageBytes + sizeof(TilesBarriers<TN, PAIR>);
 }
-static_assert(tiles_smem<256>() <= 232448 && tiles_smem<224>() <= 232448, "shared memory per block");
+static_assert(tiles_smem<256, true>() <= 232448 && tiles_smem<256, false>() <= 232448, "shared memory per block");
 
-template <typename O, int TN>
+template <typename O, int TN, bool PAIR>
 __global__ void __launch_bounds__(kTilesThreads, 1)
     linear_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, LinearArgs a,
                         int m_tiles, int n_tiles) {
-  using Shape = TilesShape<TN>;
-  constexpr int kStages = Shape::kStages, kHalf = TN / 2, kStageBytes = Shape::kStageBytes;
+  using Shape = TilesShape<TN, PAIR>;
+  constexpr int kStages = Shape::kStages, kHalf = TN / 2, kStageBytes = Shape::kStageBytes, kCtas = Shape::kCtas;
   extern __shared__ unsigned char smem_raw[];
+  // the same place in both CTAs (their shared memory starts alike)
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  auto* bars = reinterpret_cast<TilesBarriers<TN>*>(smem + kStages * kStageBytes);
+  auto* bars = reinterpret_cast<TilesBarriers<TN, PAIR>*>(smem + kStages * kStageBytes);
   const int tid = threadIdx.x, lane = tid % kWarp, warp = __shfl_sync(0xFFFFFFFFu, tid / kWarp, 0);
   volatile int* abort = &bars->abort;
+  const int rank = PAIR ? static_cast<int>(cluster_rank()) : 0;
   const int groups = static_cast<int>((a.cols + kGroup - 1) / kGroup);
-  const int tiles = m_tiles * n_tiles;
+  const int tiles = m_tiles * n_tiles, pair = blockIdx.x / kCtas, pairs = gridDim.x / kCtas;
 
   if (tid == 0) {
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(&bars->full[s], 1);
+      mbar_init(&bars->full[s], kCtas);
       mbar_init(&bars->empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&bars->sum_full[b], 1);
-      mbar_init(&bars->sum_empty[b], kSumWarps);
+      mbar_init(&bars->sum_empty[b], kCtas * kSumWarps);
     }
     mbar_init(&bars->drain, 2);
     bars->abort = 0;
     fence_barrier_init();
   }
   if (warp == kSumWarps + 1) {
-    tmem_alloc(&bars->tmem_base, 512);
-    tmem_relinquish();
+    if (PAIR) {
+      pair_tmem_alloc(&bars->tmem_base, 512);
+    } else {
+      tmem_alloc(&bars->tmem_base, 512);
+      tmem_relinquish();
+    }
   }
   tc_fence_before();
   __syncthreads();
+  if (PAIR) cluster_sync();
   tc_fence_after();
   const uint32_t tmem = bars->tmem_base;
 
-  if (warp == kSumWarps) {
-    const bool leader = elect_one();
-    const uint32_t at = smem_addr(smem);
-    uint32_t i = 0;
-    bool ok = true;
-    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-      const int m0 = t % m_tiles * kTileM, n0 = t / m_tiles * TN;
-      for (int g = 0; g < groups; ++g, ++i) {
-        const uint32_t s = i % kStages;
-        if (i >= kStages && !warp_wait(&bars->empty[s], ((i / kStages) - 1) & 1, abort)) {
-          ok = false;
-          break;
+  // 168 registers per thread at launch (three warpgroups): the sums' two take 224
+  // and the third keeps 56, 256 * 224 + 128 * 56 = 384 * 168
+  if (warp >= kSumWarps) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == kSumWarps) {
+      // each CTA loads its share; the first one's barriers count both
+      const bool leader = elect_one();
+      const uint32_t at = smem_addr(smem), full_at = PAIR ? cluster_addr(&bars->full[0], 0) : 0;
+      uint32_t i = 0;
+      bool ok = true;
+      for (int t = pair; t < tiles && ok; t += pairs) {
+        const int m0 = (t % m_tiles * kCtas + rank) * kTileM, n0 = t / m_tiles * TN + rank * (TN / kCtas);
+        for (int g = 0; g < groups; ++g, ++i) {
+          const uint32_t s = i % kStages, dst = at + s * kStageBytes, bar = full_at + s * 8;
+          if (i >= kStages && !warp_wait(&bars->empty[s], ((i / kStages) - 1) & 1, abort)) {
+            ok = false;
+            break;
+          }
+          if (leader) {
+            if (PAIR) {
+              cluster_arrive_expect_tx(bar, kStageBytes);
+              pair_tma_load_2d(dst, &map_x, g * kGroup, m0, bar);
+              pair_tma_load_2d(dst + Shape::kABytes, &map_w, g * kGroup, n0, bar);
+            } else {
+              mbar_arrive_expect_tx(&bars->full[s], kStageBytes);
+              tma_load_2d(dst, &map_x, g * kGroup, m0, &bars->full[s]);
+              tma_load_2d(dst + Shape::kABytes, &map_w, g * kGroup, n0, &bars->full[s]);
+            }
+          }
+          __syncwarp();
         }
-        if (leader) {
-          mbar_arrive_expect_tx(&bars->full[s], kStageBytes);
-          tma_load_2d(at + s * kStageBytes, &map_x, g * kGroup, m0, &bars->full[s]);
-          tma_load_2d(at + s * kStageBytes + Shape::kABytes, &map_w, g * kGroup, n0, &bars->full[s]);
+      }
+      // the copies issued land before either CTA leaves: the first one's barriers count them all, and what
+      // the products have consumed had landed
+      for (uint32_t j = i > kStages ? i - kStages : 0; j < i; ++j)
+        mbar_wait(rank == 0 ? &bars->full[j % kStages] : &bars->empty[j % kStages], (j / kStages) & 1, kLinearWaitError);
+    } else if (warp == kSumWarps + 1 || warp == kSumWarps + 2) {
+      // the first CTA issues, one warp per accumulator: a group's hand-over hides behind the other's
+      if (rank == 0) {
+        const bool leader = elect_one();
+        const uint32_t b = warp - kSumWarps - 1, d = tmem + b * 256;
+        const uint32_t idesc = umma_idesc(kCtas * kTileM, TN, 0, false);
+        const uint64_t x_desc = sw128_desc_k(smem_addr(smem)), w_desc = sw128_desc_k(smem_addr(smem) + Shape::kABytes);
+        const uint32_t mine = static_cast<uint32_t>((tiles - pair + pairs - 1) / pairs) * static_cast<uint32_t>(groups);
+        auto commit = [](uint64_t* bar) {
+          if (PAIR) pair_umma_commit(bar);
+          else umma_commit(bar);
+        };
+        for (uint32_t i = b; i < mine; i += 2) {
+          const uint32_t s = i % kStages;
+          if (i >= 2 && !warp_wait(&bars->sum_empty[b], ((i / 2) - 1) & 1, abort)) break;
+          if (!warp_wait(&bars->full[s], (i / kStages) & 1, abort)) break;
+          tc_fence_after();
+          if (leader) {
+            const uint64_t step = static_cast<uint64_t>(s * (kStageBytes / 16));
+#pragma unroll
+            for (int k = 0; k < kGroup / 32; ++k) {
+              if (PAIR) pair_umma_f8_ss(d, x_desc + step + 2 * k, w_desc + step + 2 * k, idesc, k > 0);
+              else umma_f8_ss(d, x_desc + step + 2 * k, w_desc + step + 2 * k, idesc, k > 0);
+            }
+            commit(&bars->sum_full[b]);
+            commit(&bars->empty[s]);
+          }
+          __syncwarp();
         }
+        if (leader) commit(&bars->drain);
         __syncwarp();
       }
+      mbar_wait(&bars->drain, 0, kLinearWaitError);  // in both CTAs: every product is complete
     }
-    for (uint32_t j = i > kStages ? i - kStages : 0; j < i; ++j)  // every copy issued lands before the CTA leaves
-      mbar_wait(&bars->full[j % kStages], (j / kStages) & 1, kLinearWaitError);
-  } else if (warp == kSumWarps + 1 || warp == kSumWarps + 2) {
-    // one warp per accumulator: a group's hand-over hides behind the other's
-    const bool leader = elect_one();
-    const uint32_t b = warp - kSumWarps - 1, d = tmem + b * 256;
-    const uint32_t idesc = umma_idesc(kTileM, TN, 0, false);
-    const uint64_t x_desc = sw128_desc_k(smem_addr(smem)), w_desc = sw128_desc_k(smem_addr(smem) + Shape::kABytes);
-    const uint32_t mine = (tiles - blockIdx.x + gridDim.x - 1) / gridDim.x * static_cast<uint32_t>(groups);  // groups of this CTA's tiles
-    for (uint32_t i = b; i < mine; i += 2) {
-      const uint32_t s = i % kStages;
-      if (i >= 2 && !warp_wait(&bars->sum_empty[b], ((i / 2) - 1) & 1, abort)) break;
-      if (!warp_wait(&bars->full[s], (i / kStages) & 1, abort)) break;
-      tc_fence_after();
-      if (leader) {
-        const uint64_t step = static_cast<uint64_t>(s * (kStageBytes / 16));
-#pragma unroll
-        for (int k = 0; k < kGroup / 32; ++k) umma_f8_ss(d, x_desc + step + 2 * k, w_desc + step + 2 * k, idesc, k > 0);
-        umma_commit(&bars->sum_full[b]);
-        umma_commit(&bars->empty[s]);
-      }
-      __syncwarp();
-    }
-    if (leader) umma_commit(&bars->drain);
-    __syncwarp();
-    mbar_wait(&bars->drain, 0, kLinearWaitError);
-  } else if (warp < kSumWarps) {
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     const int quad = warp % 4, half = warp / 4;
     const uint32_t from = tmem + (static_cast<uint32_t>(quad * kWarp) << 16) + half * kHalf;
+    const uint32_t empty_at = PAIR ? cluster_addr(&bars->sum_empty[0], 0) : 0;
     uint32_t i = 0;
     bool ok = true;
-    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-      const int64_t row = t % m_tiles * kTileM + quad * kWarp + lane;
+    for (int t = pair; t < tiles && ok; t += pairs) {
+      const int64_t row = (t % m_tiles * kCtas + rank) * kTileM + quad * kWarp + lane;
       const int64_t n0 = static_cast<int64_t>(t / m_tiles) * TN + half * kHalf;
       // the columns from `edge` (a multiple of 16) on belong to the next 128 of the weight's rows
       const int edge = static_cast<int>(128 - n0 % 128);
@@ -370,23 +408,38 @@ __global__ void __launch_bounds__(kTilesThreads, 1)
           break;
         }
         tc_fence_after();
+        // the next columns on their way while these are added; the accumulator is free once the last have left it
+        uint32_t d0[32], d1[32];
+        const uint32_t sums = from + b * 256;
+        auto add = [&](const uint32_t (&d)[32], int c) {
 #pragma unroll
-        for (int c = 0; c < kHalf; c += 32) {
-          uint32_t d[32];
-          const int width = kHalf - c < 32 ? 16 : 32;
-          if (width == 32) tmem_ld32(from + b * 256 + c, d);
-          else tmem_ld16(from + b * 256 + c, d);
+          for (int j = 0; j < 32; ++j)
+            if (c + j < kHalf) acc[(c + j) % kHalf] = fmaf(__uint_as_float(d[j]), c + j / 16 * 16 < edge ? f0 : f1, acc[(c + j) % kHalf]);
+        };
+        auto leave = [&] {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if (PAIR) cluster_arrive(empty_at + b * 8);
+            else mbar_arrive(&bars->sum_empty[b]);
+          }
+        };
+        tmem_ld32(sums, d0);
+        tmem_ld_wait();
+        tmem_ld32(sums + 32, d1);
+        add(d0, 0);
+        tmem_ld_wait();
+        tmem_ld32(sums + 64, d0);
+        add(d1, 32);
+        tmem_ld_wait();
+        if (kHalf > 112) tmem_ld32(sums + 96, d1);
+        else if (kHalf > 96) tmem_ld16(sums + 96, d1);
+        else leave();
+        add(d0, 64);
+        if (kHalf > 96) {
           tmem_ld_wait();
-          if (c + 32 >= kHalf) {  // the last columns have left the accumulator
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bars->sum_empty[b]);
-          }
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            if (j >= width) break;
-            acc[c + j] = fmaf(__uint_as_float(d[j]), c + j / 16 * 16 < edge ? f0 : f1, acc[c + j]);
-          }
+          leave();
+          add(d1, 96);
         }
       }
       if (!ok) break;
@@ -412,8 +465,12 @@ __global__ void __launch_bounds__(kTilesThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
+  if (PAIR) cluster_sync();  // nobody leaves while the other CTA may still signal or read here
   tc_fence_after();
-  if (warp == kSumWarps + 1) tmem_dealloc(tmem, 512);
+  if (warp == kSumWarps + 1) {
+    if (PAIR) pair_tmem_dealloc(tmem, 512);
+    else tmem_dealloc(tmem, 512);
+  }
 }
 
 // [rows][cols] bytes with a box of one group's columns and `box` rows, 128B-swizzled.
@@ -437,9 +494,9 @@ cudaError_t launch_rows(const LinearArgs& a, cudaStream_t stream) {
   if (!encode_codes(&mx, a.x, a.rows, a.cols, a.x_stride, NT) || !encode_codes(&mw, a.w, a.outs, a.cols, a.w_stride, 128))
     return cudaErrorInvalidValue;
   const int64_t tiles = ceil_div(a.outs, 128), groups = ceil_div(a.cols, kGroup), token_tiles = ceil_div(a.rows, NT);
-  // the largest cluster that keeps at least two groups per CTA and two CTAs per SM
+  // the largest cluster that keeps at least two groups per CTA and all CTAs resident at once
   int splits = 1;
-  while (splits < 8 && tiles * token_tiles * splits * 2 <= 2 * gemv_grid_ctas() && groups >= splits * 4) splits *= 2;
+  while (splits < 8 && tiles * token_tiles * splits * 2 <= RowsShape<NT>::kPerSm * gemv_grid_ctas() && groups >= splits * 4) splits *= 2;
   const int max_groups = static_cast<int>(ceil_div(groups, splits));
   auto kernel = linear_rows_kernel<O, NT>;
   const size_t smem = rows_smem<NT>(max_groups);
@@ -460,33 +517,47 @@ cudaError_t launch_rows(const LinearArgs& a, cudaStream_t stream) {
   return cudaLaunchKernelEx(&config, kernel, mx, mw, a, splits, max_groups);
 }
 
-template <typename O, int TN>
+template <typename O, int TN, bool PAIR>
 cudaError_t launch_tiles_n(const LinearArgs& a, cudaStream_t stream) {
+  constexpr int kCtas = PAIR ? 2 : 1;
   CUtensorMap mx, mw;
-  if (!encode_codes(&mx, a.x, a.rows, a.cols, a.x_stride, kTileM) || !encode_codes(&mw, a.w, a.outs, a.cols, a.w_stride, TN))
+  if (!encode_codes(&mx, a.x, a.rows, a.cols, a.x_stride, kTileM) || !encode_codes(&mw, a.w, a.outs, a.cols, a.w_stride, TN / kCtas))
     return cudaErrorInvalidValue;
-  auto kernel = linear_tiles_kernel<O, TN>;
-  constexpr int kSmem = static_cast<int>(tiles_smem<TN>());
+  auto kernel = linear_tiles_kernel<O, TN, PAIR>;
+  constexpr int kSmem = static_cast<int>(tiles_smem<TN, PAIR>());
   cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (err != cudaSuccess) return err;
-  const int64_t m_tiles = ceil_div(a.rows, kTileM), n_tiles = ceil_div(a.outs, TN);
+  const int64_t m_tiles = ceil_div(a.rows, kCtas * kTileM), n_tiles = ceil_div(a.outs, TN);
   if (m_tiles * n_tiles > INT32_MAX / 2) return cudaErrorInvalidValue;
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(m_tiles * n_tiles, gemv_grid_ctas()));
-  kernel<<<grid, kTilesThreads, kSmem, stream>>>(mx, mw, a, static_cast<int>(m_tiles), static_cast<int>(n_tiles));
-  return cudaGetLastError();
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(static_cast<unsigned>(kCtas * std::min<int64_t>(m_tiles * n_tiles, gemv_grid_ctas() / kCtas)));
+  config.blockDim = dim3(kTilesThreads);
+  config.dynamicSmemBytes = kSmem;
+  config.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = kCtas;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, kernel, mx, mw, a, static_cast<int>(m_tiles), static_cast<int>(n_tiles));
 }
 
-// The tile width whose rounds of all SMs cover the outputs with the least work:
-// 4000 x 7168 outputs are 896 tiles of 256 (7 rounds of 148, the last one all
-// but empty) or 1024 of 224 (7 rounds, each an eighth shorter).
+// The tiles whose rounds of all SMs cover the outputs with the least work:
+// 4000 x 7168 outputs are 448 tiles of a pair and 256 columns (7 rounds of 74
+// pairs, the last one all but empty) or 512 of 224 (7 rounds, each an eighth
+// shorter); 600 x 7168 are 140 tiles of one CTA and 256 (one round).  Narrower
+// tiles of one CTA were slower than a pair's (300 x 7168 x 2048: 22 us against 16).
 template <typename O>
 cudaError_t launch_tiles(const LinearArgs& a, cudaStream_t stream) {
-  auto cost = [&](int64_t tn) {
-    return ceil_div(ceil_div(a.rows, kTileM) * ceil_div(a.outs, tn), gemv_grid_ctas()) * tn;
+  auto cost = [&](int64_t tn, int64_t ctas) {
+    return ceil_div(ceil_div(a.rows, ctas * kTileM) * ceil_div(a.outs, tn), gemv_grid_ctas() / ctas) * tn;
   };
-  if (cost(224) < cost(256) && cost(224) <= cost(192)) return launch_tiles_n<O, 224>(a, stream);
-  if (cost(192) < cost(256)) return launch_tiles_n<O, 192>(a, stream);
-  return launch_tiles_n<O, 256>(a, stream);
+  const int64_t least = std::min({cost(256, 2), cost(224, 2), cost(192, 2), cost(256, 1)});
+  if (cost(256, 2) == least) return launch_tiles_n<O, 256, true>(a, stream);
+  if (cost(224, 2) == least) return launch_tiles_n<O, 224, true>(a, stream);
+  if (cost(192, 2) == least) return launch_tiles_n<O, 192, true>(a, stream);
+  return launch_tiles_n<O, 256, false>(a, stream);
 }
 
 template <typename O>
@@ -494,8 +565,10 @@ cudaError_t launch_linear(const LinearArgs& a, cudaStream_t stream) {
   if (a.rows <= 16) return launch_rows<O, 16>(a, stream);
   if (a.rows <= 32) return launch_rows<O, 32>(a, stream);
   if (a.rows <= 64) return launch_rows<O, 64>(a, stream);
-  // tiles once they fill half of the SMs, smaller and cut ones until then
-  if (ceil_div(a.rows, kTileM) * ceil_div(a.outs, 256) * 2 < gemv_grid_ctas()) return launch_rows<O, 128>(a, stream);
+  // weight streaming while its CTAs can still share a group range in twos: 128 x 7168 x 2048 12.5 us against 20.5 in
+  // tiles, 300 x 2112 x 7168 24.8 against 29.7; beyond that tiles: 600 x 2112 x 7168 30 against 43, 300 x 7168 x 7168
+  // 33 against 76
+  if (2 * ceil_div(a.rows, 128) * ceil_div(a.outs, 128) <= gemv_grid_ctas()) return launch_rows<O, 128>(a, stream);
   return launch_tiles<O>(a, stream);
 }
 
