@@ -197,8 +197,11 @@ cudaError_t launch_append_types(const AppendArgs& a, int x_dtype, int norm_dtype
 // the workspace, which the second kernel joins.  A range has at most two parts.
 //
 // Rows arrive by TMA, one box per run of positions that no page border cuts (the
-// largest power of two, up to 64, that divides the page size); runs of 64 bring
-// four chunks with one copy.  The scores of positions that do not take part are
+// largest power of two, up to 64, that divides the page size).  A copy costs the
+// issuing warp some 90 cycles, so full buffers take four chunks with each: runs
+// of 64 in the order [chunk][64 rows], shorter ones in blocks of 8 positions,
+// [8 rows of a chunk][4 chunks], an order that the operands' descriptors can
+// follow too (16-position pages: 17 copies of 8 rows instead of 68 of 16).  The scores of positions that do not take part are
 // masked; their rows of V must not hold a NaN all the same.  Runs without a
 // position, or on a page outside the cache, arrive as zeros, from coordinates
 // outside the tensor; the rows of a run behind the length that cuts it (whatever
@@ -253,7 +256,7 @@ struct AttnPlan {
   int workers;         // pairs of CTAs
   int run;             // positions per TMA box
   int shift, page_size;  // log2 of the page size where it has one, else -1
-  bool wide;           // boxes of four chunks: runs of 64, latent columns in whole chunks
+  bool wide;           // full buffers by boxes of four chunks, each of `run` (64 or 8) positions
   int groups;          // groups of 128 heads: an item is a row's group
 };
 
@@ -429,7 +432,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttnThreads, 1)
     const uint32_t buffers_at = smem_addr(buffers), q_at = smem_addr(q_smem), full_at = cluster_addr(&bars->full[0], 0);
     const int run = plan.run, runs = kHalfTile / run;
     const int outside = static_cast<int>(a.pages);  // a page that the cache does not have: zeros
-    const bool leader = elect_one(), wide = plan.wide;
+    const bool leader = elect_one(), wide = plan.wide, blocks = wide && run < kHalfTile;
     uint32_t g = 0, parts = 0;
     bool ok = true;
     // Where 64 positions lie: run `lane` (and lane + 32, where there are 64 runs of one position), its page as the
@@ -458,7 +461,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttnThreads, 1)
     // 64 positions of `n` chunks from the c-th on into dst
     auto copy = [&](uint32_t dst, const Half& r, int c, int n, uint32_t bar) {
       if (wide && n == 4) {
-        if (lane == 0) pair_tma_load_4d(dst, &map_wide, 0, r.row, c, known(r.page), bar);  // its run is the only one
+        if (lane < runs) pair_tma_load_4d(dst + lane * 4096, &map_wide, 0, r.row, c, known(r.page), bar);
         return;
       }
       const int page = known(r.page), page2 = known(r.page2);
@@ -493,8 +496,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttnThreads, 1)
       if (!warp_wait(own, cuts & 1, abort)) return false;
       ++cuts;
       unsigned char* at = buffers + first_chunk * kChunkBytes;
+      const bool in_blocks = blocks && n == 4;
+      const int chunk_bytes = in_blocks ? 1024 : kChunkBytes, atom_bytes = in_blocks ? 4096 : 1024;
       for (int row = r.dead + lane / 8; row < (r.dead + run - 1) / run * run; row += 4)
-        for (int k = 0; k < n; ++k) *reinterpret_cast<uint4*>(at + k * kChunkBytes + row * 128 + (lane % 8) * 16) = make_uint4(0, 0, 0, 0);
+        for (int k = 0; k < n; ++k)
+          *reinterpret_cast<uint4*>(at + k * chunk_bytes + row / 8 * atom_bytes + row % 8 * 128 + (lane % 8) * 16) = make_uint4(0, 0, 0, 0);
       fence_proxy_async_shared();
       __syncwarp();
       if (leader) cluster_arrive(bar);
@@ -543,9 +549,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttnThreads, 1)
       const int format = __is_same(T, __nv_bfloat16) ? 1 : 0;
       const uint32_t idesc_s = umma_idesc(kHeads, kTile, format, false), idesc_o = umma_idesc(kHeads, 256, format, true);
       const uint64_t q_desc = sw128_desc_k(smem_addr(q_smem)), p_desc = sw128_desc_k(smem_addr(p_smem));
-      const uint64_t k_desc = sw128_desc_k(smem_addr(buffers));
-      const uint64_t v_desc = sw128_desc(smem_addr(buffers) + kBufferChunk[3] * kChunkBytes, kChunkBytes);
+      // buffers in blocks of 8 positions, where they hold four chunks
+      const bool blocks = plan.wide && plan.run < kHalfTile, v_blocks = blocks && own_chunks == 4;
+      const uint64_t k_desc = sw128_desc_k(smem_addr(buffers)), block_desc = sw128_desc_k(smem_addr(buffers), 4096);
+      const uint32_t v_at = smem_addr(buffers) + kBufferChunk[3] * kChunkBytes;
+      const uint64_t v_desc = v_blocks ? sw128_desc(v_at, 1024, 4096) : sw128_desc(v_at, kChunkBytes);
       constexpr int kStep = kChunkBytes / 16;  // descriptors advance in units of 16 bytes
+      const int v_chunk = v_blocks ? 64 : kStep, v_step = v_blocks ? 2 * 4096 / 16 : 2 * 1024 / 16;  // the next chunk, 16 positions
       uint32_t g = 0, parts = 0;
       bool ok = true;
       // the scores of the tile whose number is t
@@ -557,8 +567,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttnThreads, 1)
           if (!warp_wait(&bars->full[i], t & 1, abort)) return false;
           tc_fence_after();
           if (leader) {
+            const bool in_blocks = blocks && n == 4;
+            const uint64_t k0 = (in_blocks ? block_desc : k_desc) + 4 * i * kStep;
+            const int k_chunk = in_blocks ? 64 : kStep;
             for (int c = 0; c < n; ++c) {
-              const uint64_t q = q_desc + (c0 + c) * kStep, k = k_desc + (kBufferChunk[0] + 4 * i + c) * kStep;
+              const uint64_t q = q_desc + (c0 + c) * kStep, k = k0 + c * k_chunk;
 #pragma unroll
               for (int j = 0; j < 4; ++j) pair_umma_f16_ss(d, q + 2 * j, k + 2 * j, idesc_s, i > 0 || c > 0 || j > 0);
             }
@@ -582,10 +595,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttnThreads, 1)
             tc_fence_after();
             if (leader) {
               for (int j = 0; j < v_pairs; ++j) {
-                const uint64_t pd = p_desc + h * kStep, v = v_desc + (4 * h + 2 * j) * kStep;
+                const uint64_t pd = p_desc + h * kStep, v = v_desc + 4 * h * kStep + 2 * j * v_chunk;
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                  pair_umma_f16_ss(tmem + kColO + j * 128, pd + 2 * k, v + k * (2048 / 16), idesc_o, i > 0 || h > 0 || k > 0);
+                  pair_umma_f16_ss(tmem + kColO + j * 128, pd + 2 * k, v + k * v_step, idesc_o, i > 0 || h > 0 || k > 0);
               }
               pair_umma_commit(&bars->empty[3 + h]);
               if (h == 1) pair_umma_commit(&bars->pv_done);
@@ -867,7 +880,9 @@ AttnPlan attn_plan(Plan& p, int64_t batch, int64_t heads, int64_t latent, int64_
   l.shift = -1;
   for (int i = 0; i < 31; ++i)
     if (page_size == int64_t(1) << i) l.shift = i;
-  l.wide = l.run == kHalfTile && latent % 64 == 0;
+  // four chunks at a time need whole chunks, and pay where there are four: up to 256 latent columns V has two
+  l.wide = l.run >= 8 && latent % 64 == 0 && latent > 256;
+  if (l.wide && l.run < kHalfTile) l.run = 8;
   l.part_o = p.take<float>(2 * l.workers * kHeads * latent);
   l.part_ml = p.take<float2>(2 * l.workers * kHeads);
   l.before = p.take<int64_t>(batch + 1);
@@ -918,7 +933,7 @@ cudaError_t launch_attention(const PagedAttnArgs& a, const AttnPlan& plan, cudaS
   if (!encode_rows<T>(&ql, a.q_latent, a.latent, a.heads, a.batch, a.ql_head_stride, a.ql_stride, kCtaHeads) ||
       !encode_rows<T>(&qp, a.q_pe, a.rope, a.heads, a.batch, a.qp_head_stride, a.qp_stride, kCtaHeads) ||
       !encode_rows<T>(&runs, a.cache, width, a.page_size, a.pages, a.row_stride, a.page_stride, plan.run) ||
-      (plan.wide && !encode_rows<T>(&wide, a.cache, width, a.page_size, a.pages, a.row_stride, a.page_stride, kHalfTile, a.latent / 64)))
+      (plan.wide && !encode_rows<T>(&wide, a.cache, width, a.page_size, a.pages, a.row_stride, a.page_stride, plan.run, a.latent / 64)))
     return cudaErrorInvalidValue;
   auto kernel = paged_attention_kernel<T>;
   cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kAttnSmem));

@@ -188,18 +188,18 @@ MOE_D void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint6
 
 // Shared-memory operand descriptors, 128B swizzle (rows of 128 bytes whose
 // 16-byte units are XORed with the row's index mod 8, atoms of 8 rows).
-// K-major: a row holds consecutive k; atoms of 8 rows of M or N are 1024
-// bytes apart.  MN-major: a row holds 64 16-bit values of consecutive N at
-// one k; `lead` bytes to the next 64 of N, 1024 bytes to the next 8 of k.
-MOE_D uint64_t sw128_desc(uint32_t saddr, uint32_t lead) {
+// K-major: a row holds consecutive k; atoms of 8 rows of M or N are `stride`
+// bytes apart (1024 where they follow one another).  MN-major: a row holds 64 16-bit values of consecutive N at
+// one k; `lead` bytes to the next 64 of N, `stride` to the next 8 of k.
+MOE_D uint64_t sw128_desc(uint32_t saddr, uint32_t lead, uint32_t stride = 1024) {
   uint64_t d = static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4);
   d |= static_cast<uint64_t>(lead >> 4) << 16;
-  d |= static_cast<uint64_t>(1024 >> 4) << 32;
+  d |= static_cast<uint64_t>(stride >> 4) << 32;
   d |= static_cast<uint64_t>(1) << 46;  // descriptor version of tcgen05
   d |= static_cast<uint64_t>(2) << 61;  // 128B swizzle
   return d;
 }
-MOE_D uint64_t sw128_desc_k(uint32_t saddr) { return sw128_desc(saddr, 16); }
+MOE_D uint64_t sw128_desc_k(uint32_t saddr, uint32_t stride = 1024) { return sw128_desc(saddr, 16, stride); }
 
 // Instruction descriptor: fp32 D, M x N; formats 0 = fp16 / e4m3, 1 = bf16.
 MOE_HD uint32_t umma_idesc(int m, int n, int format, bool b_mn_major) {

@@ -283,6 +283,15 @@ def test_attention_widths(latent, rope):
     _check_attn(out, lse, case)
 
 
+@pytest.mark.parametrize("latent", [256, 320, 384, 448, 512])
+@pytest.mark.parametrize("page", [2, 8, 16, 40, 64, 192])
+def test_attention_page_sizes(latent, page):
+    """Every way in which rows are copied: single rows, blocks of 8, runs of 64, whole and odd numbers of column chunks."""
+    case = _attn_case([300, 129, 0, 64], 70, latent, 64, page, bf16)
+    out, lse = serving.paged_mla_attention(*case[:5], softmax_scale=case[5], return_lse=True)
+    _check_attn(out, lse, case)
+
+
 @pytest.mark.parametrize("spread", [0.0, 40.0])
 def test_attention_flat_and_peaked(spread):
     """Equal scores, and scores of which one takes all (its maximum moving along the cache)."""
