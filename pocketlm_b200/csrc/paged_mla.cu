@@ -35,8 +35,15 @@ constexpr int kAppendVectors = 4;  // 8-value vectors of a latent row per lane: 
 struct Angles {
   float cos[4], sin[4];
 };
+template <bool VEC>
 MOE_D Angles angles_at(const float* cos, const float* sin, int c, int n) {
   Angles a;
+  if (VEC) {  // whole and aligned, like the values
+    const float4 k = __ldg(reinterpret_cast<const float4*>(cos + c / 2)), s = __ldg(reinterpret_cast<const float4*>(sin + c / 2));
+    a.cos[0] = k.x, a.cos[1] = k.y, a.cos[2] = k.z, a.cos[3] = k.w;
+    a.sin[0] = s.x, a.sin[1] = s.y, a.sin[2] = s.z, a.sin[3] = s.w;
+    return a;
+  }
 #pragma unroll
   for (int p = 0; p < 4; ++p) {
     a.cos[p] = 2 * p < n ? __ldg(cos + c / 2 + p) : 0.0f;
@@ -106,7 +113,7 @@ __global__ void __launch_bounds__(kAppendThreads + kWarp, 5) paged_append_kernel
       for (int c = 8 * lane; c < rope; c += 8 * kWarp) {
         const int n = min(rope - c, 8);
         load8<T, VEC>(src + latent + c, n, e[0]);
-        store8<C, VEC>(dst + latent + c, n, rotated<T, C>(e[0], angles_at(cos, sin, c, n)));
+        store8<C, VEC>(dst + latent + c, n, rotated<T, C>(e[0], angles_at<VEC>(cos, sin, c, n)));
       }
       continue;
     }
@@ -122,7 +129,7 @@ __global__ void __launch_bounds__(kAppendThreads + kWarp, 5) paged_append_kernel
         if (h + i * at_once < a.heads) load8<C, VEC>(q + (h + i * at_once) * a.q_head_stride, n, e[i]);
     };
     load(h0);  // before the angles, which wait for the position
-    const Angles turn = angles_at(cos, sin, c, n);
+    const Angles turn = angles_at<VEC>(cos, sin, c, n);
     for (int h = h0; h < a.heads; h += at_once * kAppendLoads) {
       if (h != h0) load(h);
 #pragma unroll
@@ -141,7 +148,7 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 template <typename T, typename W, typename C>
 cudaError_t launch_append(const AppendArgs& a, cudaStream_t stream) {
   auto whole = [](int64_t n, int64_t size) { return n * size % 16 == 0; };
-  const bool vec = a.latent % 8 == 0 && a.rope % 8 == 0 && aligned16(a.kv) && whole(a.kv_stride, sizeof(T)) &&
+  const bool vec = a.latent % 8 == 0 && a.rope % 8 == 0 && aligned16(a.cos) && aligned16(a.sin) && aligned16(a.kv) && whole(a.kv_stride, sizeof(T)) &&
                    aligned16(a.norm_w) && aligned16(a.cache) && whole(a.page_stride, sizeof(C)) &&
                    whole(a.row_stride, sizeof(C)) &&
                    (!a.q || (aligned16(a.q) && aligned16(a.q_out) && whole(a.q_stride, sizeof(C)) &&
