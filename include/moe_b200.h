@@ -605,7 +605,8 @@ int moe_fp8_block_linear(const uint8_t* x_codes, int64_t x_stride, const float* 
  * fp32.  A slot past the cache, or a row to store whose position is outside
  * the tables, is skipped and sets code 512 in moe_b200_device_error; queries
  * of such a position are written as zeros.  The slots of one call are
- * distinct (a slot given twice is left with an unspecified row). */
+ * distinct (a slot given twice is left with an unspecified row); the cache's
+ * rows do not overlap. */
 int moe_paged_mla_append(const void* kv_rows, int64_t kv_stride, int kv_dtype, const void* kv_norm_weight,
                          int norm_dtype, const int64_t* slots, const int64_t* positions, const float* rope_cos,
                          const float* rope_sin, int64_t table_rows, void* cache, int cache_dtype, int64_t pages,

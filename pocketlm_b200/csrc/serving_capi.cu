@@ -84,6 +84,10 @@ int moe_paged_mla_append(const void* kv_rows, int64_t kv_stride, int kv_dtype, c
       (norm_dtype != cache_dtype && norm_dtype != kDtypeF32))
     return fail(kUnsupported, "the cache is bf16 or fp16; rows and norm weight of the cache's type or fp32");
   if (kv_lora_rank > 1024 || qk_rope_dim > 1024 || heads > (1 << 20)) return fail(kUnsupported, "dimension too large");
+  // (a dimension of one has no stride)
+  const int64_t width = kv_lora_rank + qk_rope_dim;
+  if ((pages > 1 && page_stride < width) || (page_size > 1 && row_stride < width))
+    return fail(kUnsupported, "the cache's rows overlap");
   if (tokens == 0) return kOk;
   AppendArgs a{};
   a.kv = kv_rows; a.norm_w = kv_norm_weight; a.slots = slots; a.positions = positions; a.cos = rope_cos;
@@ -101,7 +105,8 @@ static int attention_supported(int64_t batch, int64_t heads, int64_t latent, int
     return fail(kBadDims, "bad dimensions");
   if (latent > 512 || latent % 8 || rope > 64 || rope % 8)
     return fail(kUnsupported, "kv_lora_rank up to 512 and qk_rope_dim up to 64, multiples of 8");
-  if (batch > 65535 || heads > (1 << 16) || batch * heads > INT32_MAX || table_cols > INT32_MAX / page_size)
+  // (positions, rounded up to whole tiles, stay inside 32 bits)
+  if (batch > 65535 || heads > (1 << 16) || batch * heads > INT32_MAX || table_cols > (INT32_MAX - 256) / page_size)
     return fail(kUnsupported, "dimension too large");
   return kOk;
 }
@@ -122,6 +127,7 @@ int moe_paged_mla_attention(const void* q_latent, int64_t ql_stride, int64_t ql_
   const int code = attention_supported(batch, heads, kv_lora_rank, qk_rope_dim, table_cols, page_size);
   if (code != kOk) return code;
   if (pages <= 0) return fail(kBadDims, "bad dimensions");
+  if (pages >= INT32_MAX) return fail(kUnsupported, "dimension too large");
   if (!is_16bit(dtype)) return fail(kUnsupported, "queries and cache are bf16 or fp16");
   if (!(softmax_scale >= 0.0f) || softmax_scale > 3.0e38f) return fail(kBadDims, "softmax_scale must be finite and not negative");
   if (((reinterpret_cast<uintptr_t>(q_latent) | reinterpret_cast<uintptr_t>(q_pe) | reinterpret_cast<uintptr_t>(cache) |

@@ -106,6 +106,7 @@ def test_entry_point_codes():
     f = lib.moe_paged_mla_append
     assert f(*_args(append)) == 0 and f(*_args(append, qo=None)) == -1 and f(*_args(append, sl=None)) == -1
     assert f(*_args(append, rope=15)) == -2 and f(*_args(append, pages=0)) == -2 and f(*_args(append, heads=0)) == -2
+    assert f(*_args(append, pst=0)) == -5 and f(*_args(append, rst=79)) == -5  # tokens would share a row's memory
     assert f(*_args(append, cd=0)) == -5 and f(*_args(append, kd=2)) == -5 and f(*_args(append, latent=2048)) == -5
     attn = dict(ql=FAKE, qls=192, qlh=64, qp=FAKE, qps=48, qph=16, ca=FAKE, dt=1, pages=4, ps=8, pst=640, rst=80, t=FAKE, ts=2, tc=2, le=FAKE,
                 batch=0, heads=3, latent=64, rope=16, sc=0.1, out=FAKE, lse=None, ws=None, wb=0, st=None)
@@ -114,6 +115,8 @@ def test_entry_point_codes():
     assert f(*_args(attn, tc=0)) == -2 and f(*_args(attn, sc=-1.0)) == -2 and f(*_args(attn, sc=float("nan"))) == -2
     assert f(*_args(attn, latent=520)) == -5 and f(*_args(attn, rope=72)) == -5 and f(*_args(attn, latent=60)) == -5
     assert f(*_args(attn, rst=81)) == -5 and f(*_args(attn, dt=0)) == -5 and f(*_args(attn, batch=70000)) == -5
-    assert f(*_args(attn, ca=ctypes.c_void_p(0x1002))) == -5
+    assert f(*_args(attn, ca=ctypes.c_void_p(0x1002))) == -5 and f(*_args(attn, ws=ctypes.c_void_p(0x1010), wb=1 << 30)) == -5
+    assert f(*_args(attn, batch=2, qls=0)) == -5 and f(*_args(attn, batch=2, pst=0)) == -5
+    assert f(*_args(attn, tc=1 << 20, ps=1 << 11)) == -5 and f(*_args(attn, pages=(1 << 31) - 1)) == -5  # positions and pages past 32 bits
     assert lib.moe_paged_mla_attention_workspace_bytes(2, 3, 520, 16, 2, 8) == -1
     assert lib.moe_paged_mla_attention_workspace_bytes(2, 3, 64, 16, 2, 8) >= 0
