@@ -12,11 +12,15 @@
 // are M (128 of them per CTA), the tokens N (16 to 128), so no tensor work is
 // spent on absent tokens; the groups are cut over the CTAs of a cluster, whose
 // sums are added through distributed shared memory in rank order (the same
-// result on every run).
+// result on every run).  Measured: 64 x 24576 x 1536 14.4 us (41 MB, 2.8 TB/s),
+// 1 x 2112 x 7168 7.1 us: the launch, the first bytes' latency and the cluster's
+// sum are most of so short a call.
 //
 // Many rows (linear_tiles_kernel): the tensor cores bound it.  256 tokens x up
 // to 256 outputs per pair of CTAs and tile, two accumulators so that the sums
-// of one group are read while the next is computed; persistent.
+// of one group are read while the next is computed; persistent.  Measured:
+// 4000 x 7168 x 16384 458 us, 2.05 PFLOP/s.  Its groups' sums bound it: 256 x 256
+// fp32 values leave tensor memory for every 520 cycles of products.
 #include <algorithm>
 
 #include "fp8_gemv.cuh"
@@ -55,7 +59,6 @@ struct RowsBarriers {
   uint32_t tmem_base;
   int abort;
 };
-
 
 template <int NT>
 size_t rows_smem(int groups) {
@@ -494,7 +497,8 @@ cudaError_t launch_rows(const LinearArgs& a, cudaStream_t stream) {
   if (!encode_codes(&mx, a.x, a.rows, a.cols, a.x_stride, NT) || !encode_codes(&mw, a.w, a.outs, a.cols, a.w_stride, 128))
     return cudaErrorInvalidValue;
   const int64_t tiles = ceil_div(a.outs, 128), groups = ceil_div(a.cols, kGroup), token_tiles = ceil_div(a.rows, NT);
-  // the largest cluster that keeps at least two groups per CTA and all CTAs resident at once
+  // the largest cluster that keeps at least two groups per CTA and all CTAs resident at once (1 x 576 x 1536,
+  // 12 groups: clusters of eight 4.7 us, of four, as here, 4.7, of two 5.6)
   int splits = 1;
   while (splits < 8 && tiles * token_tiles * splits * 2 <= RowsShape<NT>::kPerSm * gemv_grid_ctas() && groups >= splits * 4) splits *= 2;
   const int max_groups = static_cast<int>(ceil_div(groups, splits));

@@ -7,7 +7,8 @@
 // are rotated by the same angles.  rot turns the pairs (2p, 2p + 1) by
 // (cos[position, p], sin[position, p]).  fp32 throughout, one rounding to the
 // stored type.  Bytes bound it: every value is read once and written once; a
-// warp takes a token's cache row or 256 of its query values.
+// warp takes a token's cache row or 256 of its query values.  Measured with 128
+// heads: 4096 tokens 35 us (145 MB, 4.1 TB/s), 32 tokens 3.6 us.
 //
 // Attention.  score[l] = scale (q_latent . c[l] + q_pe . r[l]) over the row's
 // first `length` positions, position l in page table[l / page_size];
@@ -208,18 +209,24 @@ cudaError_t launch_append_types(const AppendArgs& a, int x_dtype, int norm_dtype
 // issuing warp some 90 cycles, so full buffers take four chunks with each: runs
 // of 64 in the order [chunk][64 rows], shorter ones in blocks of 8 positions,
 // [8 rows of a chunk][4 chunks], an order that the operands' descriptors can
-// follow too (16-position pages: 17 copies of 8 rows instead of 68 of 16).  The scores of positions that do not take part are
-// masked; their rows of V must not hold a NaN all the same.  Runs without a
-// position, or on a page outside the cache, arrive as zeros, from coordinates
-// outside the tensor; the rows of a run behind the length that cuts it (whatever
-// their memory holds) are cleared in shared memory before the products may read.
-// K is asked into L2 two tiles ahead: a buffer's reload would otherwise show
-// memory's latency in every tile.
+// follow too (128 rows of 16 heads on 16-position pages: 90 us with 8-row blocks,
+// 113 with a copy per chunk and 16 rows).  The scores of positions that do not
+// take part are masked; their rows of V must not hold a NaN all the same.  Runs
+// without a position, or on a page outside the cache, arrive as zeros, from
+// coordinates outside the tensor; the rows of a run behind the length that cuts
+// it (whatever their memory holds) are cleared in shared memory before the
+// products may read.
 //
 // Warps 0-3: softmax, result.  4: copies of queries and K.  5, 6: copies of V's
 // halves.  7: tensor memory and, in the first CTA, the products (the whole warp
 // walks the work, so that operand descriptors stay in uniform registers; one
 // lane issues).
+//
+// Measured, bf16: 64 rows of 128 heads and up to 8192 positions 105 us (393 MB,
+// 3.7 TB/s; 91 GFLOP, 0.86 PFLOP/s): a tile of a pair takes some 2970 cycles, of
+// which its products keep the tensor cores 51 % busy, and the parts' results and
+// their join some 15 us at the end.  One row of 4096 positions 18.6 us: launches,
+// two tiles per pair, and the join of its parts.
 constexpr int kTile = 128, kHalfTile = 64;
 constexpr int kHeads = 128, kCtaHeads = 64;
 constexpr int kChunkBytes = 64 * 128;
@@ -787,7 +794,9 @@ MOE_D void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: 
 // positions.  A CTA takes kJoinHeads heads of a row (of one group), a thread four
 // columns of each; the parts' weights first, all at once, then their columns
 // with eight loads in flight: eight heads' where there are many rows, each cut
-// into two or three parts, and eight parts of one head where there are few.
+// into two or three parts (64 rows of 128 heads and 4096 positions 72 us against
+// 80), and eight parts of one head where there are few (one row 18.5 us against
+// 28.7, 16 rows 36.5 against 38.8).
 constexpr int kJoinThreads = 128, kMostWorkers = 128;
 template <typename T, int kJoinHeads>
 __global__ void __launch_bounds__(kJoinThreads) paged_attention_join_kernel(PagedAttnArgs a, AttnPlan plan) {
