@@ -8,7 +8,7 @@
 // (cos[position, p], sin[position, p]).  fp32 throughout, one rounding to the
 // stored type.  Bytes bound it: every value is read once and written once; a
 // warp takes a token's cache row or 256 of its query values.  Measured with 128
-// heads: 4096 tokens 35 us (145 MB, 4.1 TB/s), 32 tokens 3.6 us.
+// heads: 4096 tokens 26.4 us (145 MB, 5.5 TB/s), 32 tokens 2.7 us.
 //
 // Attention.  score[l] = scale (q_latent . c[l] + q_pe . r[l]) over the row's
 // first `length` positions, position l in page table[l / page_size];
@@ -64,37 +64,42 @@ MOE_D Eight<C> rotated(const Eight<T>& e, const Angles& a) {
   return r;
 }
 
-// A CTA per token (and step): its last warp the cache row, the others the
-// queries: a thread keeps its eight columns of a head, and their angles, over
-// the heads that it takes, kAppendLoads of them in flight.
-constexpr int kAppendLoads = 4;
+// A CTA takes tokens in turn: its last warp the cache rows, the others the
+// queries: a thread keeps its eight columns of a head, and their angles, over the
+// heads that it takes, kAppendLoads of them in flight, and asks for the next
+// token's first ones before it turns this token's.  Three CTAs per SM: 4096
+// tokens of 128 heads 26.4 us; four, where registers run short, 34, two 31, and a
+// CTA per token without the loads ahead 35.
+constexpr int kAppendLoads = 4, kAppendCtas = 3;
 template <typename T, typename W, typename C, bool VEC>
-__global__ void __launch_bounds__(kAppendThreads + kWarp, 5) paged_append_kernel(AppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads + kWarp, kAppendCtas) paged_append_kernel(AppendArgs a) {
   const int tid = threadIdx.x, q_threads = blockDim.x - kWarp, lane = tid % kWarp;
   const int latent = static_cast<int>(a.latent), rope = static_cast<int>(a.rope);
-  for (int64_t t = blockIdx.x; t < a.tokens; t += gridDim.x) {
-    const int64_t pos = a.positions[t];
-    const bool placed = pos >= 0 && pos < a.table_rows;
-    const float* cos = a.cos + (placed ? pos : 0) * (rope / 2);
-    const float* sin = a.sin + (placed ? pos : 0) * (rope / 2);
-    if (tid >= q_threads) {
-      const int64_t slot = a.slots[t];
-      if (slot < 0) continue;
-      if (!placed || slot >= a.pages * a.page_size) {
-        if (lane == 0) atomicOr(&g_device_error, kPagedRangeError);
-        continue;
-      }
+  auto in_table = [&](int64_t pos) { return pos >= 0 && pos < a.table_rows; };
+  if (tid >= q_threads) {
+    for (int64_t t = blockIdx.x; t < a.tokens; t += gridDim.x) {
       const T* src = static_cast<const T*>(a.kv) + t * a.kv_stride;
-      const int64_t page = slot / a.page_size;
-      C* dst = static_cast<C*>(a.cache) + page * a.page_stride + (slot - page * a.page_size) * a.row_stride;
-      Eight<T> e[kAppendVectors];
-      float ss = 0.0f;
+      const int64_t pos = a.positions[t], slot = a.slots[t];
+      Eight<T> e[kAppendVectors], r;
+      const int r_col = 8 * lane, r_n = min(rope - r_col, 8);
+      clear8(r);
+      if (r_n > 0) load8<T, VEC>(src + latent + r_col, r_n, r);
 #pragma unroll
       for (int v = 0; v < kAppendVectors; ++v) {
         const int c = 8 * (lane + v * kWarp), n = min(latent - c, 8);
         clear8(e[v]);
         if (n > 0) load8<T, VEC>(src + c, n, e[v]);
       }
+      if (slot < 0) continue;
+      if (!in_table(pos) || slot >= a.pages * a.page_size) {
+        if (lane == 0) atomicOr(&g_device_error, kPagedRangeError);
+        continue;
+      }
+      const float* cos = a.cos + pos * (rope / 2);
+      const float* sin = a.sin + pos * (rope / 2);
+      const int64_t page = slot / a.page_size;
+      C* dst = static_cast<C*>(a.cache) + page * a.page_stride + (slot - page * a.page_size) * a.row_stride;
+      float ss = 0.0f;
 #pragma unroll
       for (int v = 0; v < kAppendVectors; ++v)
 #pragma unroll
@@ -111,28 +116,38 @@ __global__ void __launch_bounds__(kAppendThreads + kWarp, 5) paged_append_kernel
         for (int j = 0; j < 8; ++j) o.v[j] = from_float<C>(widen<T>(e[v].v[j]) * inv * widen<W>(w.v[j]));
         store8<C, VEC>(dst + c, n, o);
       }
-      for (int c = 8 * lane; c < rope; c += 8 * kWarp) {
-        const int n = min(rope - c, 8);
-        load8<T, VEC>(src + latent + c, n, e[0]);
-        store8<C, VEC>(dst + latent + c, n, rotated<T, C>(e[0], angles_at<VEC>(cos, sin, c, n)));
+      for (int c = r_col, n = r_n; n > 0;) {
+        store8<C, VEC>(dst + latent + c, n, rotated<T, C>(r, angles_at<VEC>(cos, sin, c, n)));
+        c += 8 * kWarp;
+        n = min(rope - c, 8);
+        if (n > 0) load8<T, VEC>(src + latent + c, n, r);
       }
-      continue;
     }
-    const int per_head = (rope + 7) / 8, at_once = q_threads / per_head;  // heads at once
-    if (tid >= at_once * per_head) continue;
-    const int h0 = tid / per_head, c = 8 * (tid - h0 * per_head), n = min(rope - c, 8);
+    return;
+  }
+  const int per_head = (rope + 7) / 8, at_once = q_threads / per_head;  // heads at once
+  if (tid >= at_once * per_head) return;
+  const int h0 = tid / per_head, c = 8 * (tid - h0 * per_head), n = min(rope - c, 8);
+  auto load = [&](int64_t t, int h, Eight<C> (&e)[kAppendLoads]) {
     const C* q = static_cast<const C*>(a.q) + t * a.q_stride + c;
-    C* out = static_cast<C*>(a.q_out) + t * a.heads * rope + c;
-    Eight<C> e[kAppendLoads];
-    auto load = [&](int h) {
 #pragma unroll
-      for (int i = 0; i < kAppendLoads; ++i)
-        if (h + i * at_once < a.heads) load8<C, VEC>(q + (h + i * at_once) * a.q_head_stride, n, e[i]);
-    };
-    load(h0);  // before the angles, which wait for the position
-    const Angles turn = angles_at<VEC>(cos, sin, c, n);
+    for (int i = 0; i < kAppendLoads; ++i)
+      if (h + i * at_once < a.heads) load8<C, VEC>(q + (h + i * at_once) * a.q_head_stride, n, e[i]);
+  };
+  Eight<C> e[kAppendLoads], ahead[kAppendLoads];
+  int64_t t = blockIdx.x, pos = a.positions[t], pos_ahead = 0;
+  load(t, h0, e);  // before the angles, which wait for the position
+  for (; t < a.tokens; t += gridDim.x) {
+    const bool placed = in_table(pos);
+    const int64_t row = (placed ? pos : 0) * (rope / 2);
+    const Angles turn = angles_at<VEC>(a.cos + row, a.sin + row, c, n);
+    if (t + gridDim.x < a.tokens) {
+      pos_ahead = a.positions[t + gridDim.x];
+      load(t + gridDim.x, h0, ahead);
+    }
+    C* out = static_cast<C*>(a.q_out) + t * a.heads * rope + c;
     for (int h = h0; h < a.heads; h += at_once * kAppendLoads) {
-      if (h != h0) load(h);
+      if (h != h0) load(t, h, e);
 #pragma unroll
       for (int i = 0; i < kAppendLoads; ++i) {
         if (h + i * at_once >= a.heads) break;
@@ -141,6 +156,9 @@ __global__ void __launch_bounds__(kAppendThreads + kWarp, 5) paged_append_kernel
         store8<C, VEC>(out + (h + i * at_once) * rope, n, o);
       }
     }
+    pos = pos_ahead;
+#pragma unroll
+    for (int i = 0; i < kAppendLoads; ++i) e[i] = ahead[i];
   }
 }
 
@@ -156,7 +174,7 @@ cudaError_t launch_append(const AppendArgs& a, cudaStream_t stream) {
                              whole(a.q_head_stride, sizeof(C))));
   const int64_t vectors = a.q ? a.heads * ceil_div(a.rope, 8) : 0;
   const int threads = static_cast<int>(std::min<int64_t>(ceil_div(vectors, kWarp) * kWarp, kAppendThreads)) + kWarp;
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(a.tokens, INT32_MAX));
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(a.tokens, kAppendCtas * gemv_grid_ctas()));
   if (vec) paged_append_kernel<T, W, C, true><<<grid, threads, 0, stream>>>(a);
   else paged_append_kernel<T, W, C, false><<<grid, threads, 0, stream>>>(a);
   return cudaGetLastError();
