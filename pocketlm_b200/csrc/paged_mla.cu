@@ -240,11 +240,11 @@ cudaError_t launch_append_types(const AppendArgs& a, int x_dtype, int norm_dtype
 // walks the work, so that operand descriptors stay in uniform registers; one
 // lane issues).
 //
-// Measured, bf16: 64 rows of 128 heads and up to 8192 positions 105 us (393 MB,
-// 3.7 TB/s; 91 GFLOP, 0.86 PFLOP/s): a tile of a pair takes some 2970 cycles, of
+// Measured, bf16: 64 rows of 128 heads and up to 8192 positions 102 us (393 MB,
+// 3.9 TB/s; 91 GFLOP, 0.89 PFLOP/s): a tile of a pair takes some 2970 cycles, of
 // which its products keep the tensor cores 51 % busy, and the parts' results and
-// their join some 15 us at the end.  One row of 4096 positions 18.6 us: launches,
-// two tiles per pair, and the join of its parts.
+// their join some 12 us.  One row of 4096 positions 16.7 us: launches, two tiles
+// per pair, and the join of its parts.
 constexpr int kTile = 128, kHalfTile = 64;
 constexpr int kHeads = 128, kCtaHeads = 64;
 constexpr int kChunkBytes = 64 * 128;
@@ -257,7 +257,7 @@ constexpr int kSoftmaxWarps = 4, kSoftmaxThreads = kSoftmaxWarps * kWarp;
 constexpr int kKeysWarp = 4, kValuesWarp = 5, kProductsWarp = 7;
 constexpr int kAttnWarps = 8, kAttnThreads = kAttnWarps * kWarp;
 constexpr uint32_t kColO = 0, kColS = 256;
-constexpr int kMinTiles = 2;  // fewest tiles worth a range of their own: one row of 4096 positions 18.6 us (1: 19.1, 4: 20.9)
+constexpr int kMinTiles = 2;  // fewest tiles worth a range of their own: one row of 4096 positions 16.7 us, 1 would take 17.9
 constexpr float kMovesBy = 8.0f;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -282,7 +282,7 @@ constexpr size_t kAttnSmem = 1024 + static_cast<size_t>(kQChunks + kBufferChunks
 static_assert(kAttnSmem <= 232448, "shared memory per block");
 
 struct AttnPlan {
-  float* part_o;       // [2 workers][128 heads][latent]: unnormalised
+  float* part_o;       // [2 workers][latent / 8][128 heads][8]: unnormalised; a warp stores 32 heads' sectors side by side
   float2* part_ml;     // [2 workers][128 heads]: reference maximum (log2 domain), sum
   int64_t* before;     // [batch + 1]: tiles before each row
   int workers;         // pairs of CTAs
@@ -761,7 +761,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttnThreads, 1)
       const bool has = row < a.heads - p.group * kHeads;
       T* out = static_cast<T*>(a.out) + (p.b * a.heads + p.group * kHeads + row) * latent;
       const bool sectors = latent % 16 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 31u) == 0;
-      float* part = plan.part_o + (static_cast<int64_t>(p.slot) * kHeads + row) * latent;
+      float* part = plan.part_o + static_cast<int64_t>(p.slot) * kHeads * latent + row * 8;
       for (int c = 0; c < own_chunks; ++c) {  // 64 columns
         const int col0 = (part_of * own_chunks + c) * 64;
         if (col0 >= latent) break;
@@ -774,8 +774,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttnThreads, 1)
         for (int j = 0; j < 64; j += 16) {
           if (col0 + j >= latent) break;
           if (!p.whole) {
-            store_sector(part + col0 + j, o + j);
-            if (col0 + j + 8 < latent) store_sector(part + col0 + j + 8, o + j + 8);
+            store_sector(part + (col0 + j) * kHeads, o + j);
+            if (col0 + j + 8 < latent) store_sector(part + (col0 + j + 8) * kHeads, o + j + 8);
             continue;
           }
           uint32_t v[8];
@@ -809,12 +809,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttnThreads, 1)
 MOE_D void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // Joins the parts of the rows that were cut, and writes the rows without
-// positions.  A CTA takes kJoinHeads heads of a row (of one group), a thread four
-// columns of each; the parts' weights first, all at once, then their columns
-// with eight loads in flight: eight heads' where there are many rows, each cut
-// into two or three parts (64 rows of 128 heads and 4096 positions 72 us against
-// 80), and eight parts of one head where there are few (one row 18.5 us against
-// 28.7, 16 rows 36.5 against 38.8).
+// positions.  A CTA takes kJoinHeads heads of a row (of one group), a thread one
+// of them and half of every (64 / kJoinHeads)-th block of eight columns; the
+// parts' weights first, all at once, then their columns with eight loads in
+// flight: four blocks of two parts and four heads where there are many rows,
+// each cut into two or three parts (64 rows of 128 heads and 4096 positions
+// 67.5 us against 75.7 with one head per CTA, 24 rows 36.7 against 40.0), and eight
+// parts of one head where there are few (one row 16.7 us against 21.2, 4 rows
+// 23.0 against 26.8; 16 rows 33.5 against 32.5).
 constexpr int kJoinThreads = 128, kMostWorkers = 128;
 template <typename T, int kJoinHeads>
 __global__ void __launch_bounds__(kJoinThreads) paged_attention_join_kernel(PagedAttnArgs a, AttnPlan plan) {
@@ -822,16 +824,17 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attention_join_kernel(Page
   const int per_row = static_cast<int>(ceil_div(a.heads, kJoinHeads));
   const int64_t b = blockIdx.x / per_row, h0 = static_cast<int64_t>(blockIdx.x - b * per_row) * kJoinHeads;
   const int heads = static_cast<int>(min(a.heads - h0, static_cast<int64_t>(kJoinHeads)));
-  const int lane = threadIdx.x % kWarp, warp = threadIdx.x / kWarp, c = 4 * threadIdx.x;
-  const bool in = c < a.latent;
+  const int lane = threadIdx.x % kWarp, warp = threadIdx.x / kWarp;
+  constexpr int kBlocks = kJoinThreads / 2 / kJoinHeads;  // of eight columns, at once
+  const int head = threadIdx.x / 2 % kJoinHeads, c0 = threadIdx.x / (2 * kJoinHeads) * 8 + threadIdx.x % 2 * 4;
+  auto in = [&](int i) { return head < heads && c0 + i * kBlocks * 8 < a.latent; };
   wait_for_previous_kernel();
   const int64_t total = plan.before[a.batch], first = plan.before[b], next = plan.before[b + 1];
-  T* out = static_cast<T*>(a.out) + (b * a.heads + h0) * a.latent + c;
+  T* out = static_cast<T*>(a.out) + (b * a.heads + h0 + head) * a.latent + c0;
   if (first == next) {
-    for (int h = 0; h < heads; ++h) {
-      if (in) *reinterpret_cast<uint2*>(out + h * a.latent) = make_uint2(0, 0);
-      if (a.lse && c == 0) a.lse[b * a.heads + h0 + h] = -INFINITY;
-    }
+    for (int i = 0; i < kJoinHeads; ++i)
+      if (in(i)) *reinterpret_cast<uint2*>(out + i * kBlocks * 8) = make_uint2(0, 0);
+    if (a.lse && threadIdx.x < heads) a.lse[b * a.heads + h0 + threadIdx.x] = -INFINITY;
     return;
   }
   const int64_t workers = used_workers(total, plan.workers), group = h0 / kHeads, tiles = (next - first) / plan.groups;
@@ -840,14 +843,14 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attention_join_kernel(Page
   if (w0 == w1) return;  // finished where it was computed
   // the first part is its range's last, the others open theirs
   const int64_t row0 = h0 - group * kHeads;
-  auto at = [&](int w) { return (2 * static_cast<int64_t>(w) + (w == w0 ? 1 : 0)) * kHeads + row0; };
+  auto slot = [&](int w) { return (2 * static_cast<int64_t>(w) + (w == w0 ? 1 : 0)) * kHeads; };
   for (int h = warp; h < heads; h += kJoinThreads / kWarp) {
     float2 ml[kMostWorkers / kWarp];
     float top = -INFINITY, sum = 0.0f;
 #pragma unroll
     for (int k = 0; k < kMostWorkers / kWarp; ++k) {
       const int w = w0 + k * kWarp + lane;
-      ml[k] = w <= w1 ? plan.part_ml[at(w) + h] : make_float2(-INFINITY, 0.0f);
+      ml[k] = w <= w1 ? plan.part_ml[slot(w) + row0 + h] : make_float2(-INFINITY, 0.0f);
       top = fmaxf(top, ml[k].x);
     }
 #pragma unroll
@@ -866,38 +869,36 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attention_join_kernel(Page
     }
   }
   __syncthreads();
-  float4 acc[kJoinHeads];
+  float4 acc[kJoinHeads];  // of the thread's blocks
 #pragma unroll
-  for (int h = 0; h < kJoinHeads; ++h) acc[h] = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (in) {
-    constexpr int kAtOnce = 8 / kJoinHeads;  // parts
-    for (int w = w0; w <= w1; w += kAtOnce) {
-      float4 o[kAtOnce][kJoinHeads];
+  for (int i = 0; i < kJoinHeads; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  constexpr int kAtOnce = 8 / kJoinHeads;  // parts
+  const int64_t from = static_cast<int64_t>(c0 / 8) * kHeads * 8 + (row0 + head) * 8 + c0 % 8;
+  for (int w = w0; w <= w1; w += kAtOnce) {
+    float4 o[kAtOnce][kJoinHeads];
 #pragma unroll
-      for (int k = 0; k < kAtOnce; ++k)
+    for (int k = 0; k < kAtOnce; ++k)
 #pragma unroll
-        for (int h = 0; h < kJoinHeads; ++h)
-          o[k][h] = h < heads && w + k <= w1 ? __ldcg(reinterpret_cast<const float4*>(plan.part_o + (at(w + k) + h) * a.latent + c))
-                                             : make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int i = 0; i < kJoinHeads; ++i)
+        o[k][i] = w + k <= w1 && in(i) ? __ldcg(reinterpret_cast<const float4*>(plan.part_o + slot(w + k) * a.latent + from + i * kBlocks * 8 * kHeads))
+                                       : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int k = 0; k < kAtOnce; ++k)
+    for (int k = 0; k < kAtOnce; ++k) {
+      if (w + k > w1) break;
+      const float e = weight[head][w + k - w0];
 #pragma unroll
-        for (int h = 0; h < kJoinHeads; ++h) {
-          if (h >= heads || w + k > w1) break;
-          const float e = weight[h][w + k - w0];
-          acc[h].x = fmaf(o[k][h].x, e, acc[h].x);
-          acc[h].y = fmaf(o[k][h].y, e, acc[h].y);
-          acc[h].z = fmaf(o[k][h].z, e, acc[h].z);
-          acc[h].w = fmaf(o[k][h].w, e, acc[h].w);
-        }
-    }
-#pragma unroll
-    for (int h = 0; h < kJoinHeads; ++h) {
-      if (h >= heads) break;
-      const float inv = total_of[h] == 0.0f ? 0.0f : 1.0f / total_of[h];
-      *reinterpret_cast<uint2*>(out + h * a.latent) = make_uint2(pack2<T>(acc[h].x * inv, acc[h].y * inv), pack2<T>(acc[h].z * inv, acc[h].w * inv));
+      for (int i = 0; i < kJoinHeads; ++i) {
+        acc[i].x = fmaf(o[k][i].x, e, acc[i].x);
+        acc[i].y = fmaf(o[k][i].y, e, acc[i].y);
+        acc[i].z = fmaf(o[k][i].z, e, acc[i].z);
+        acc[i].w = fmaf(o[k][i].w, e, acc[i].w);
+      }
     }
   }
+  const float inv = total_of[head] == 0.0f ? 0.0f : 1.0f / total_of[head];
+#pragma unroll
+  for (int i = 0; i < kJoinHeads; ++i)
+    if (in(i)) *reinterpret_cast<uint2*>(out + i * kBlocks * 8) = make_uint2(pack2<T>(acc[i].x * inv, acc[i].y * inv), pack2<T>(acc[i].z * inv, acc[i].w * inv));
   if (a.lse && threadIdx.x < heads)
     a.lse[b * a.heads + h0 + threadIdx.x] =
         total_of[threadIdx.x] == 0.0f ? -INFINITY : (ref_of[threadIdx.x] + log2f(total_of[threadIdx.x])) * kLn2;
@@ -976,8 +977,8 @@ cudaError_t launch_attention(const PagedAttnArgs& a, const AttnPlan& plan, cudaS
   kernel<<<static_cast<unsigned>(2 * plan.workers), kAttnThreads, kAttnSmem, stream>>>(wide, runs, ql, qp, a, plan);
   err = cudaGetLastError();
   if (err != cudaSuccess) return err;
-  if (a.batch * a.heads >= 16 * gemv_grid_ctas())
-    return launch_dependent(paged_attention_join_kernel<T, 8>, static_cast<unsigned>(a.batch * ceil_div(a.heads, 8)), kJoinThreads, stream, a, plan);
+  if (a.batch * a.heads >= 12 * gemv_grid_ctas())
+    return launch_dependent(paged_attention_join_kernel<T, 4>, static_cast<unsigned>(a.batch * ceil_div(a.heads, 4)), kJoinThreads, stream, a, plan);
   return launch_dependent(paged_attention_join_kernel<T, 1>, static_cast<unsigned>(a.batch * a.heads), kJoinThreads, stream, a, plan);
 }
 
