@@ -12,8 +12,8 @@
 // are M (128 of them per CTA), the tokens N (16 to 128), so no tensor work is
 // spent on absent tokens; the groups are cut over the CTAs of a cluster, whose
 // sums are added through distributed shared memory in rank order (the same
-// result on every run).  Measured: 64 x 24576 x 1536 14.4 us (41 MB, 2.8 TB/s),
-// 1 x 2112 x 7168 7.1 us: the launch, the first bytes' latency and the cluster's
+// result on every run).  Measured: 64 x 24576 x 1536 12.7 us (41 MB, 3.2 TB/s),
+// 1 x 2112 x 7168 7.0 us: the launch, the first bytes' latency and the cluster's
 // sum are most of so short a call.
 //
 // Many rows (linear_tiles_kernel): the tensor cores bound it.  256 tokens x up
@@ -42,6 +42,7 @@ MOE_D bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
 
 constexpr int kRowsThreads = 192;  // warps 0-3: sums (a thread per weight row); 4: TMA; 5: products
 constexpr int kWTileBytes = 128 * kGroup;
+constexpr int kSumStride = 132;  // floats per token of a CTA's sums in shared memory: no bank is hit twice
 template <int NT>
 struct RowsShape {
   static constexpr int kStages = NT <= 32 ? 5 : NT <= 64 ? 4 : 6;
@@ -50,6 +51,7 @@ struct RowsShape {
   static constexpr int kCols = NT * kBufs < 32 ? 32 : NT * kBufs;
   static constexpr int kStageBytes = kWTileBytes + NT * kGroup;
   static constexpr int kPipeBytes = kStages * kStageBytes;
+  static_assert(NT * kSumStride * 4 <= kPipeBytes, "the sums take the pipeline's place");
 };
 template <int NT>
 struct RowsBarriers {
@@ -64,6 +66,12 @@ template <int NT>
 size_t rows_smem(int groups) {
   return 1024 + RowsShape<NT>::kPipeBytes + sizeof(float) * NT * groups + sizeof(RowsBarriers<NT>);
 }
+
+// Four bytes into shared memory, on their way until copies4_wait().
+MOE_D void copy4_async(float* dst, const float* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_addr(dst)), "l"(src) : "memory");
+}
+MOE_D void copies4_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 MOE_D float4 ld_cluster(const float* p, uint32_t rank) {
   const uint32_t at = cluster_addr(p, rank);
@@ -84,8 +92,8 @@ __global__ void __launch_bounds__(kRowsThreads) linear_rows_kernel(const __grid_
   using Shape = RowsShape<NT>;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* factor = reinterpret_cast<float*>(smem + Shape::kPipeBytes);  // [group][token]: the two scales' product
-  auto* bars = reinterpret_cast<RowsBarriers<NT>*>(factor + NT * max_groups);
+  float* scale = reinterpret_cast<float*>(smem + Shape::kPipeBytes);  // [group][token]
+  auto* bars = reinterpret_cast<RowsBarriers<NT>*>(scale + NT * max_groups);
   const int tid = threadIdx.x, lane = tid % kWarp, warp = __shfl_sync(0xFFFFFFFFu, tid / kWarp, 0);
   volatile int* abort = &bars->abort;
   const int rank = splits > 1 ? static_cast<int>(cluster_rank()) : 0;
@@ -115,9 +123,12 @@ __global__ void __launch_bounds__(kRowsThreads) linear_rows_kernel(const __grid_
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars->tmem_base;
-  float acc[NT];
+  // by 16 tokens and half of the warp's 32 weight rows, as tmem_ld16x16 gives them: four rows and NT / 4 tokens
+  // per thread, so that a group's scales are read from shared memory a quarter as often as with a row per thread
+  // (64 x 24576 x 1536: 12.7 us against 14.3)
+  float acc[NT / 16][2][8];
 #pragma unroll
-  for (int j = 0; j < NT; ++j) acc[j] = 0.0f;
+  for (int j = 0; j < NT; ++j) acc[j / 16][j / 8 % 2][j % 8] = 0.0f;
 
   if (warp == 4) {
     const bool leader = elect_one();
@@ -158,31 +169,45 @@ __global__ void __launch_bounds__(kRowsThreads) linear_rows_kernel(const __grid_
     __syncwarp();
     mbar_wait(&bars->drain, 0, kLinearWaitError);
   } else {
-    // the groups' factors: a token's scales are consecutive
+    // the tokens' scales, all in flight at once; a token's are consecutive
     for (int i = tid; i < NT * groups; i += 128) {
       const int t = i / groups, g = i - t * groups;
-      const float sw = __ldg(a.w_scales + static_cast<int64_t>(tile) * groups_all + g0 + g);
-      factor[g * NT + t] = t0 + t < a.rows ? __ldg(a.x_scales + static_cast<int64_t>(t0 + t) * groups_all + g0 + g) * sw : 0.0f;
+      if (t0 + t < a.rows) copy4_async(scale + g * NT + t, a.x_scales + static_cast<int64_t>(t0 + t) * groups_all + g0 + g);
+      else scale[g * NT + t] = 0.0f;
     }
+    const float* w_scale = a.w_scales + static_cast<int64_t>(tile) * groups_all + g0;
+    float next_w = groups > 0 ? __ldg(w_scale) : 0.0f;
+    copies4_wait();
     named_barrier_sync(1, 128);
     const uint32_t my_lanes = static_cast<uint32_t>(warp * kWarp) << 16;
     for (int i = 0; i < groups; ++i) {
       const int b = i % Shape::kBufs;
+      const float sw = next_w;
+      if (i + 1 < groups) next_w = __ldg(w_scale + i + 1);
       if (!warp_wait(&bars->sum_full[b], (i / Shape::kBufs) & 1, abort)) break;
       tc_fence_after();
-      const float4* f4 = reinterpret_cast<const float4*>(factor + i * NT);
+      const float* f = scale + i * NT + lane % 4 * 2;
+      constexpr int kAtOnce = NT < 64 ? NT : 64;
 #pragma unroll
-      for (int c = 0; c < NT; c += 16) {
-        uint32_t d[16];
-        tmem_ld16(tmem + my_lanes + b * NT + c, d);
+      for (int c = 0; c < NT; c += kAtOnce) {
+        uint32_t d[kAtOnce / 16][2][8];
+#pragma unroll
+        for (int j = 0; j < kAtOnce; j += 16) {
+          tmem_ld16x16(tmem + my_lanes + b * NT + c + j, d[j / 16][0]);
+          tmem_ld16x16(tmem + my_lanes + (16u << 16) + b * NT + c + j, d[j / 16][1]);
+        }
         tmem_ld_wait();
 #pragma unroll
-        for (int j = 0; j < 16; j += 4) {
-          const float4 f = f4[(c + j) / 4];
-          acc[c + j] = fmaf(__uint_as_float(d[j]), f.x, acc[c + j]);
-          acc[c + j + 1] = fmaf(__uint_as_float(d[j + 1]), f.y, acc[c + j + 1]);
-          acc[c + j + 2] = fmaf(__uint_as_float(d[j + 2]), f.z, acc[c + j + 2]);
-          acc[c + j + 3] = fmaf(__uint_as_float(d[j + 3]), f.w, acc[c + j + 3]);
+        for (int j = 0; j < kAtOnce; j += 8) {
+          float2 s = *reinterpret_cast<const float2*>(f + c + j);
+          s = make_float2(s.x * sw, s.y * sw);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float* sum = acc[(c + j) / 16][h] + j % 16 / 2;
+            const uint32_t* v = d[j / 16][h] + j % 16 / 2;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) sum[q] = fmaf(__uint_as_float(v[q]), q % 2 ? s.y : s.x, sum[q]);
+          }
         }
       }
       tc_fence_before();
@@ -195,41 +220,49 @@ __global__ void __launch_bounds__(kRowsThreads) linear_rows_kernel(const __grid_
   tc_fence_after();
   if (warp == 5) tmem_dealloc(tmem, Shape::kCols);
 
-  O* out = static_cast<O*>(a.out);
-  if (splits == 1) {
-    const int64_t n = n0 + tid;
-    if (tid < 128 && n < a.outs) {
-#pragma unroll
-      for (int j = 0; j < NT; ++j)
-        if (t0 + j < a.rows) out[(t0 + j) * a.outs + n] = from_float<O>(acc[j]);
-    }
-    return;
-  }
-  // the cluster's sums: each CTA's [NT][128] in its own shared memory (the
-  // pipeline's, now idle), a share of the tokens added up by each
+  // each CTA's sums [NT][128] in its own shared memory (the pipeline's, now idle), a share of the tokens added up
+  // by each CTA of the cluster
   float* part = reinterpret_cast<float*>(smem);
-  if (tid < 128) {
+  if (warp < 4) {
+    float* at = part + lane % 4 * 2 * kSumStride + warp * kWarp + lane / 4;
 #pragma unroll
-    for (int j = 0; j < NT; ++j) part[j * 128 + tid] = acc[j];
+    for (int c = 0; c < NT; c += 16)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int q = 0; q < 8; ++q) at[(c + q / 4 * 8 + q % 2) * kSumStride + h * 16 + q / 2 % 2 * 8] = acc[c / 16][h][q];
   }
-  cluster_sync();
+  if (splits > 1) cluster_sync();
+  else __syncthreads();
+  O* out = static_cast<O*>(a.out);
+  const bool whole = a.outs % 4 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15u) == 0;
   for (int i = tid; i < NT * 32 / splits; i += kRowsThreads) {
     const int e = i + rank * (NT * 32 / splits), t = e / 32, c = (e % 32) * 4;
-    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int r = 0; r < splits; ++r) {
-      const float4 v = ld_cluster(part + t * 128 + c, r);
-      sum.x += v.x;
-      sum.y += v.y;
-      sum.z += v.z;
-      sum.w += v.w;
+    if (t0 + t >= a.rows || n0 + c >= a.outs) continue;
+    float4 sum = *reinterpret_cast<const float4*>(part + t * kSumStride + c);
+    if (splits > 1) {
+      sum = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int r = 0; r < splits; ++r) {
+        const float4 v = ld_cluster(part + t * kSumStride + c, r);
+        sum.x += v.x;
+        sum.y += v.y;
+        sum.z += v.z;
+        sum.w += v.w;
+      }
     }
-    if (t0 + t >= a.rows) continue;
-    const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+    struct alignas(4 * sizeof(O)) Four {
+      O v[4];
+    } o{{from_float<O>(sum.x), from_float<O>(sum.y), from_float<O>(sum.z), from_float<O>(sum.w)}};
+    O* to = out + static_cast<int64_t>(t0 + t) * a.outs + n0 + c;
+    if (whole) {
+      *reinterpret_cast<Four*>(to) = o;
+    } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (n0 + c + j < a.outs) out[(t0 + t) * a.outs + n0 + c + j] = from_float<O>(v[j]);
+      for (int j = 0; j < 4; ++j)
+        if (n0 + c + j < a.outs) to[j] = o.v[j];
+    }
   }
-  cluster_sync();  // nobody leaves while its sums are being read
+  if (splits > 1) cluster_sync();  // nobody leaves while its sums are being read
 }
 
 // ----------------------------------------------------------------- many rows
@@ -504,7 +537,7 @@ cudaError_t launch_rows(const LinearArgs& a, cudaStream_t stream) {
   const int max_groups = static_cast<int>(ceil_div(groups, splits));
   auto kernel = linear_rows_kernel<O, NT>;
   const size_t smem = rows_smem<NT>(max_groups);
-  if (smem > 232448) return launch_tiles<O>(a, stream);  // the factors of so many groups do not fit
+  if (smem > 232448) return launch_tiles<O>(a, stream);  // the scales of so many groups do not fit
   cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   if (err != cudaSuccess) return err;
   cudaLaunchConfig_t config{};
@@ -569,9 +602,9 @@ cudaError_t launch_linear(const LinearArgs& a, cudaStream_t stream) {
   if (a.rows <= 16) return launch_rows<O, 16>(a, stream);
   if (a.rows <= 32) return launch_rows<O, 32>(a, stream);
   if (a.rows <= 64) return launch_rows<O, 64>(a, stream);
-  // weight streaming while its CTAs can still share a group range in twos: 128 x 7168 x 2048 12.5 us against 20.5 in
-  // tiles, 300 x 2112 x 7168 24.8 against 29.7; beyond that tiles: 600 x 2112 x 7168 30 against 43, 300 x 7168 x 7168
-  // 33 against 76
+  // weight streaming while its CTAs can still share a group range in twos: 128 x 7168 x 2048 11.8 us against 20.5 in
+  // tiles, 300 x 2112 x 7168 22.3 against 27.1; beyond that tiles: 600 x 2112 x 7168 28 against 35, 300 x 7168 x 7168
+  // 32 against 66
   if (2 * ceil_div(a.rows, 128) * ceil_div(a.outs, 128) <= gemv_grid_ctas()) return launch_rows<O, 128>(a, stream);
   return launch_tiles<O>(a, stream);
 }
