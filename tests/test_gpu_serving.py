@@ -138,6 +138,16 @@ def test_linear_large():
     assert torch.equal(out, serving.fp8_block_linear(*args))  # sums do not depend on who comes first
 
 
+@pytest.mark.parametrize("rows,outs,cols", [(100, 1003, 4096), (64, 5001, 640), (9, 387, 2064), (300, 1030, 1000)])
+def test_linear_few_rows_of_odd_outputs(rows, outs, cols):
+    """Outputs that are not stored four at a time, with a cluster's sums and without."""
+    args = _linear_inputs(rows, outs, cols)
+    for dtype in (bf16, f32):
+        out = serving.fp8_block_linear(*args, out_dtype=dtype)
+        _check_linear(out, *args)
+        assert torch.equal(out, serving.fp8_block_linear(*args, out_dtype=dtype))
+
+
 def test_linear_strides_and_shapes():
     codes, scales, w, ws = _linear_inputs(24, 200, 300)
     want = serving.fp8_block_linear(codes, scales, w, ws)
@@ -229,6 +239,19 @@ def test_append_out_of_range_is_skipped():
     assert _error_word() == 0
 
 
+@pytest.mark.parametrize("tokens,heads,latent,rope", [(1000, 130, 512, 64), (1500, 5, 72, 16), (2000, 33, 40, 10), (900, 1, 16, 280)])
+def test_append_many_tokens(tokens, heads, latent, rope):
+    """More tokens than CTAs, whose next tokens are read ahead; more heads than a CTA turns at once."""
+    kv, w, cache, slots, pos, cos, sin, q = _append_case(tokens, heads, latent, rope, 16, bf16, bf16)
+    before = cache.clone()
+    q_out = serving.paged_mla_append(kv, w, cache, slots, pos, cos, sin, eps=1e-6, q_pe=q)
+    _check_append(before, cache, q_out, kv, w, slots, pos, cos, sin, q)
+    lost = pos.clone()
+    lost[slots < 0] = 1 << 40  # rows to leave out, without a place in the sequence: zeros, and no error
+    q_lost = serving.paged_mla_append(kv, w, cache, slots, lost, cos, sin, eps=1e-6, q_pe=q)
+    assert not q_lost[slots < 0].any() and torch.equal(q_lost[slots >= 0], q_out[slots >= 0])
+
+
 def test_append_no_tokens():
     kv, w, cache, slots, pos, cos, sin, q = _append_case(4, 2, 64, 16, 8, f16, f16)
     before = cache.clone()
@@ -290,6 +313,15 @@ def test_attention_page_sizes(latent, page):
     case = _attn_case([300, 129, 0, 64], 70, latent, 64, page, bf16)
     out, lse = serving.paged_mla_attention(*case[:5], softmax_scale=case[5], return_lse=True)
     _check_attn(out, lse, case)
+
+
+@pytest.mark.parametrize("lengths,heads,latent", [([190, 64, 3, 0] * 20, 37, 512), ([700, 129] * 8, 130, 512), ([1, 400, 260] * 15, 41, 72)])
+def test_attention_many_rows_of_odd_heads(lengths, heads, latent):
+    """Parts joined four heads at a time, of which the last do not exist."""
+    case = _attn_case(lengths, heads, latent, 64, 32, f16)
+    out, lse = serving.paged_mla_attention(*case[:5], softmax_scale=case[5], return_lse=True)
+    _check_attn(out, lse, case)
+    assert torch.equal(out, serving.paged_mla_attention(*case[:5], softmax_scale=case[5]))
 
 
 @pytest.mark.parametrize("spread", [0.0, 40.0])
