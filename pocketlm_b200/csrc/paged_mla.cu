@@ -643,7 +643,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttnThreads, 1)
       if (leader) pair_umma_commit(&bars->drain);
       __syncwarp();
     }
-    mbar_wait(&bars->drain, 0, kPagedWaitError);  // in both CTAs: every product is complete
   } else {
     // ------------------------------------------------- softmax and result
     const float c2 = fmaxf(a.scale * kLog2e, 1e-37f);  // above 0: a masked score's -inf stays one
@@ -801,6 +800,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAttnThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
+  // in both CTAs: every product is complete.  Only now, after the CTA's own work: the second one's products
+  // warp has none, and a wait from its start on would bound the whole call, not a lack of progress.
+  if (warp == kProductsWarp) {
+    mbar_wait(&bars->drain, 0, kPagedWaitError);
+    __syncwarp();
+  }
   cluster_sync();  // nobody leaves while the other CTA may still signal or read here
   tc_fence_after();
   if (warp == kProductsWarp) pair_tmem_dealloc(tmem, 512);
