@@ -409,7 +409,6 @@ __global__ void __launch_bounds__(kTilesThreads, 1)
         if (leader) commit(&bars->drain);
         __syncwarp();
       }
-      mbar_wait(&bars->drain, 0, kLinearWaitError);  // in both CTAs: every product is complete
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
@@ -501,6 +500,12 @@ __global__ void __launch_bounds__(kTilesThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
+  // in both CTAs: every product is complete.  Only now, after the CTA's own work: the second one's products
+  // warps have none, and a wait from their start on would bound the whole call, not a lack of progress.
+  if (warp == kSumWarps + 1) {
+    mbar_wait(&bars->drain, 0, kLinearWaitError);
+    __syncwarp();
+  }
   if (PAIR) cluster_sync();  // nobody leaves while the other CTA may still signal or read here
   tc_fence_after();
   if (warp == kSumWarps + 1) {

@@ -69,3 +69,26 @@ def test_attention_longer_than_a_wait(cuda_device):
     off, lse_off = (out.double() - want).abs(), (lse.double() - want_lse - math.log(turns)).abs()
     assert bool((off <= tol + 9 * more * values).all())
     assert bool((lse_off <= lse_tol + more + 2 * oracle.F32 * math.log(turns)).all())
+
+
+def test_linear_longer_than_a_wait(cuda_device):
+    """Codes and weight in the same memory, all 1, and scales that add up to 1: outputs of 1."""
+    _room(72)
+    cols, most = 409600, 98304
+    codes = torch.full((most, cols), 0x38, dtype=torch.uint8, device="cuda")  # 1 in e4m3
+    blocks = cols // 128
+    scales = torch.full((most, blocks), 2.0 ** -7, device="cuda")
+    scale_inv = torch.full((most // 128, blocks), 1 / blocks, device="cuda")
+
+    def call(rows):
+        return serving.fp8_block_linear(codes[:rows], scales[:rows], codes, scale_inv)
+
+    _error_word()
+    _, ms = _timed(lambda: call(8192))
+    rows = min(most, math.ceil(32 * 1.3 * LIMIT_MS / ms) * 256)  # whole tiles of a pair of CTAs
+    out, ms = _timed(lambda: call(rows))
+    print(f"{rows} rows: {ms:.0f} ms")
+    assert ms > LIMIT_MS  # a shorter call shows nothing
+    assert _error_word() == 0
+    # 3200 groups whose sums are 128, exactly, times 2^-7 / 3200, rounded, added in fp32 to at most 1; then bf16's rounding
+    assert bool(((out.float() - 1).abs() <= blocks * 2 * oracle.F32 + oracle.half(torch.bfloat16)).all())
