@@ -594,6 +594,11 @@ int moe_fp8_quantize_rows(const void* x, int64_t x_stride, int x_dtype, int64_t 
 int moe_fp8_block_linear(const uint8_t* x_codes, int64_t x_stride, const float* x_scales, const uint8_t* fp8_weight,
                          int64_t weight_stride, const float* scale_inv, int64_t rows, int64_t out_rows,
                          int64_t in_cols, void* out, int out_dtype, void* stream);
+/* The tile of the kernel that the call above runs for these dimensions on the
+ * current device, 1000 * tokens + outputs: 16128 to 128128 stream the weight
+ * past 16 to 128 tokens, 256192 to 256256 are tiles of a pair of CTAs, 128256
+ * of one CTA; 0 without rows, negative for dimensions the call rejects. */
+int moe_fp8_block_linear_tile(int64_t rows, int64_t out_rows, int64_t in_cols);
 
 /* Token t's cache row [RMSNorm(kv[:kv_lora_rank]) * kv_norm_weight,
  * rot(kv[kv_lora_rank:], positions[t])] to slot slots[t] = page * page_size +

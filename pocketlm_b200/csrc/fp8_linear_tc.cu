@@ -526,8 +526,20 @@ bool encode_codes(CUtensorMap* map, const uint8_t* base, int64_t rows, int64_t c
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename O>
-cudaError_t launch_tiles(const LinearArgs& a, cudaStream_t stream);
+// How many CTAs share a weight tile's groups: the largest cluster that keeps at least two groups per CTA and all
+// CTAs resident at once (1 x 576 x 1536, 12 groups: clusters of eight 4.7 us, of four, as here, 4.7, of two 5.6).
+template <int NT>
+int rows_splits(const LinearArgs& a) {
+  const int64_t tiles = ceil_div(a.outs, 128), groups = ceil_div(a.cols, kGroup), token_tiles = ceil_div(a.rows, NT);
+  int splits = 1;
+  while (splits < 8 && tiles * token_tiles * splits * 2 <= RowsShape<NT>::kPerSm * gemv_grid_ctas() && groups >= splits * 4) splits *= 2;
+  return splits;
+}
+// Shared memory of a CTA, with the scales of all of its groups.
+template <int NT>
+size_t rows_smem_of(const LinearArgs& a) {
+  return rows_smem<NT>(static_cast<int>(ceil_div(ceil_div(a.cols, kGroup), rows_splits<NT>(a))));
+}
 
 template <typename O, int NT>
 cudaError_t launch_rows(const LinearArgs& a, cudaStream_t stream) {
@@ -535,14 +547,9 @@ cudaError_t launch_rows(const LinearArgs& a, cudaStream_t stream) {
   if (!encode_codes(&mx, a.x, a.rows, a.cols, a.x_stride, NT) || !encode_codes(&mw, a.w, a.outs, a.cols, a.w_stride, 128))
     return cudaErrorInvalidValue;
   const int64_t tiles = ceil_div(a.outs, 128), groups = ceil_div(a.cols, kGroup), token_tiles = ceil_div(a.rows, NT);
-  // the largest cluster that keeps at least two groups per CTA and all CTAs resident at once (1 x 576 x 1536,
-  // 12 groups: clusters of eight 4.7 us, of four, as here, 4.7, of two 5.6)
-  int splits = 1;
-  while (splits < 8 && tiles * token_tiles * splits * 2 <= RowsShape<NT>::kPerSm * gemv_grid_ctas() && groups >= splits * 4) splits *= 2;
-  const int max_groups = static_cast<int>(ceil_div(groups, splits));
+  const int splits = rows_splits<NT>(a), max_groups = static_cast<int>(ceil_div(groups, splits));
   auto kernel = linear_rows_kernel<O, NT>;
-  const size_t smem = rows_smem<NT>(max_groups);
-  if (smem > 232448) return launch_tiles<O>(a, stream);  // the scales of so many groups do not fit
+  const size_t smem = rows_smem_of<NT>(a);
   cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   if (err != cudaSuccess) return err;
   cudaLaunchConfig_t config{};
@@ -590,28 +597,46 @@ cudaError_t launch_tiles_n(const LinearArgs& a, cudaStream_t stream) {
 // pairs, the last one all but empty) or 512 of 224 (7 rounds, each an eighth
 // shorter); 600 x 7168 are 140 tiles of one CTA and 256 (one round).  Narrower
 // tiles of one CTA were slower than a pair's (300 x 7168 x 2048: 22 us against 16).
-template <typename O>
-cudaError_t launch_tiles(const LinearArgs& a, cudaStream_t stream) {
+LinearTile many_rows_tile(const LinearArgs& a) {
   auto cost = [&](int64_t tn, int64_t ctas) {
     return ceil_div(ceil_div(a.rows, ctas * kTileM) * ceil_div(a.outs, tn), gemv_grid_ctas() / ctas) * tn;
   };
   const int64_t least = std::min({cost(256, 2), cost(224, 2), cost(192, 2), cost(256, 1)});
-  if (cost(256, 2) == least) return launch_tiles_n<O, 256, true>(a, stream);
-  if (cost(224, 2) == least) return launch_tiles_n<O, 224, true>(a, stream);
-  if (cost(192, 2) == least) return launch_tiles_n<O, 192, true>(a, stream);
-  return launch_tiles_n<O, 256, false>(a, stream);
+  if (cost(256, 2) == least) return {2 * kTileM, 256};
+  if (cost(224, 2) == least) return {2 * kTileM, 224};
+  if (cost(192, 2) == least) return {2 * kTileM, 192};
+  return {kTileM, 256};
+}
+
+LinearTile tile_of(const LinearArgs& a) {
+  constexpr size_t kMost = 232448;  // where the scales do not fit beside the pipeline: tiles, which read them as they go
+  if (a.rows <= 16) return rows_smem_of<16>(a) <= kMost ? LinearTile{16, 128} : many_rows_tile(a);
+  if (a.rows <= 32) return rows_smem_of<32>(a) <= kMost ? LinearTile{32, 128} : many_rows_tile(a);
+  if (a.rows <= 64) return rows_smem_of<64>(a) <= kMost ? LinearTile{64, 128} : many_rows_tile(a);
+  // weight streaming while its CTAs can still share a group range in twos: 128 x 7168 x 2048 11.8 us against 20.5 in
+  // tiles, 300 x 2112 x 7168 22.3 against 27.1; beyond that tiles: 600 x 2112 x 7168 28 against 35, 300 x 7168 x 7168
+  // 32 against 66
+  if (2 * ceil_div(a.rows, 128) * ceil_div(a.outs, 128) <= gemv_grid_ctas() && rows_smem_of<128>(a) <= kMost) return {128, 128};
+  return many_rows_tile(a);
 }
 
 template <typename O>
 cudaError_t launch_linear(const LinearArgs& a, cudaStream_t stream) {
-  if (a.rows <= 16) return launch_rows<O, 16>(a, stream);
-  if (a.rows <= 32) return launch_rows<O, 32>(a, stream);
-  if (a.rows <= 64) return launch_rows<O, 64>(a, stream);
-  // weight streaming while its CTAs can still share a group range in twos: 128 x 7168 x 2048 11.8 us against 20.5 in
-  // tiles, 300 x 2112 x 7168 22.3 against 27.1; beyond that tiles: 600 x 2112 x 7168 28 against 35, 300 x 7168 x 7168
-  // 32 against 66
-  if (2 * ceil_div(a.rows, 128) * ceil_div(a.outs, 128) <= gemv_grid_ctas()) return launch_rows<O, 128>(a, stream);
-  return launch_tiles<O>(a, stream);
+  const LinearTile tile = tile_of(a);
+  if (tile.outs == 128) {
+    switch (tile.tokens) {
+      case 16: return launch_rows<O, 16>(a, stream);
+      case 32: return launch_rows<O, 32>(a, stream);
+      case 64: return launch_rows<O, 64>(a, stream);
+      default: return launch_rows<O, 128>(a, stream);
+    }
+  }
+  if (tile.tokens == kTileM) return launch_tiles_n<O, 256, false>(a, stream);
+  switch (tile.outs) {
+    case 256: return launch_tiles_n<O, 256, true>(a, stream);
+    case 224: return launch_tiles_n<O, 224, true>(a, stream);
+    default: return launch_tiles_n<O, 192, true>(a, stream);
+  }
 }
 
 }  // namespace
@@ -622,6 +647,12 @@ cudaError_t launch_fp8_linear(const LinearArgs& a, int out_dtype, cudaStream_t s
     case kDtypeBF16: return launch_linear<__nv_bfloat16>(a, stream);
     default: return launch_linear<__half>(a, stream);
   }
+}
+
+LinearTile fp8_linear_tile(int64_t rows, int64_t outs, int64_t cols) {
+  LinearArgs a{};
+  a.rows = rows; a.outs = outs; a.cols = cols;
+  return tile_of(a);
 }
 
 int read_and_clear_linear_error(cudaStream_t stream) { return read_and_clear_local_error(stream); }

@@ -36,6 +36,12 @@ struct LinearArgs {
   void* out;              // [rows, outs]
   int64_t rows, outs, cols, x_stride, w_stride;
 };
+// The kernel that a call takes: weight streaming with 128 outputs and 16 to 128 tokens per CTA, or tiles of
+// 192 to 256 outputs and 256 tokens (a pair of CTAs) or 128 (one).
+struct LinearTile {
+  int tokens, outs;
+};
+LinearTile fp8_linear_tile(int64_t rows, int64_t outs, int64_t cols);
 cudaError_t launch_fp8_linear(const LinearArgs& a, int out_dtype, cudaStream_t stream);
 int read_and_clear_linear_error(cudaStream_t stream);
 

@@ -49,14 +49,27 @@ int moe_fp8_quantize_rows(const void* x, int64_t x_stride, int x_dtype, int64_t 
   return kOk;
 }
 
+static int linear_supported(int64_t rows, int64_t out_rows, int64_t in_cols) {
+  if (rows < 0 || out_rows <= 0 || in_cols <= 0) return fail(kBadDims, "bad dimensions");
+  if (rows > INT32_MAX - 256 || out_rows > INT32_MAX - 256 || in_cols > INT32_MAX - 256)
+    return fail(kUnsupported, "a dimension beyond 32 bits");
+  return kOk;
+}
+
+int moe_fp8_block_linear_tile(int64_t rows, int64_t out_rows, int64_t in_cols) {
+  const int code = linear_supported(rows, out_rows, in_cols);
+  if (code != kOk || rows == 0) return code;
+  const LinearTile t = fp8_linear_tile(rows, out_rows, in_cols);
+  return t.tokens * 1000 + t.outs;
+}
+
 int moe_fp8_block_linear(const uint8_t* x_codes, int64_t x_stride, const float* x_scales, const uint8_t* fp8_weight,
                          int64_t weight_stride, const float* scale_inv, int64_t rows, int64_t out_rows,
                          int64_t in_cols, void* out, int out_dtype, void* stream) {
   if (!x_codes || !x_scales || !fp8_weight || !scale_inv || !out) return fail(kNullPointer, "null pointer");
-  if (rows < 0 || out_rows <= 0 || in_cols <= 0 || x_stride < in_cols || weight_stride < in_cols)
-    return fail(kBadDims, "bad dimensions");
-  if (rows > INT32_MAX - 256 || out_rows > INT32_MAX - 256 || in_cols > INT32_MAX - 256)
-    return fail(kUnsupported, "a dimension beyond 32 bits");
+  const int code = linear_supported(rows, out_rows, in_cols);
+  if (code != kOk) return code;
+  if (x_stride < in_cols || weight_stride < in_cols) return fail(kBadDims, "bad dimensions");
   if (!is_type(out_dtype)) return fail(kUnsupported, "the output is fp32, bf16 or fp16");
   if (((reinterpret_cast<uintptr_t>(x_codes) | reinterpret_cast<uintptr_t>(fp8_weight)) & 15u) || x_stride % 16 ||
       weight_stride % 16)

@@ -157,6 +157,7 @@ _SIGNATURES: dict[str, tuple[list, object]] = {
     "moe_rmsnorm_fp8": ([_P, _I64, _INT, _P, _I64, _P, _INT, _I64, _I64, _F32, _P, _I64, _P, _P, _P, _P], _INT),
     "moe_fp8_quantize_rows": ([_P, _I64, _INT, _I64, _I64, _P, _I64, _P, _P], _INT),
     "moe_fp8_block_linear": ([_P, _I64, _P, _P, _I64, _P, _I64, _I64, _I64, _P, _INT, _P], _INT),
+    "moe_fp8_block_linear_tile": ([_I64] * 3, _INT),
     "moe_paged_mla_append": ([_P, _I64, _INT, _P, _INT, _P, _P, _P, _P, _I64, _P, _INT, _I64, _I64, _I64, _I64, _P,
                               _I64, _I64, _I64, _P, _I64, _I64, _I64, _F32, _P], _INT),
     "moe_paged_mla_attention_workspace_bytes": ([_I64] * 6, _I64),

@@ -11,6 +11,7 @@ import torch
 
 import serving_oracle as oracle
 from pocketlm_b200 import native, serving
+from test_serving_host import LINEAR_TILES
 
 pytestmark = pytest.mark.gpu
 
@@ -173,6 +174,50 @@ def test_linear_nan_codes_stay_in_their_rows():
     assert bool(out[3].all()) and bool(out[:, 100].all())
     out[3], out[:, 100] = False, False
     assert not out.any()
+
+
+def _tile(rows, outs, cols):
+    return native.load_library().moe_fp8_block_linear_tile(rows, outs, cols)
+
+
+def _of_148_sms():
+    if torch.cuda.get_device_properties(0).multi_processor_count != 148:
+        pytest.skip("shapes chosen for the tiles that 148 SMs take")
+
+
+# outputs that are no multiple of a vector, a tile or a weight block, columns that end inside a group, a pair whose second CTA
+# has no tokens (rows % 256 up to 128), several tiles per CTA; and whole ones
+@pytest.mark.parametrize("dtype", [bf16, f16, f32])
+@pytest.mark.parametrize("tile,rows,outs,cols", LINEAR_TILES)
+def test_linear_every_tile(dtype, tile, rows, outs, cols):
+    _of_148_sms()
+    assert _tile(rows, outs, cols) == tile
+    args = _linear_inputs(rows, outs, cols)
+    out = serving.fp8_block_linear(*args, out_dtype=dtype)
+    _check_linear(out, *args)
+    assert torch.equal(out, serving.fp8_block_linear(*args, out_dtype=dtype))
+
+
+@pytest.mark.parametrize("rows,outs,cols", [(513, 5377, 333), (257, 7109, 515), (129, 4745, 333), (514, 6163, 333)])
+def test_linear_nan_codes_stay_in_their_rows_of_every_tile(rows, outs, cols):
+    codes, scales, w, ws = _linear_inputs(rows, outs, cols)
+    codes, w = codes.clone(), w.clone()
+    codes.view(torch.uint8)[rows - 1, cols - 1] = 0x7F
+    w.view(torch.uint8)[outs - 2, 5] = 0xFF
+    out = serving.fp8_block_linear(codes, scales, w, ws, out_dtype=f32).isnan()
+    assert bool(out[rows - 1].all()) and bool(out[:, outs - 2].all())
+    out[rows - 1], out[:, outs - 2] = False, False
+    assert not out.any()
+
+
+@pytest.mark.parametrize("rows,outs,cols", [(1, 3, 2225152), (17, 3, 1030144), (33, 5, 531456), (65, 130, 68608)])
+def test_linear_more_groups_than_scales_fit(rows, outs, cols):
+    """The longest rows whose scales stay in shared memory, and one column more."""
+    _of_148_sms()
+    assert _tile(rows, outs, cols) % 1000 == 128 and _tile(rows, outs, cols + 1) == 256192
+    for k in (cols, cols + 1):
+        args = _linear_inputs(rows, outs, k)
+        _check_linear(serving.fp8_block_linear(*args, out_dtype=f32), *args)
 
 
 # ----------------------------------------------------------------------- append

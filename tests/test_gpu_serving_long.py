@@ -89,6 +89,7 @@ def test_linear_longer_than_a_wait(cuda_device):
     out, ms = _timed(lambda: call(rows))
     print(f"{rows} rows: {ms:.0f} ms")
     assert ms > LIMIT_MS  # a shorter call shows nothing
+    assert native.load_library().moe_fp8_block_linear_tile(rows, most, cols) // 1000 == 256  # a pair's tiles
     assert _error_word() == 0
     # 3200 groups whose sums are 128, exactly, times 2^-7 / 3200, rounded, added in fp32 to at most 1; then bf16's rounding
     assert bool(((out.float() - 1).abs() <= blocks * 2 * oracle.F32 + oracle.half(torch.bfloat16)).all())

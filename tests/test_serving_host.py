@@ -120,3 +120,20 @@ def test_entry_point_codes():
     assert f(*_args(attn, tc=1 << 20, ps=1 << 11)) == -5 and f(*_args(attn, pages=(1 << 31) - 1)) == -5  # positions and pages past 32 bits
     assert lib.moe_paged_mla_attention_workspace_bytes(2, 3, 520, 16, 2, 8) == -1
     assert lib.moe_paged_mla_attention_workspace_bytes(2, 3, 64, 16, 2, 8) >= 0
+
+
+# shapes that reach every instance of the many-row linear, and the many tokens of weight streaming, on 148 SMs
+LINEAR_TILES = [
+    (256256, 513, 5377, 333), (256256, 2000, 2112, 1111), (256224, 257, 7109, 515), (256224, 385, 7168, 1024), (256224, 1500, 7171, 130),
+    (256192, 129, 4745, 333), (256192, 2000, 5000, 1111), (256192, 256, 7680, 384), (128256, 514, 6163, 333), (128256, 600, 7168, 700),
+    (128128, 100, 1003, 257), (128128, 300, 2112, 900)]
+
+
+def test_linear_tiles():
+    """Without a device the rule is that of 148 SMs."""
+    f = native.load_library().moe_fp8_block_linear_tile
+    if not torch.cuda.is_available():
+        for tile, rows, outs, cols in LINEAR_TILES:
+            assert f(rows, outs, cols) == tile
+    assert f(1, 2112, 7168) == 16128 and f(17, 130, 257) == 32128 and f(64, 1000, 1536) == 64128
+    assert f(0, 128, 128) == 0 and f(-1, 128, 128) == -2 and f(1, 0, 128) == -2 and f(1, 128, 1 << 31) == -5
