@@ -535,6 +535,23 @@ def test_a_decode_step(batch):
     assert far <= 2e-2
 
 
+@pytest.mark.parametrize("batch", [1, 5, 70])
+def test_what_a_decode_step_appends(batch):
+    """Each sequence's new row, by itself; every other row of the cache bit for bit as it was."""
+    step = _Step(batch)
+    before = step.cache.clone()
+    step.run()
+    want = step.plain()[2]
+    where = (step.slots // step.page, step.slots % step.page)
+    new, row = step.cache[where].double(), want[where].double()
+    # one linear of 8-bit codes lies before the row (2e-2 as above), and two roundings to 16 bits that may go apart by a step each
+    rel = (new - row).norm(dim=1) / row.norm(dim=1)
+    assert float(rel.max()) <= 2e-2 + 2 * 2 * oracle.half(bf16)
+    rest = step.cache.clone()
+    rest[where] = before[where]
+    assert torch.equal(rest, before)
+
+
 def test_a_decode_step_in_a_graph_and_on_another_stream():
     step = _Step(6)
     before = step.cache.clone()
