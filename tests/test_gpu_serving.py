@@ -369,6 +369,38 @@ def test_attention_many_rows_of_odd_heads(lengths, heads, latent):
     assert torch.equal(out, serving.paged_mla_attention(*case[:5], softmax_scale=case[5]))
 
 
+@pytest.mark.parametrize("batch,heads,page", [(257, 16, 16), (300, 129, 64), (600, 5, 7), (1030, 12, 32)])
+def test_attention_more_rows_than_threads(batch, heads, page):
+    """A thread adds up the tiles of several rows and finds its range's first one among them: long rows and long stretches of
+    rows without positions, at both ends and in between."""
+    lengths = [(37 * i) % 90 + 1 for i in range(batch)]
+    lengths[:9] = [0] * 9
+    lengths[60:140] = [0] * 80
+    lengths[140], lengths[batch - 2], lengths[batch - 1] = 2500, 1300, 0
+    case = _attn_case(lengths, heads, 64, 16, page, bf16)
+    out, lse = serving.paged_mla_attention(*case[:5], softmax_scale=case[5], return_lse=True)
+    _check_attn(out, lse, case)
+    assert torch.equal(out, serving.paged_mla_attention(*case[:5], softmax_scale=case[5]))
+
+
+def test_attention_most_rows():
+    """As many rows as a call takes.  A row of one tile is never cut, so that it does not depend on the rows beside it."""
+    batch, heads, latent, rope, page = 65535, 3, 64, 16, 16
+    g = _gen(9)
+    cache = _rnd(g, 1000, page, latent + rope).to(bf16)
+    table = torch.randint(0, 1000, (batch, 8), generator=g, device="cuda", dtype=torch.int32)
+    lengths = torch.randint(0, 129, (batch,), generator=g, device="cuda", dtype=torch.int32)
+    lengths[1000:3000] = 0
+    q = _rnd(g, batch, heads, latent + rope).to(bf16)
+    ql, qp = q[..., :latent].contiguous(), q[..., latent:].contiguous()
+    out, lse = serving.paged_mla_attention(ql, qp, cache, table, lengths, softmax_scale=0.1, return_lse=True)
+    for at in range(0, batch, 1000):
+        rows = slice(at, at + 200)
+        few, few_lse = serving.paged_mla_attention(ql[rows], qp[rows], cache, table[rows], lengths[rows], softmax_scale=0.1, return_lse=True)
+        assert torch.equal(out[rows], few) and torch.equal(lse[rows], few_lse)
+    _check_attn(out[-100:], lse[-100:], (ql[-100:], qp[-100:], cache, table[-100:], lengths[-100:], 0.1))
+
+
 @pytest.mark.parametrize("spread", [0.0, 40.0])
 def test_attention_flat_and_peaked(spread):
     """Equal scores, and scores of which one takes all (its maximum moving along the cache)."""
