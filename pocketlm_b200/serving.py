@@ -220,11 +220,12 @@ def paged_mla_append(kv_rows: torch.Tensor, kv_norm_weight: torch.Tensor, cache:
     code, kv_shape, table = _CODE[dtype], kv_rows.shape, rope_cos.shape
     if kv_norm_weight.ndim != 1 or len(table) != 2 or table != rope_sin.shape:
         raise ValueError("kv_norm_weight must be [latent], rope_cos and rope_sin [max_positions, rope / 2]")
-    latent, rope, tokens = kv_norm_weight.shape[0], 2 * table[1], kv_shape[0]
+    latent, rope = kv_norm_weight.shape[0], 2 * table[1]
     if len(kv_shape) != 2 or kv_shape[1] != width or latent + rope != width:
         raise ValueError("kv_rows, cache and norm weight sizes do not match")
     if latent == 0 or rope == 0 or table[0] == 0:
         raise ValueError("latent, rope and the tables must not be empty")
+    tokens = kv_shape[0]
     if slots.shape != (tokens,) or positions.shape != (tokens,):
         raise ValueError("slots and positions must be [tokens]")
     if slots.dtype != torch.int64 or positions.dtype != torch.int64:

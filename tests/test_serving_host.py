@@ -62,6 +62,15 @@ def test_append_refusals(change, match):
     _refused(match, serving.paged_mla_append, **{**_append_args(), **change})
 
 
+@pytest.mark.parametrize("name", [k for k, v in _append_args().items()])
+def test_append_refuses_other_numbers_of_dimensions(name):
+    given = _append_args()[name]
+    for bad in (given.new_zeros(()), given[None]):
+        with pytest.raises(ValueError) as refusal:
+            serving.paged_mla_append(**{**_append_args(), name: bad})
+        assert "CUDA device" not in str(refusal.value)  # not for where the tensors are
+
+
 def _attn_args(batch=2, heads=3, latent=64, rope=16, dtype=bf16):
     return dict(q_latent=torch.zeros(batch, heads, latent, dtype=dtype), q_pe=torch.zeros(batch, heads, rope, dtype=dtype),
                 cache=torch.zeros(4, 8, latent + rope, dtype=dtype), page_table=torch.zeros(batch, 2, dtype=i32),
