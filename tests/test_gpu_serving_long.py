@@ -14,6 +14,14 @@ pytestmark = pytest.mark.gpu
 LIMIT_MS = 2000.0
 
 
+@pytest.fixture(autouse=True)
+def _memory_goes_back(cuda_device):
+    """The tests behind these start processes of their own, which need the memory."""
+    torch.cuda.empty_cache()
+    yield
+    torch.cuda.empty_cache()
+
+
 def _timed(call):
     """What call() gives and the milliseconds that it takes on the device."""
     start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
@@ -29,12 +37,11 @@ def _error_word():
 
 
 def _room(gigabytes):
-    torch.cuda.empty_cache()
     if torch.cuda.mem_get_info()[0] < gigabytes << 30:
         pytest.skip(f"needs {gigabytes} GB")
 
 
-def test_attention_longer_than_a_wait(cuda_device):
+def test_attention_longer_than_a_wait():
     """Rows that walk the same sixteen pages over and over: the attention over the pages once, its lse higher by log(turns)."""
     _room(8)
     heads, page, cols, turns = 8, 64, 8192, 512
@@ -71,7 +78,7 @@ def test_attention_longer_than_a_wait(cuda_device):
     assert bool((lse_off <= lse_tol + more + 2 * oracle.F32 * math.log(turns)).all())
 
 
-def test_linear_longer_than_a_wait(cuda_device):
+def test_linear_longer_than_a_wait():
     """Codes and weight in the same memory, all 1, and scales that add up to 1: outputs of 1."""
     _room(72)
     cols, most = 409600, 98304
