@@ -590,7 +590,9 @@ int moe_fp8_quantize_rows(const void* x, int64_t x_stride, int x_dtype, int64_t 
  * per 128 columns, the weight [out_rows, in_cols] with 128 x 128 block
  * scales), products and sums in fp32, one rounding to out_dtype.  Code rows
  * start on 16-byte boundaries.  Unlike the fp32-activation linears above, the
- * codes 0x7F / 0xFF are NaN here, as e4m3 defines them. */
+ * codes 0x7F / 0xFF are NaN here, as e4m3 defines them.  The order of the sums
+ * goes by the dimensions: the same call gives the same bits, another number of
+ * rows may give a row other last bits. */
 int moe_fp8_block_linear(const uint8_t* x_codes, int64_t x_stride, const float* x_scales, const uint8_t* fp8_weight,
                          int64_t weight_stride, const float* scale_inv, int64_t rows, int64_t out_rows,
                          int64_t in_cols, void* out, int out_dtype, void* stream);
@@ -627,8 +629,11 @@ int moe_paged_mla_append(const void* kv_rows, int64_t kv_stride, int kv_dtype, c
  * zeros and -inf.  Several tokens of one sequence (a verify batch) are rows
  * that share a table row with lengths one apart.  Table entries at and past a
  * row's last page are not read.  A page outside [0, pages) or a length past
- * the table is skipped and sets code 512 in moe_b200_device_error.
- * kv_lora_rank <= 512 and qk_rope_dim <= 64, both multiples of 8; rows of
+ * the table is skipped and sets code 512 in moe_b200_device_error.  The
+ * probabilities are rounded to the cache's type before they multiply the
+ * latent rows; all else is fp32.  Where a row's positions are cut into parts
+ * goes by all rows' lengths: the same call gives the same bits, another batch
+ * may give a row other last bits.  kv_lora_rank <= 512 and qk_rope_dim <= 64, both multiples of 8; rows of
  * queries and cache start on 16-byte boundaries, strides positive; batch <=
  * 65535.  workspace (on a 32-byte boundary):
  * moe_paged_mla_attention_workspace_bytes (-1 for dimensions it rejects). */

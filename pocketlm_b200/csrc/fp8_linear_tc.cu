@@ -8,19 +8,25 @@
 // so a pipeline stage is one group of both operands, loaded by TMA as stored;
 // absent rows and columns arrive as zeros.
 //
-// Few rows (linear_rows_kernel): the weights' bytes bound it.  The weight's rows
+// Few rows (linear_rows_kernel).  The weight's rows
 // are M (128 of them per CTA), the tokens N (16 to 128), so no tensor work is
 // spent on absent tokens; the groups are cut over the CTAs of a cluster, whose
 // sums are added through distributed shared memory in rank order (the same
-// result on every run).  Measured: 64 x 24576 x 1536 12.7 us (41 MB, 3.2 TB/s),
-// 1 x 2112 x 7168 7.0 us: the launch, the first bytes' latency and the cluster's
-// sum are most of so short a call.
+// result on every run).  Measured at 1965 MHz: 64 x 24576 x 1536 13.4 us with the
+// weight from memory (41 MB, 3.1 TB/s), 11.5 from L2; 1 x 2112 x 7168 8.6 and 6.8 us.
+// Latency bounds it: the launch, the first bytes and the cluster's sum, then some
+// 0.6 us per group and CTA, from the load over the products to the sums, whether
+// the weight is in L2 or not.
 //
-// Many rows (linear_tiles_kernel): the tensor cores bound it.  256 tokens x up
+// Many rows (linear_tiles_kernel).  256 tokens x up
 // to 256 outputs per pair of CTAs and tile, two accumulators so that the sums
 // of one group are read while the next is computed; persistent.  Measured:
-// 4000 x 7168 x 16384 458 us, 2.05 PFLOP/s.  Its groups' sums bound it: 256 x 256
-// fp32 values leave tensor memory for every 520 cycles of products.
+// 4000 x 7168 x 16384 541 us in a loop of a second (1.74 PFLOP/s at the 1530 MHz
+// that the power limit leaves), 476 us after a rest.  A group of a 256 x 256 tile
+// takes 870 cycles, 520 of them products.  No unit is busy all the time (2000 x
+// 7168 x 7168: tensor cores 51 % of the cycles, tensor memory 47 %, issue slots
+// 51 %): the handing of two accumulators to and fro between products and sums,
+// and the power, bound it.
 #include <algorithm>
 
 #include "fp8_gemv.cuh"
@@ -273,7 +279,7 @@ __global__ void __launch_bounds__(kRowsThreads) linear_rows_kernel(const __grid_
 // cycles over the pair, of M = 128, N = 256 on one CTA 690).  Otherwise one CTA
 // takes 128 tokens x TN.  In both a group's sums must leave tensor memory every
 // 500 cycles, and the two come within a twentieth of each other per round of all
-// SMs (4000 x 7168 x 16384: 458 us in pairs, 483 alone); the finer tiles of one
+// SMs (4000 x 7168 x 16384, short runs: 458 us in pairs, 483 alone); the finer tiles of one
 // CTA fill the SMs where a pair's do not (600 x 7168 x 7168: 36 us against 63).
 constexpr int kTileM = 128;  // tokens per CTA
 constexpr int kSumWarps = 8;  // warp w: tokens 32 (w % 4) .. + 31, half w / 4 of the TN columns
@@ -527,7 +533,8 @@ bool encode_codes(CUtensorMap* map, const uint8_t* base, int64_t rows, int64_t c
 }
 
 // How many CTAs share a weight tile's groups: the largest cluster that keeps at least two groups per CTA and all
-// CTAs resident at once (1 x 576 x 1536, 12 groups: clusters of eight 4.7 us, of four, as here, 4.7, of two 5.6).
+// CTAs resident at once (1 x 576 x 1536, 12 groups, from L2: clusters of eight 4.7 us, of four, as here, 4.7, of
+// two 5.6).
 template <int NT>
 int rows_splits(const LinearArgs& a) {
   const int64_t tiles = ceil_div(a.outs, 128), groups = ceil_div(a.cols, kGroup), token_tiles = ceil_div(a.rows, NT);
@@ -609,13 +616,16 @@ LinearTile many_rows_tile(const LinearArgs& a) {
 }
 
 LinearTile tile_of(const LinearArgs& a) {
-  constexpr size_t kMost = 232448;  // where the scales do not fit beside the pipeline: tiles, which read them as they go
+  // Where the scales do not fit beside the pipeline: tiles, which read them as they go.  They are slower there (100 x
+  // 7168: 16384 columns 42 us, 18432, past the limit, 68).
+  constexpr size_t kMost = 232448;
   if (a.rows <= 16) return rows_smem_of<16>(a) <= kMost ? LinearTile{16, 128} : many_rows_tile(a);
   if (a.rows <= 32) return rows_smem_of<32>(a) <= kMost ? LinearTile{32, 128} : many_rows_tile(a);
   if (a.rows <= 64) return rows_smem_of<64>(a) <= kMost ? LinearTile{64, 128} : many_rows_tile(a);
-  // weight streaming while its CTAs can still share a group range in twos: 128 x 7168 x 2048 11.8 us against 20.5 in
-  // tiles, 300 x 2112 x 7168 22.3 against 27.1; beyond that tiles: 600 x 2112 x 7168 28 against 35, 300 x 7168 x 7168
-  // 32 against 66
+  // weight streaming while its CTAs can still share a group range in twos (from L2): 128 x 7168 x 2048 11.8 us against
+  // 20.5 in tiles, 300 x 2112 x 7168 22.3 against 27.1; beyond that tiles: 600 x 2112 x 7168 28 against 35, 300 x 7168 x
+  // 7168 32 against 66.  Over 24576 x 1536, weights from memory, where tiles begin at 65 rows: 64 rows 13.4 us, 65 rows
+  // 13.5, 128 rows 16, 300 rows 25.
   if (2 * ceil_div(a.rows, 128) * ceil_div(a.outs, 128) <= gemv_grid_ctas() && rows_smem_of<128>(a) <= kMost) return {128, 128};
   return many_rows_tile(a);
 }

@@ -13,9 +13,12 @@
 // Bytes bound both (a row is read once and kept in registers between the
 // mean and the codes).  Eight consecutive columns belong to a thread, so
 // sixteen neighbouring lanes hold a scale group and find its amax with four
-// shuffles.  Measured, bf16: 8192 x 7168 with the residual and the 16-bit rows
-// 88.8 us (530 MB, 6.0 TB/s), one row 3.1 us; 4096 x 16384 without a norm
-// 35.5 us (203 MB, 5.7 TB/s).
+// shuffles.  Measured, bf16, inputs from memory, 1965 MHz: 8192 x 7168 with the
+// residual and the 16-bit rows 89 us (530 MB, 5.9 TB/s), one row 3.4 us (2.8 from
+// L2); 4096 x 16384 without a norm 36 us (203 MB, 5.7 TB/s), 64 x 16384 3.2 us.
+// Where columns, a pointer or a row stride do not allow 16-byte accesses, every
+// array goes element by element: with rows of x one value longer the first takes
+// 390 us, 4096 x 16384 134 us.
 #include <algorithm>
 
 #include "fp8_gemv.cuh"
@@ -239,9 +242,9 @@ bool aligned(const void* p, int64_t bytes) { return reinterpret_cast<uintptr_t>(
 template <typename T, typename W, bool VEC>
 cudaError_t launch_norm(const NormArgs& a, cudaStream_t stream) {
   // No more rows than SMs: a thread per vector, the shortest way through a row
-  // (7168 columns, 1 row 3.1 us against 4.3, 148 rows 3.3 against 4.6).  More:
-  // four vectors per thread, more rows at once (296 rows 5.3 us against 5.7, 592
-  // 8.8 against 12.6).
+  // (7168 columns, inputs in L2, 1 row 3.1 us against 4.3, 148 rows 3.3 against
+  // 4.6).  More: four vectors per thread, more rows at once (296 rows 5.3 us
+  // against 5.7, 592 8.8 against 12.6).
   const int64_t vectors = ceil_div(a.cols, 8);
   const int v = vectors <= 1024 && a.rows <= gemv_grid_ctas() ? 1 : vectors <= 2048 ? 4 : 8;
   const int threads = static_cast<int>(ceil_div(ceil_div(vectors, v), 32) * 32);

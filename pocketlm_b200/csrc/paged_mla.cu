@@ -8,7 +8,8 @@
 // (cos[position, p], sin[position, p]).  fp32 throughout, one rounding to the
 // stored type.  Bytes bound it: every value is read once and written once; a
 // warp takes a token's cache row or 256 of its query values.  Measured with 128
-// heads: 4096 tokens 26.4 us (145 MB, 5.5 TB/s), 32 tokens 2.7 us.
+// heads, inputs from memory: 4096 tokens 26.6 us (145 MB, 5.4 TB/s), 32 tokens 3.6 us
+// (2.8 from L2).
 //
 // Attention.  score[l] = scale (q_latent . c[l] + q_pe . r[l]) over the row's
 // first `length` positions, position l in page table[l / page_size];
@@ -240,11 +241,13 @@ cudaError_t launch_append_types(const AppendArgs& a, int x_dtype, int norm_dtype
 // walks the work, so that operand descriptors stay in uniform registers; one
 // lane issues).
 //
-// Measured, bf16: 64 rows of 128 heads and up to 8192 positions 102 us (393 MB,
-// 3.9 TB/s; 91 GFLOP, 0.89 PFLOP/s): a tile of a pair takes some 2970 cycles, of
-// which its products keep the tensor cores 51 % busy, and the parts' results and
-// their join some 12 us.  One row of 4096 positions 16.7 us: launches, two tiles
-// per pair, and the join of its parts.
+// Measured, bf16, cache from memory: 64 rows of 128 heads and up to 8192 positions
+// 114 us in a loop of a second (393 MB, 3.5 TB/s; 91 GFLOP, 0.80 PFLOP/s, at the
+// 1700 MHz that the power limit leaves), 106 us after a rest.  A tile of a pair takes
+// some 3350 cycles, 2280 of them products, with 16 heads as with 128 and from
+// L2 as from memory; the parts' results and their join take some 12 us.  One row of
+// 4096 positions 18.8 us, 16.5 from L2: launches, two tiles per pair, and the join
+// of its parts.
 constexpr int kTile = 128, kHalfTile = 64;
 constexpr int kHeads = 128, kCtaHeads = 64;
 constexpr int kChunkBytes = 64 * 128;
@@ -257,7 +260,7 @@ constexpr int kSoftmaxWarps = 4, kSoftmaxThreads = kSoftmaxWarps * kWarp;
 constexpr int kKeysWarp = 4, kValuesWarp = 5, kProductsWarp = 7;
 constexpr int kAttnWarps = 8, kAttnThreads = kAttnWarps * kWarp;
 constexpr uint32_t kColO = 0, kColS = 256;
-constexpr int kMinTiles = 2;  // fewest tiles worth a range of their own: one row of 4096 positions 16.7 us, 1 would take 17.9
+constexpr int kMinTiles = 2;  // fewest tiles worth a range of their own: one row of 4096 positions, from L2, 16.7 us, 1 would take 17.9
 constexpr float kMovesBy = 8.0f;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 

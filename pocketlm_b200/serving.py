@@ -162,7 +162,8 @@ def fp8_block_linear(codes: torch.Tensor, scales: torch.Tensor, fp8_weight: torc
     codes [..., in] and scales [..., ceil(in / 128)] as rmsnorm_fp8 and quantize_fp8_rows give them; fp8_weight
     [out, in] e4m3 (or its bytes) and scale_inv [ceil(out / 128), ceil(in / 128)] as the checkpoints hold them.
     Sums in fp32, one rounding to out_dtype (bf16, fp16 or fp32).  NaN codes are NaN (the fp32-activation linears
-    of `native` read them as 0).  Rows that do not start on 16-byte boundaries are copied first."""
+    of `native` read them as 0).  Rows that do not start on 16-byte boundaries are copied first.  The sums' order goes
+    by the sizes, so that a row's last bits may be others beside more or fewer rows (never from run to run)."""
     if not (codes.dtype in _FP8 and fp8_weight.dtype in _FP8):
         raise ValueError("codes and fp8_weight must be e4m3")
     if not (scales.dtype == torch.float32 and scale_inv.dtype == torch.float32):
@@ -287,7 +288,11 @@ def paged_mla_attention(q_latent: torch.Tensor, q_pe: torch.Tensor, cache: torch
     (the new token included).  Returns [batch, heads, latent] in the queries' type, for W_UV, and with
     return_lse also log(sum exp(score)) fp32 [batch, heads].  A row of length 0 gives zeros (and -inf); entries of
     page_table past a row's last page are not read.  Several tokens of one sequence are rows with the same pages and
-    lengths one apart.  latent <= 512 and rope <= 64, multiples of 8; any page size."""
+    lengths one apart.  latent <= 512 and rope <= 64, multiples of 8; any page size.
+
+    Scores, sums and their parts are fp32; the probabilities are rounded to the cache's type before they multiply the
+    latent rows, half a step each.  Where a row's positions are cut into parts goes by all rows' lengths, so that its
+    last bits may be others in another batch (never from run to run)."""
     pages, page_size, width, dtype, strides = _cache_layout(cache)
     q_shape, pe_shape, table_shape = q_latent.shape, q_pe.shape, page_table.shape
     if len(q_shape) != 3 or len(pe_shape) != 3:
